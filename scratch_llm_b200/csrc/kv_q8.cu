@@ -1,0 +1,377 @@
+// Keys and values into a cache of 8-bit numbers, and back (q8.cuh says what such a cache holds).
+//
+// Write: rotary position encoding of q and k (32-bit angles and arithmetic, each product and each difference
+// rounded on its own), the turned queries into a buffer of their own, keys and values quantised as they are
+// stored.  The 8-bit form of rope_cache.cu, with its conventions: qkv [n_tokens, (H + 2G) * hd], q heads,
+// then k heads, then v heads; `bias` (may be null) added first; only the first `rot` entries of a head
+// turn, in pairs (2j, 2j + 1) or (j, j + rot / 2).  Row r brings the tokens row_start[r] .. row_start[r + 1] - 1, at
+// the positions from row_pos0[r] on; tokens behind the last row are left alone.
+//   pages  [n_pages, 2, G, page_size, hd]             e4m3
+//   scales [n_pages, 2, G, page_size / block]         e8m0
+// A block's scale comes from the values that this step stores in it and, where the row has stored earlier
+// tokens in it (positions before row_pos0[r]), from the scale that it has: it only grows, and then the
+// earlier tokens' numbers are rounded again at the new one.  What a block that starts with this step held
+// before is never looked at.
+#include "q8.cuh"
+
+namespace sllm {
+
+struct WriteArgs {
+    const int* row_start; const int* row_pos0;
+    const float* cos_t; const float* sin_t; const float* bias;
+    uint8_t* pages; uint8_t* scales; const int* table;
+    int table_stride, page_size, block, n_rows, n_tokens, H, G, hd, rot, interleaved, single;
+    int lanes;              // threads of a block of the cache: a power of two up to 32, or whole warps
+    int kv_ctas, q_groups;
+    int64_t n_tasks, n_q_items;
+};
+
+// a thread keeps up to 64 entries in registers
+constexpr int WRITE_THREADS = 512;
+template <int W> constexpr int WRITE_UNITS = 32 / W;
+
+// Unit u of a head: 2 W entries, W at e0 and W at e1; turned pairs are (e0 + i, e1 + i), or, where neighbours
+// pair, the pairs within 2 W neighbouring entries.  Entries that do not turn come 2 W neighbours at a time.
+template <int W> struct Unit {
+    int e0, e1, pair0;      // pair0: its first pair's column of the tables; -1 where it does not turn
+    __device__ __forceinline__ Unit(int u, int rot, int interleaved) {
+        const int n_turn = rot / (2 * W);
+        pair0 = u < n_turn ? W * u : -1;
+        if (u < n_turn && !interleaved) { e0 = W * u; e1 = rot / 2 + W * u; }
+        else { e0 = 2 * W * u; e1 = e0 + W; }
+    }
+};
+
+template <typename T, int W> __device__ __forceinline__ void load_w(const T* p, float* v) {
+    if constexpr (W == 1) v[0] = to_float(p[0]);
+    else {
+#pragma unroll
+        for (int i = 0; i < W; i += Vec<T>::N) Vec<T>::load(p + i, v + i);
+    }
+}
+template <typename T, int W> __device__ __forceinline__ void store_w(T* p, const float* v) {
+    if constexpr (W == 1) p[0] = from_float<T>(v[0]);
+    else {
+#pragma unroll
+        for (int i = 0; i < W; i += Vec<T>::N) Vec<T>::store(p + i, v + i);
+    }
+}
+
+template <int W>
+__device__ __forceinline__ void load_angles(const WriteArgs& a, const Unit<W>& u, int pos, float* c, float* s) {
+    if (u.pair0 < 0) return;
+    load_w<float, W>(a.cos_t + (int64_t)pos * (a.rot / 2) + u.pair0, c);
+    load_w<float, W>(a.sin_t + (int64_t)pos * (a.rot / 2) + u.pair0, s);
+}
+
+// One unit of a head: loaded, with the bias, turned.  v[0 .. W): the entries at e0, v[W .. 2 W): those at e1.
+template <typename T, int W>
+__device__ __forceinline__ void load_unit(const WriteArgs& a, const T* head, const float* bias, const Unit<W>& u,
+                                          bool turns, const float* c, const float* s, float* v) {
+    load_w<T, W>(head + u.e0, v);
+    load_w<T, W>(head + u.e1, v + W);
+    if (bias != nullptr) {
+        float b[2 * W];
+        load_w<float, W>(bias + u.e0, b);
+        load_w<float, W>(bias + u.e1, b + W);
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) v[i] = __fadd_rn(v[i], b[i]);
+    }
+    if (turns && u.pair0 >= 0) {
+        auto turn = [&](float& x0, float& x1, int i) {
+            const float y0 = __fsub_rn(__fmul_rn(x0, c[i]), __fmul_rn(x1, s[i]));
+            x1 = __fadd_rn(__fmul_rn(x0, s[i]), __fmul_rn(x1, c[i]));
+            x0 = y0;
+        };
+        if (a.interleaved) {      // (places in registers are known to the compiler either way)
+#pragma unroll
+            for (int i = 0; i < W; ++i) turn(v[2 * i], v[2 * i + 1], i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) turn(v[i], v[i + W], i);
+        }
+    }
+}
+
+// the row of token n: the last one that starts at or before it and is not empty
+__device__ __forceinline__ int row_of(const WriteArgs& a, int n) {
+    int lo = 0, hi = a.n_rows - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (a.row_start[mid] <= n) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// CTAs 0 .. kv_ctas - 1: a group of a.lanes threads takes one block of the cache (what a row stores in it), for
+// one plane and kv head.  Row r has the slots from row_start[r] / block + 2 r on, at least as many as it touches
+// blocks: n new tokens touch at most n / block + 2.  The other CTAs turn the queries.
+template <typename T, int W>
+__global__ void __launch_bounds__(WRITE_THREADS)
+rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const WriteArgs a) {
+    __shared__ float warp_top[WRITE_THREADS / 32];
+    pdl_wait();
+    pdl_trigger();
+    const int heads = a.H + 2 * a.G, upt = a.hd / (2 * W);
+    if ((int)blockIdx.x >= a.kv_ctas) {
+        // ---- queries: a thread takes a unit of a token and walks a share of the token's heads with it
+        const int per_group = (a.H + a.q_groups - 1) / a.q_groups;
+        for (int64_t i = (int64_t)(blockIdx.x - a.kv_ctas) * blockDim.x + threadIdx.x; i < a.n_q_items;
+             i += (int64_t)(gridDim.x - a.kv_ctas) * blockDim.x) {
+            const int u_ = (int)(i % upt);
+            const int64_t t = i / upt;
+            const int group = (int)(t % a.q_groups), n = (int)(t / a.q_groups);
+            if (n >= a.row_start[a.n_rows]) continue;
+            const int r = row_of(a, n), pos = a.row_pos0[r] + n - a.row_start[r];
+            const Unit<W> u(u_, a.rot, a.interleaved);
+            float c[W], s[W];
+            load_angles<W>(a, u, pos, c, s);
+            const int end = min(a.H, (group + 1) * per_group);
+#pragma unroll 2
+            for (int h = group * per_group; h < end; ++h) {
+                float v[2 * W];
+                load_unit<T, W>(a, qkv + ((int64_t)n * heads + h) * a.hd, a.bias ? a.bias + (int64_t)h * a.hd : nullptr,
+                                u, true, c, s, v);
+                T* to = q_out + ((int64_t)n * a.H + h) * a.hd;
+                store_w<T, W>(to + u.e0, v);
+                store_w<T, W>(to + u.e1, v + W);
+            }
+        }
+        return;
+    }
+    // ---- keys and values
+    const int lanes = a.lanes, in_cta = blockDim.x / lanes;
+    const int64_t task = (int64_t)blockIdx.x * in_cta + threadIdx.x / lanes;
+    const int lane = threadIdx.x % lanes;
+    const int pg = (int)(task % (2 * a.G)), plane = pg / a.G, g = pg - plane * a.G;
+    const int slot = (int)(task / (2 * a.G));
+    bool live = task < a.n_tasks;
+    int r = slot, at = 0;
+    if (live && !a.single) {
+        int lo = 0, hi = a.n_rows - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (a.row_start[mid] / a.block + 2 * mid <= slot) lo = mid; else hi = mid - 1;
+        }
+        r = lo;
+        at = slot - (a.row_start[r] / a.block + 2 * r);
+    }
+    int t0 = 0, pos0 = 0, n_old = 0, first = 0, count = 0;
+    if (live) {
+        t0 = a.row_start[r];
+        const int n_new = a.row_start[r + 1] - t0;
+        pos0 = a.row_pos0[r];
+        const int begin = (pos0 / a.block + at) * a.block;       // the block's first position
+        first = max(pos0, begin);
+        count = min(pos0 + n_new, begin + a.block) - first;
+        n_old = first - begin;
+        live = count > 0;
+    }
+    int page = -1, cell = 0, had = 0;
+    if (live) {
+        const int begin = first - n_old;
+        page = a.table[(int64_t)r * a.table_stride + begin / a.page_size];
+        cell = begin % a.page_size;
+        live = page >= 0;                                         // (no page, nothing to store)
+    }
+    const int64_t plane_of = ((int64_t)page * 2 + plane) * a.G + g;
+    uint8_t* scale = a.scales + (live ? plane_of * (a.page_size / a.block) + cell / a.block : 0);
+    if (live && n_old > 0) had = *scale;
+    const int head = a.H + pg;
+    const float* bias = a.bias ? a.bias + (int64_t)head * a.hd : nullptr;
+    constexpr int UNITS = WRITE_UNITS<W>;
+    float v[UNITS][2 * W], top = 0.f;
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k) {
+        const int i = lane + k * lanes, tok = i / upt;
+        if (!live || tok >= count) continue;
+        const Unit<W> u(i - tok * upt, a.rot, a.interleaved);
+        float c[W], s[W];
+        if (plane == 0) load_angles<W>(a, u, first + tok, c, s);
+        load_unit<T, W>(a, qkv + ((int64_t)(t0 + first - pos0 + tok) * heads + head) * a.hd, bias, u, plane == 0, c, s, v[k]);
+#pragma unroll
+        for (int j = 0; j < 2 * W; ++j) top = fmaxf(top, q8_finite(v[k][j]) ? fabsf(v[k][j]) : 0.f);
+    }
+    for (int o = min(lanes, 32) / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lanes > 32) {                                             // (the CTA is one group)
+        if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+        __syncthreads();
+        for (int w = 0; w < lanes / 32; ++w) top = fmaxf(top, warp_top[w]);
+    }
+    if (!live) return;
+    const int byte = max(q8_scale_byte(top), had);
+    const float inv = q8_inverse(byte);
+    uint8_t* cells = a.pages + (plane_of * a.page_size + cell) * a.hd;
+    if (n_old > 0 && byte > had) {
+        // the earlier tokens at the scale of now (hd is a multiple of 16, the tokens of a block are neighbours)
+        const float shift = q8_power(max(had, 1)) * inv;
+        for (int i = lane; i < n_old * a.hd / 16; i += lanes) {
+            uint4 x = *reinterpret_cast<uint4*>(cells + 16 * i);
+            uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 lo = q8_float2(w[k] & 0xffffu), hi = q8_float2(w[k] >> 16);
+                w[k] = q8_pack4(lo.x * shift, lo.y * shift, hi.x * shift, hi.y * shift);
+            }
+            *reinterpret_cast<uint4*>(cells + 16 * i) = x;
+        }
+    }
+    if (lane == 0) *scale = (uint8_t)byte;
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k) {
+        const int i = lane + k * lanes, tok = i / upt;
+        if (tok >= count) continue;
+        const Unit<W> u(i - tok * upt, a.rot, a.interleaved);
+        uint8_t* to = cells + (int64_t)(n_old + tok) * a.hd;
+        float x[2 * W];
+#pragma unroll
+        for (int j = 0; j < 2 * W; ++j) x[j] = q8_finite(v[k][j]) ? v[k][j] * inv : __int_as_float(0x7fffffff);
+        if constexpr (W == 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = q8_pack4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+            *reinterpret_cast<uint2*>(to + u.e0) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2*>(to + u.e1) = make_uint2(w[2], w[3]);
+        } else {
+            const uint32_t two = q8_pack2(x[0], x[1]);
+            to[u.e0] = (uint8_t)two;
+            to[u.e1] = (uint8_t)(two >> 8);
+        }
+    }
+}
+
+// The values of positions row_from[r] .. row_to[r] - 1 of every row, into pages of T through a table of their
+// own.  A page is one run of bytes; a thread takes READ_PIECES pieces of 16.  grid (pieces of a page, pages of a
+// row, rows).
+constexpr int READ_THREADS = 256, READ_PIECES = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(READ_THREADS)
+kv_read_q8_kernel(const uint8_t* __restrict__ pages, const uint8_t* __restrict__ scales, const int* __restrict__ table,
+                  int table_stride, const int* __restrict__ row_from, const int* __restrict__ row_to, T* __restrict__ out,
+                  const int* __restrict__ out_table, int out_stride, int page_size, int block, int G, int hd, int first_row) {
+    pdl_wait();
+    pdl_trigger();
+    const int r = first_row + blockIdx.z;
+    const int from = max(row_from[r], 0), to = row_to[r];
+    const int pieces = 2 * G * page_size * hd / 16;
+    for (int64_t p = from / page_size + (int64_t)blockIdx.y; p * page_size < to; p += gridDim.y) {
+        const int page = table[(int64_t)r * table_stride + p], out_page = out_table[(int64_t)r * out_stride + p];
+        if (page < 0 || out_page < 0) continue;
+        const uint8_t* src = pages + (int64_t)page * pieces * 16;
+        const uint8_t* sc = scales + (int64_t)page * (2 * G * (page_size / block));
+        T* dst = out + (int64_t)out_page * pieces * 16;
+        const int c0 = blockIdx.x * READ_THREADS * READ_PIECES + threadIdx.x;
+        uint4 x[READ_PIECES];
+        int b[READ_PIECES];
+#pragma unroll
+        for (int k = 0; k < READ_PIECES; ++k) {
+            const int c = c0 + k * READ_THREADS, row = c * 16 / hd;         // of the page's 2 G page_size rows
+            const int64_t pos = p * page_size + row % page_size;
+            b[k] = -1;
+            if (c < pieces && pos >= from && pos < to) {
+                x[k] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+                b[k] = sc[row / block];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < READ_PIECES; ++k) {
+            if (b[k] < 0) continue;
+            const float power = q8_power(b[k]);
+            const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 lo = q8_float2(w[j] & 0xffffu), hi = q8_float2(w[j] >> 16);
+                v[4 * j] = lo.x * power;
+                v[4 * j + 1] = lo.y * power;
+                v[4 * j + 2] = hi.x * power;
+                v[4 * j + 3] = hi.y * power;
+            }
+            store_w<T, 16>(dst + (int64_t)(c0 + k * READ_THREADS) * 16, v);
+        }
+    }
+}
+
+}  // namespace sllm
+
+using namespace sllm;
+
+template <typename T, int W>
+static int launch_write(const void* qkv, void* q_out, const WriteArgs& a, int64_t ctas, int threads, cudaStream_t stream) {
+    return (int)sllm_launch_pdl(rope_kv_write_q8_kernel<T, W>, dim3((unsigned)ctas), dim3(threads), 0, stream,
+                                (const T*)qkv, (T*)q_out, a);
+}
+
+// write = 0: only the queries.  dtype 0: float32, 1: bfloat16.  block divides page_size and block * hd <= 32768.
+SLLM_EXPORT int sllm_rope_kv_write_q8(const void* qkv, void* q_out, const int* row_start, const int* row_pos0, int n_rows,
+                                      int n_tokens, int max_new, const float* cos_t, const float* sin_t, int rot,
+                                      int interleaved, const float* bias, void* pages, void* scales, const int* table,
+                                      int table_stride, int page_size, int block, int H, int G, int hd, int write, int dtype,
+                                      cudaStream_t stream) {
+    if (n_rows <= 0 || n_tokens <= 0 || max_new <= 0) return 0;
+    if (H <= 0 || G <= 0 || hd <= 0 || hd % 16 || rot < 0 || rot > hd || rot % 2 || page_size <= 0 || block <= 0 ||
+        page_size % block || (int64_t)block * hd > 64 * WRITE_THREADS || (dtype != 0 && dtype != 1))
+        return (int)cudaErrorInvalidValue;
+    if (((uintptr_t)pages | (uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)bias | (uintptr_t)cos_t | (uintptr_t)sin_t) & 15)
+        return (int)cudaErrorInvalidValue;
+    const bool wide = rot % 16 == 0;     // (the tables' rows are then whole 16-byte words too)
+    const int W = wide ? 8 : 1;
+    WriteArgs a = {row_start, row_pos0, cos_t, sin_t, bias, (uint8_t*)pages, (uint8_t*)scales, table, table_stride, page_size,
+                   block, n_rows, n_tokens, H, G, hd, rot, interleaved, max_new == 1};
+    const int upt = hd / (2 * W);
+    // the most that a row stores in a block, in threads of `hold` units
+    const int hold = wide ? WRITE_UNITS<8> : WRITE_UNITS<1>;
+    const int units = (max_new < block ? max_new : block) * upt;
+    const int need = (units + hold - 1) / hold;
+    if (need > WRITE_THREADS) return (int)cudaErrorInvalidValue;
+    if (need <= 32) {
+        a.lanes = 1;
+        // (a unit a thread where a warp holds them all: fewer steps in a row)
+        while (a.lanes < need || (a.lanes < 32 && a.lanes < units)) a.lanes *= 2;
+    } else {
+        a.lanes = (need + 31) / 32 * 32;
+    }
+    const int threads = a.lanes > 32 ? a.lanes : 256;
+    const int64_t slots = a.single ? n_rows : (int64_t)n_tokens / block + 2 * (int64_t)n_rows;
+    a.n_tasks = write ? slots * 2 * G : 0;
+    const int in_cta = threads / a.lanes;
+    const int64_t kv_ctas = (a.n_tasks + in_cta - 1) / in_cta;
+    a.q_groups = H < 4 ? H : 4;
+    a.n_q_items = (int64_t)n_tokens * a.q_groups * upt;
+    int64_t q_ctas = (a.n_q_items + threads - 1) / threads;
+    const int64_t most = 148 * 16 * 256 / threads;
+    if (q_ctas > most) q_ctas = most;
+    if (kv_ctas + q_ctas > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    a.kv_ctas = (int)kv_ctas;
+    if (dtype == 0) return wide ? launch_write<float, 8>(qkv, q_out, a, kv_ctas + q_ctas, threads, stream)
+                                : launch_write<float, 1>(qkv, q_out, a, kv_ctas + q_ctas, threads, stream);
+    return wide ? launch_write<__nv_bfloat16, 8>(qkv, q_out, a, kv_ctas + q_ctas, threads, stream)
+                : launch_write<__nv_bfloat16, 1>(qkv, q_out, a, kv_ctas + q_ctas, threads, stream);
+}
+
+SLLM_EXPORT int sllm_kv_read_q8(const void* pages, const void* scales, const int* table, int table_stride,
+                                const int* row_from, const int* row_to, void* out, const int* out_table, int out_stride,
+                                int n_rows, int max_tokens, int page_size, int block, int G, int hd, int dtype,
+                                cudaStream_t stream) {
+    if (n_rows <= 0 || max_tokens <= 0) return 0;
+    if (G <= 0 || hd <= 0 || hd % 16 || page_size <= 0 || block <= 0 || page_size % block ||
+        (int64_t)G * page_size * hd > (1 << 27) || (((uintptr_t)pages | (uintptr_t)out) & 15) || (dtype != 0 && dtype != 1))
+        return (int)cudaErrorInvalidValue;
+    const int pieces = 2 * G * page_size * hd / 16, per = READ_THREADS * READ_PIECES;
+    // (max_tokens positions that start anywhere touch this many pages)
+    int64_t most = (int64_t)(max_tokens - 1) / page_size + 2;
+    if (most > 65535) most = 65535;
+    for (int r = 0; r < n_rows; r += 65535) {
+        const dim3 grid((pieces + per - 1) / per, (unsigned)most, n_rows - r < 65535 ? n_rows - r : 65535);
+        const cudaError_t e = dtype == 0
+            ? sllm_launch_pdl(kv_read_q8_kernel<float>, grid, dim3(READ_THREADS), 0, stream, (const uint8_t*)pages,
+                              (const uint8_t*)scales, table, table_stride, row_from, row_to, (float*)out, out_table,
+                              out_stride, page_size, block, G, hd, r)
+            : sllm_launch_pdl(kv_read_q8_kernel<__nv_bfloat16>, grid, dim3(READ_THREADS), 0, stream, (const uint8_t*)pages,
+                              (const uint8_t*)scales, table, table_stride, row_from, row_to, (__nv_bfloat16*)out, out_table,
+                              out_stride, page_size, block, G, hd, r);
+        if (e != cudaSuccess) return (int)e;
+    }
+    return 0;
+}

@@ -51,6 +51,8 @@ EXTRA_LIBRARIES: dict[str, tuple[tuple[str, ...], tuple[str, ...]]] = {
     "sllm_sum_norm": (("sum_norm.cu",), ()),
     "sllm_streams": (("streams.cu",), ()),
     "sllm_channel_scan": (("channel_scan.cu",), ()),
+    "sllm_kv_q8": (("kv_q8.cu",), ()),
+    "sllm_drafts": (("drafts.cu",), ()),
 }
 
 
@@ -66,6 +68,11 @@ def attention_mma_library(head_dim: int) -> tuple[str, tuple[str, ...], tuple[st
 
 def attention_tc_library(head_dim: int) -> tuple[str, tuple[str, ...], tuple[str, ...]]:
     return (f"sllm_attention_tc_hd{head_dim}", ("attention_tc.cu",),
+            (f"SLLM_HEAD_DIM={head_dim}",))
+
+
+def attention_q8_library(head_dim: int) -> tuple[str, tuple[str, ...], tuple[str, ...]]:
+    return (f"sllm_attention_q8_hd{head_dim}", ("attention_q8.cu",),
             (f"SLLM_HEAD_DIM={head_dim}",))
 
 
@@ -899,7 +906,204 @@ def attention_mma_scratch_floats(n_tokens: int, n_heads: int, head_dim: int, n_s
     return n_tokens * n_heads * n_splits * (head_dim + 1) if n_splits > 1 else 0
 
 
+# ------------------------------------------------------------------------- a cache in 8 bits
+
+#: what a cache in 8 bits holds: values as e4m3 numbers, and per block of tokens, plane and kv head one power of two
+Q8_DTYPE, Q8_SCALE_DTYPE = torch.float8_e4m3fn, torch.float8_e8m0fnu
+#: the kernels that read and write such a cache take head sizes that are multiples of 16 up to this
+Q8_MAX_HEAD_DIM = 256
+#: a block of the cache has at most this many entries (tokens x head size): what writes it keeps it in registers
+Q8_MAX_BLOCK_ENTRIES = 32768
+
+
+def _here(**tensors: torch.Tensor | None) -> None:
+    """Every tensor lies on the current device, whose stream the kernel is launched on."""
+    device = torch.cuda.current_device()
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != device:
+            raise KernelError(f"{name} is on {t.device}, the current device is cuda:{device}")
+
+
+def _i32_rows(t: torch.Tensor, n: int, name: str) -> None:
+    _need(t, torch.int32, name)
+    if t.dim() != 1 or t.numel() < n:
+        raise KernelError(f"{name} must have {n} entries")
+
+
+def _table(t: torch.Tensor, n_rows: int, name: str) -> None:
+    _need(t, torch.int32, name, contiguous=False)
+    if t.dim() != 2 or t.shape[0] < n_rows or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise KernelError(f"{name} must have {n_rows} contiguous rows")
+
+
+def _q8_cache(pages: torch.Tensor, scales: torch.Tensor, n_kv_heads: int, page_size: int, head_dim: int) -> int:
+    """Checks a cache in 8 bits and returns the tokens of its blocks."""
+    _need(pages, Q8_DTYPE, "pages")
+    _need(scales, Q8_SCALE_DTYPE, "scales")
+    if pages.dim() != 5 or pages.shape[1:] != (2, n_kv_heads, page_size, head_dim):
+        raise KernelError(f"pages must be [n_pages, 2, {n_kv_heads}, {page_size}, {head_dim}], got {list(pages.shape)}")
+    if scales.dim() != 4 or scales.shape[:3] != (pages.shape[0], 2, n_kv_heads) or scales.shape[3] < 1 \
+            or page_size % scales.shape[3]:
+        raise KernelError(f"scales must be [{pages.shape[0]}, 2, {n_kv_heads}, blocks of a page] with blocks that divide "
+                          f"the page's {page_size} tokens, got {list(scales.shape)}")
+    if head_dim % 16 or not 16 <= head_dim <= Q8_MAX_HEAD_DIM:
+        raise KernelError(f"head size {head_dim}: a cache in 8 bits takes multiples of 16 up to {Q8_MAX_HEAD_DIM}")
+    block = page_size // scales.shape[3]
+    if block * head_dim > Q8_MAX_BLOCK_ENTRIES:
+        raise KernelError(f"blocks of {block} tokens of {head_dim} entries: at most {Q8_MAX_BLOCK_ENTRIES} entries")
+    if pages.data_ptr() % 16:
+        raise KernelError("pages must start on a 16-byte boundary")
+    return block
+
+
+def rope_kv_write_q8(qkv: torch.Tensor, row_start: torch.Tensor, row_pos0: torch.Tensor, n_rows: int, max_new: int,
+                     cos: torch.Tensor | None, sin: torch.Tensor | None, q_out: torch.Tensor, pages: torch.Tensor,
+                     scales: torch.Tensor, block_table: torch.Tensor, page_size: int, n_heads: int, n_kv_heads: int,
+                     head_dim: int, interleaved: bool, write: bool = True, bias: torch.Tensor | None = None) -> None:
+    """:func:`rope_kv_write` into a cache held in 8 bits: the rotated queries go to ``q_out`` [N, H * hd] (``qkv`` is left
+    as it is), keys and values are quantised as they are stored.  ``pages`` float8_e4m3fn [n_pages, 2, G, page_size, hd],
+    ``scales`` float8_e8m0fnu [n_pages, 2, G, page_size / block]: one power of two per block of tokens, the smallest
+    with which the block's largest finite value is at most 448.  Row r brings the tokens ``row_start[r]`` to
+    ``row_start[r + 1] - 1`` (at most ``max_new``), at the positions from ``row_pos0[r]`` on; a block in which the row has
+    earlier tokens keeps its scale or takes a larger one, at which the earlier tokens' numbers are rounded again.
+    Infinities and NaN are stored as NaN.  Two rows of a step share no block.  Tables of fewer than ``head_dim / 2``
+    columns rotate only the first ``2 * columns`` entries of a head; ``cos`` None rotates nothing."""
+    _need(qkv, None, "qkv")
+    _need(q_out, qkv.dtype, "q_out")
+    block = _q8_cache(pages, scales, n_kv_heads, page_size, head_dim)
+    n = qkv.shape[0]
+    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim:
+        raise KernelError("qkv width does not match the head counts")
+    if q_out.shape != (n, n_heads * head_dim):
+        raise KernelError(f"q_out must be [{n}, {n_heads * head_dim}], got {list(q_out.shape)}")
+    _i32_rows(row_start, n_rows + 1, "row_start")
+    _i32_rows(row_pos0, n_rows, "row_pos0")
+    _table(block_table, n_rows, "block_table")
+    rot = 0
+    if cos is not None:
+        _need(cos, torch.float32, "cos")
+        _need(sin, torch.float32, "sin")
+        if cos.dim() != 2 or not 1 <= cos.shape[1] <= head_dim // 2 or sin.shape != cos.shape:
+            raise KernelError("rotary table width")
+        rot = 2 * cos.shape[1]
+    if bias is not None:
+        _need(bias, torch.float32, "bias")
+        if bias.numel() != qkv.shape[1]:
+            raise KernelError("bias must have one entry per column of qkv")
+    _here(qkv=qkv, q_out=q_out, row_start=row_start, row_pos0=row_pos0, cos=cos, sin=sin, pages=pages, scales=scales,
+          block_table=block_table, bias=bias)
+    for t, name in ((qkv, "qkv"), (q_out, "q_out"), (cos, "cos"), (sin, "sin"), (bias, "bias")):
+        if t is not None and t.data_ptr() % 16:
+            raise KernelError(f"{name} must start on a 16-byte boundary")
+    _check(_core("sllm_kv_q8").sllm_rope_kv_write_q8(
+        _ptr(qkv), _ptr(q_out), _ptr(row_start), _ptr(row_pos0), c_int(n_rows), c_int(n), c_int(max_new), _ptr(cos),
+        _ptr(sin), c_int(rot), c_int(int(interleaved)), _ptr(bias), _ptr(pages), _ptr(scales), _ptr(block_table),
+        c_int(block_table.stride(0)), c_int(page_size), c_int(block), c_int(n_heads), c_int(n_kv_heads), c_int(head_dim),
+        c_int(int(write)), c_int(_code(qkv.dtype)), _stream()), "rope_kv_write_q8")
+
+
+def kv_read_q8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, page_size: int,
+               row_from: torch.Tensor, row_to: torch.Tensor, out: torch.Tensor, out_table: torch.Tensor, n_rows: int,
+               max_tokens: int) -> torch.Tensor:
+    """Reads a cache in 8 bits back: the keys and values at the positions ``row_from[r]`` to ``row_to[r] - 1`` of every
+    row (at most ``max_tokens``) go to the same places of the pages that ``out_table`` names, ``out``
+    [n, 2, G, page_size, hd] in bfloat16 or float32, in which they are exact.  All other places are left alone."""
+    _need(out, None, "out")
+    if out.dim() != 5:
+        raise KernelError(f"out must be [n, 2, kv heads, {page_size}, head size], got {list(out.shape)}")
+    _, _, g, _, hd = out.shape
+    block = _q8_cache(pages, scales, g, page_size, hd)
+    if out.shape[1:] != pages.shape[1:]:
+        raise KernelError(f"out must have pages like the cache's {list(pages.shape[1:])}, got {list(out.shape[1:])}")
+    _i32_rows(row_from, n_rows, "row_from")
+    _i32_rows(row_to, n_rows, "row_to")
+    _table(block_table, n_rows, "block_table")
+    _table(out_table, n_rows, "out_table")
+    _here(pages=pages, scales=scales, block_table=block_table, row_from=row_from, row_to=row_to, out=out,
+          out_table=out_table)
+    if out.data_ptr() % 16:
+        raise KernelError("out must start on a 16-byte boundary")
+    _check(_core("sllm_kv_q8").sllm_kv_read_q8(
+        _ptr(pages), _ptr(scales), _ptr(block_table), c_int(block_table.stride(0)), _ptr(row_from), _ptr(row_to), _ptr(out),
+        _ptr(out_table), c_int(out_table.stride(0)), c_int(n_rows), c_int(max_tokens), c_int(page_size), c_int(block),
+        c_int(g), c_int(hd), c_int(_code(out.dtype)), _stream()), "kv_read_q8")
+    return out
+
+
+def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, page_size: int,
+                 row_start: torch.Tensor, row_pos0: torch.Tensor, out: torch.Tensor, row_list: torch.Tensor | None,
+                 n_list: int, max_new: int, max_context: int, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
+                 window: int | None = None) -> torch.Tensor:
+    """Causal attention of the listed rows (all ``n_list`` of them in order for ``row_list`` None) over a cache held in 8
+    bits (:func:`rope_kv_write_q8`), for single tokens, drafted tokens and portions of prompts alike.  ``q`` [N, H * hd] may be
+    a column slice; bfloat16 or float32, and ``out`` likewise.  No row brings more than ``max_new`` tokens, and no query
+    stands at a position of ``max_context`` or more."""
+    _need(q, None, "q", contiguous=False)
+    _need(out, q.dtype, "out", contiguous=False)
+    block = _q8_cache(pages, scales, n_kv_heads, page_size, head_dim)
+    if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] != n_heads * head_dim or out.shape != q.shape or out.stride(1) != 1:
+        raise KernelError("attention q/out layout")
+    if n_heads % n_kv_heads:
+        raise KernelError(f"{n_heads} query heads do not group evenly over {n_kv_heads} kv heads")
+    if row_list is not None:
+        _i32_rows(row_list, n_list, "row_list")
+    need = n_list if row_list is None else 1
+    _i32_rows(row_start, need + 1, "row_start")
+    _i32_rows(row_pos0, need, "row_pos0")
+    _table(block_table, need, "block_table")
+    if window is not None and window < 0:
+        raise KernelError(f"window must not be negative, got {window}")
+    _here(q=q, pages=pages, scales=scales, block_table=block_table, row_start=row_start, row_pos0=row_pos0, out=out,
+          row_list=row_list)
+    _check(_load(*attention_q8_library(head_dim)).sllm_attn_q8(
+        _ptr(q), c_int64(q.stride(0)), _ptr(pages), _ptr(scales), _ptr(block_table), c_int(block_table.stride(0)),
+        c_int(page_size), c_int(block), _ptr(row_start), _ptr(row_pos0), _ptr(row_list), c_int(n_list), c_int(max_new),
+        _ptr(out), c_int64(out.stride(0)), c_int(n_heads), c_int(n_kv_heads), c_float(scale), c_int(window or 0),
+        c_int(_code(q.dtype)), _stream()), "attention_q8")
+    return out
+
+
 # --------------------------------------------------------------------------------- sampling
+
+def verify_drafts(probs: torch.Tensor, drafts: torch.Tensor, draft_start: torch.Tensor, uniforms: torch.Tensor,
+                  tokens: torch.Tensor, accepted: torch.Tensor, max_drafts: int,
+                  draft_probs: torch.Tensor | None = None) -> None:
+    """Verify drafted tokens against the target's probabilities.  Row r has the drafts ``draft_start[r]`` to
+    ``draft_start[r + 1] - 1`` of ``drafts`` (int32 [K]; none to ``max_drafts``), and one more row of ``probs`` (float32
+    [K + n, V], the target's distribution after the drafts before it), number of ``uniforms`` (float32 [K + n], in
+    [0, 1)) and place of ``tokens`` (int32 [K + n]), all from ``draft_start[r] + r`` on.  ``draft_probs`` (float32 [K, V]):
+    the distributions that the drafts were drawn from; None: drafts that were looked up, each with all of its mass on
+    the draft.  Draft i is accepted while ``u_i * q_i(x_i) < p_i(x_i)``; the first that is not is replaced by a draw from
+    ``max(p_i - q_i, 0)``, and k accepted ones are followed by a draw from ``p_k``, both with the row's last number:
+    the first token whose cumulative weight exceeds it times the total.  ``tokens`` then holds the accepted drafts, the
+    drawn token and -1 behind it, ``accepted`` (int32 [n]) how many drafts that are.  A NaN counts as no probability, as
+    does a draft outside the vocabulary; where no weight is left the row draws from ``p_i``, and a row of no probability at
+    all gets the token -1.  Sums are formed in 64 bits."""
+    _need(probs, torch.float32, "probs", contiguous=False)
+    _need(uniforms, torch.float32, "uniforms")
+    for t, name in ((drafts, "drafts"), (draft_start, "draft_start"), (tokens, "tokens"), (accepted, "accepted")):
+        _need(t, torch.int32, name)
+    n, k = accepted.numel(), drafts.numel()
+    if probs.dim() != 2 or probs.shape[0] != k + n or probs.shape[1] < 1 or (probs.shape[1] > 1 and probs.stride(1) != 1):
+        raise KernelError(f"probs must be [{k + n}, V] with contiguous rows, got {list(probs.shape)}")
+    if draft_start.numel() != n + 1 or uniforms.numel() != k + n or tokens.numel() != k + n:
+        raise KernelError(f"{k} drafts in {n} rows need {n + 1} starts and {k + n} uniforms and tokens")
+    if draft_probs is not None:
+        _need(draft_probs, torch.float32, "draft_probs", contiguous=False)
+        if draft_probs.shape != (k, probs.shape[1]) or (probs.shape[1] > 1 and draft_probs.stride(1) != 1):
+            raise KernelError(f"draft_probs must be [{k}, {probs.shape[1]}] with contiguous rows, got "
+                              f"{list(draft_probs.shape)}")
+    if max_drafts < 0:
+        raise KernelError(f"max_drafts must not be negative, got {max_drafts}")
+    _here(probs=probs, drafts=drafts, draft_start=draft_start, uniforms=uniforms, tokens=tokens, accepted=accepted,
+          draft_probs=draft_probs)
+    if n == 0:
+        return
+    _check(_core("sllm_drafts").sllm_verify_drafts(
+        _ptr(probs), c_int64(probs.stride(0)), _ptr(draft_probs),
+        c_int64(draft_probs.stride(0) if draft_probs is not None else 0), _ptr(drafts), _ptr(draft_start), _ptr(uniforms),
+        c_int(n), c_int(probs.shape[1]), _ptr(tokens), _ptr(accepted), _stream()), "verify_drafts")
+
 
 def argmax_scratch_bytes(n_rows: int) -> int:
     lib = _core("sllm_sampling")
