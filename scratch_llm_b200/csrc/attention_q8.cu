@@ -3,6 +3,22 @@
 // h / (H / G).  Scores, softmax and sums are 32-bit arithmetic.
 //   s_j = scale * q . k_j,   out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s)
 // Compiled once per head size: -DSLLM_HEAD_DIM=<multiple of 16, at most 256>.
+//
+// Numbers.  An e4m3 number is a half exactly, and one instruction turns two of them, so the products run on the tensor
+// cores' f16 form with the cache's numbers as they are; the blocks' powers of two join the scores (2^ek) and the
+// probabilities (2^ev) in 32 bits.  A query is brought into f16's range by a power of two of its own (largest entry
+// in [2^14, 2^15)): bfloat16 entries keep all their bits down to 2^-38 of the largest, 32-bit ones are split into two
+// halves (22 bits).  A probability is multiplied by its key's 2^ev before it becomes a half, against a running
+// maximum of its own, M = max(s + ev): what counts towards the output keeps 11 bits (22 in the 32-bit form) down
+// to 2^-20 of the largest, whatever the blocks' scales.
+//
+// Layout.  The products are taken transposed, keys and then the values' entries as the 16 rows of mma.m16n8k16, queries as
+// its 8 columns: a decoded token's group of up to 8 query heads fills the instruction, and an output is spread over
+// half as many registers.  Which entry of a head stands in which k step is free as long as queries and keys agree:
+// a lane takes a quarter of each key's bytes as they lie, and of the values an eighth of four keys, so keys and values come
+// from global memory straight into the operands' registers, a whole line a request, with no shared memory between.
+// P becomes an operand by movmatrix.  The next tile's keys are requested once this tile's have met the queries, its
+// values once these are used: half of a warp's registers are always on their way.
 #include "q8.cuh"
 
 #ifndef SLLM_HEAD_DIM
@@ -13,37 +29,101 @@ namespace sllm {
 
 constexpr int HD = SLLM_HEAD_DIM;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size: a multiple of 16 up to 256");
-constexpr int DPL = (HD + 31) / 32;     // entries of a head a lane
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int KSTEPS = HD / 16;                          // k steps of q k; also 16-row tiles of the values' entries
+constexpr bool V_WORDS = HD % 32 == 0;                   // a lane's entries of a value are whole words (else 2 bytes a tile)
+constexpr int VREGS = V_WORDS ? HD / 32 : HD / 16;
+constexpr int DPL = (HD + 31) / 32;                      // entries of a head a lane (scalar form)
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOWEST = -1e30f;                         // below every score; finite, so that differences are numbers
+constexpr float STALE = 8.f;                             // how far a maximum may lag behind the scores (base 2)
+constexpr float P_SHIFT = 6.f;                           // probabilities become halves times 2^6: 2^14 at most
 
 struct Q8Args {
     int64_t q_stride, out_stride;
     const uint8_t* pages; const uint8_t* scales; const int* table;
     const int* row_start; const int* row_pos0; const int* row_list;
-    int table_stride, page_size, block, H, G, window;
-    float scale;
+    float* part; int64_t part_tokens;                    // [tokens, H, n_splits, HD + 2]: sums, maximum, denominator
+    int table_stride, page_size, block, H, G, window, n_splits, wq, q_vec;
+    float scale_log2;
 };
 
-// A warp per token and head, key after key: grid (tokens of a row, rows, heads / 4).
+template <typename T, int NT> struct Form {
+    static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;           // halves that an operand of T is split into
+    static constexpr int KT = HD <= 128 && NT * PARTS <= 2 ? 32 : 16;   // keys of a tile
+    static constexpr int Q_REGS = NT * PARTS * KSTEPS * 2;
+    static constexpr bool Q_SHARED = Q_REGS > 32;
+    static constexpr int LD = HD + 4;
+    static constexpr size_t merge_bytes() { return sizeof(float) * WARPS * 8 * NT * LD; }
+    static constexpr size_t q_bytes() { return Q_SHARED ? sizeof(uint32_t) * WARPS * 32 * Q_REGS : 0; }
+    static constexpr size_t smem() { return merge_bytes() > q_bytes() ? merge_bytes() : q_bytes(); }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// d (16 x 8, f32) += a (16 x 16, f16) * b (16 x 8, f16)
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {       // an 8 x 8 tile of halves
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t halves(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// what is left of (a, b) beside their halves
+__device__ __forceinline__ uint32_t halves_rest(float a, float b, uint32_t h) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    return halves(a - f.x, b - f.y);
+}
+
+// BYTES from global memory into words, in the widest loads that every lane's address allows
+template <int BYTES, int N> __device__ __forceinline__ void fetch(const uint8_t* p, uint32_t (&w)[N]) {
+    if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+        }
+    } else if constexpr (BYTES % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 8; ++i) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>(p) + i);
+            w[2 * i] = x.x; w[2 * i + 1] = x.y;
+        }
+    } else if constexpr (BYTES % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint16_t*>(p) + i);
+    }
+}
+
+// One query over the keys lo .. hi that it sees, key after key, by all warps of the CTA: sums relative to m (base 2) in
+// acc [HD], and (m, l).  For tiles in which a NaN came out: a tensor-core product multiplies also what a query does
+// not see by zero, and zero times a NaN is one.
 template <typename T>
-__global__ void __launch_bounds__(128) attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
-    pdl_wait();
-    pdl_trigger();
-    const int r = a.row_list ? a.row_list[blockIdx.y] : blockIdx.y, lane = threadIdx.x & 31;
-    const int h = blockIdx.z * 4 + threadIdx.x / 32, g = h / (a.H / a.G);
-    const int t0 = a.row_start[r], n_new = a.row_start[r + 1] - t0;
-    if ((int)blockIdx.x >= n_new || h >= a.H) return;
-    const int64_t token = t0 + blockIdx.x;
-    const int pos = a.row_pos0[r] + blockIdx.x;
-    float x[DPL], o[DPL], m = -INFINITY, l = 0.f;
+__device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args& a, const int* __restrict__ table, int g,
+                                           int lo, int hi, float* acc, float* ml, float* smem) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int blocks = a.page_size / a.block;
+    float x[DPL], o[DPL], m = LOWEST, l = 0.f;
 #pragma unroll
     for (int c = 0; c < DPL; ++c) {
-        const int d = lane + 32 * c;
-        x[c] = d < HD ? to_float(q[token * a.q_stride + (int64_t)h * HD + d]) * a.scale : 0.f;
+        x[c] = lane + 32 * c < HD ? to_float(q[lane + 32 * c]) * a.scale_log2 : 0.f;
         o[c] = 0.f;
     }
-    const int blocks = a.page_size / a.block;
-    for (int j = a.window > 0 ? max(0, pos - a.window + 1) : 0; j <= pos; ++j) {
-        const int page = a.table[(int64_t)r * a.table_stride + j / a.page_size], off = j % a.page_size;
+    for (int j = lo + warp; j <= hi; j += WARPS) {
+        const int page = table[j / a.page_size], off = j % a.page_size;
         if (page < 0) continue;
         const int64_t k_plane = (int64_t)page * 2 * a.G + g, v_plane = k_plane + a.G;
         const uint8_t* k = a.pages + (k_plane * a.page_size + off) * HD;
@@ -53,37 +133,496 @@ __global__ void __launch_bounds__(128) attn_q8_kernel(const T* __restrict__ q, T
         for (int c = 0; c < DPL; ++c)
             if (lane + 32 * c < HD) s = fmaf(x[c], q8_float2(k[lane + 32 * c]).x, s);
         s = warp_sum(s) * q8_power(a.scales[k_plane * blocks + off / a.block]);
-        const float top = fmaxf(m, s), keep = m == -INFINITY ? 0.f : expf(m - top);
-        const float p = expf(s - top), pv = p * q8_power(a.scales[v_plane * blocks + off / a.block]);
+        const float top = fmaxf(m, s), keep = exp2f(m - top);
+        const float p = exp2f(s - top), pv = p * q8_power(a.scales[v_plane * blocks + off / a.block]);
         m = top;
         l = l * keep + p;
 #pragma unroll
         for (int c = 0; c < DPL; ++c)
             if (lane + 32 * c < HD) o[c] = o[c] * keep + pv * q8_float2(v[lane + 32 * c]).x;
     }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < DPL; ++c)
+        if (lane + 32 * c < HD) smem[warp * HD + lane + 32 * c] = o[c];
+    if (lane == 0) { ml[2 * warp] = m; ml[2 * warp + 1] = l; }
+    __syncthreads();
+    float top = LOWEST, total = 0.f;
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[2 * w]);
+    for (int w = 0; w < WARPS; ++w) total += ml[2 * w + 1] * exp2f(ml[2 * w] - top);
+    for (int d = threadIdx.x; d < HD; d += THREADS) {
+        float sum = 0.f;
+        for (int w = 0; w < WARPS; ++w) sum += smem[w * HD + d] * exp2f(ml[2 * w] - top);
+        acc[d] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) { ml[2 * WARPS] = top; ml[2 * WARPS + 1] = total; }
+    __syncthreads();
+}
+
+// The queries of a row and kv head are packed: p = token * GS + j is the row's token `token` and query head g GS + j.  A
+// CTA takes 8 NT wq packed queries over a share of the keys; its warps are wq groups of queries by 4 / wq groups of keys,
+// which take turns at the tiles.  A CTA with fewer queries than the launch allows has fewer groups of queries.
+// grid (kv heads, splits x tiles of queries, rows), the tiles with the most keys first.
+template <typename T, int NT>
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
+attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
+    using F = Form<T, NT>;
+    constexpr int PARTS = F::PARTS, KT = F::KT, KG = KT / 16, LD = F::LD;
+    extern __shared__ __align__(16) float smem[];
+    __shared__ float sm_m[WARPS][8 * NT], sm_l[WARPS][8 * NT], sm_ml[2 * WARPS + 2];
+    pdl_wait();
+    pdl_trigger();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n8 = lane >> 2, c4 = lane & 3;
+    const int r = a.row_list ? a.row_list[blockIdx.z] : blockIdx.z, g = blockIdx.x, GS = a.H / a.G;
+    const int split = blockIdx.y % a.n_splits;
+    const int q0 = ((int)(gridDim.y / a.n_splits) - 1 - (int)blockIdx.y / a.n_splits) * 8 * NT * a.wq;
+    const int t0 = a.row_start[r], n_packed = (a.row_start[r + 1] - t0) * GS;
+    if (q0 >= n_packed) return;
+    const int pos0 = a.row_pos0[r], nq = min(n_packed - q0, 8 * NT * a.wq);
+    const int first_pos = pos0 + q0 / GS, last_pos = pos0 + (q0 + nq - 1) / GS;
+    const int wq = min(a.wq, nq <= 8 * NT ? 1 : nq <= 16 * NT ? 2 : 4), wk = WARPS / wq;
+    const int* table = a.table + (int64_t)r * a.table_stride;
+    const int k_lo = a.window > 0 ? max(0, first_pos - a.window + 1) / KT * KT : 0;
+    const int n_tiles = (last_pos - k_lo) / KT + 1;
+    const int per_split = (n_tiles + a.n_splits - 1) / a.n_splits;
+    const int tile_begin = min(n_tiles, split * per_split), tile_end = min(n_tiles, tile_begin + per_split);
+
+    // ---- this warp's queries
+    const int w0 = q0 + (warp % wq) * 8 * NT, w_nq = min(8 * NT, q0 + nq - w0);     // (w_nq may be 0 or less)
+    const int w_first = pos0 + w0 / GS, w_last = pos0 + (w0 + max(w_nq, 1) - 1) / GS;
+    uint32_t qf[F::Q_SHARED ? 1 : PARTS][F::Q_SHARED ? 1 : NT][F::Q_SHARED ? 1 : KSTEPS][2];
+    uint2* q_sh = reinterpret_cast<uint2*>(smem) + warp * (F::Q_REGS / 2) * 32 + lane;   // [part][nt][ks][lane]
+    float fq[NT][2];                      // scale * log2 e / the query's power of two, of queries 2 c4 and 2 c4 + 1
+    int qpos[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int i = nt * 8 + n8, p = w0 + i;
+        const bool there = i < w_nq;
+        const int tok = there ? p / GS : 0, j = there ? p - tok * GS : 0;
+        const T* src = q + (int64_t)(t0 + tok) * a.q_stride + (int64_t)(g * GS + j) * HD + c4 * (HD / 4);
+        float x[HD / 4], top = 0.f;
+        if (a.q_vec) {
+#pragma unroll
+            for (int d = 0; d < HD / 4; d += 4) {
+                if constexpr (sizeof(T) == 4) {
+                    Vec<float>::load(reinterpret_cast<const float*>(src) + d, x + d);
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(src + d);
+                    x[d] = __uint_as_float(w.x << 16); x[d + 1] = __uint_as_float(w.x & 0xffff0000u);
+                    x[d + 2] = __uint_as_float(w.y << 16); x[d + 3] = __uint_as_float(w.y & 0xffff0000u);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int d = 0; d < HD / 4; ++d) x[d] = to_float(src[d]);
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 4; ++d) {
+            if (!there) x[d] = 0.f;
+            top = fmaxf(top, q8_finite(x[d]) ? fabsf(x[d]) : 0.f);
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^k with top * 2^k in [2^14, 2^15); at most 2^100, so that its inverse times the scale is a normal number
+        const int k = top > 0.f ? min(100, 14 + 127 - (__float_as_int(top) >> 23)) : 0;
+        const float up = __int_as_float((k + 127) << 23);
+        const float own = a.scale_log2 * __int_as_float((127 - k) << 23);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            fq[nt][e] = __shfl_sync(0xffffffffu, own, (2 * c4 + e) * 4);
+            const int pe = nt * 8 + 2 * c4 + e;
+            qpos[nt][e] = pe < w_nq ? pos0 + (w0 + pe) / GS : -1;
+        }
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+            const float y0 = x[4 * ks] * up, y1 = x[4 * ks + 1] * up, y2 = x[4 * ks + 2] * up, y3 = x[4 * ks + 3] * up;
+            const uint32_t h0 = halves(y0, y1), h1 = halves(y2, y3);
+            uint32_t r0 = 0, r1 = 0;
+            if constexpr (PARTS == 2) {
+                r0 = halves_rest(y0, y1, h0);
+                r1 = halves_rest(y2, y3, h1);
+            }
+            if constexpr (F::Q_SHARED) {
+                q_sh[(nt * KSTEPS + ks) * 32] = make_uint2(h0, h1);
+                if constexpr (PARTS == 2) q_sh[((NT + nt) * KSTEPS + ks) * 32] = make_uint2(r0, r1);
+            } else {
+                qf[0][nt][ks][0] = h0; qf[0][nt][ks][1] = h1;
+                if constexpr (PARTS == 2) { qf[1][nt][ks][0] = r0; qf[1][nt][ks][1] = r1; }
+            }
+        }
+    }
+
+    float o[KSTEPS][NT][4], m[NT][2], M[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][nt][e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) { m[nt][e] = M[nt][e] = LOWEST; l[nt][e] = 0.f; }
+    }
+
+    // ---- where a tile's keys lie: lane i looks up key i (page, then its two scales) and tells the others
+    const int blocks = a.page_size / a.block;
+    const uint32_t v_rows = (uint32_t)a.G * a.page_size;
+    int tile_stop = tile_end;             // this warp's queries see nothing from here on
+    if (w_nq <= 0) tile_stop = tile_begin;
+    else tile_stop = min(tile_stop, (w_last - k_lo) / KT + 1);
+    auto page_of = [&](int tile) {
+        const int kpos = k_lo + tile * KT + lane % KT;
+        return tile < tile_stop && kpos <= w_last ? __ldg(table + kpos / a.page_size) : -1;
+    };
+    auto row_of = [&](int tile, int page) {       // the key's row among all rows of HD bytes (at most 2^32 - 2), ~0: none
+        const int off = (k_lo + tile * KT + lane % KT) % a.page_size;
+        return page >= 0 ? ((uint32_t)page * 2u * a.G + g) * a.page_size + off : 0xffffffffu;
+    };
+    auto scales_of = [&](int tile, int page) {
+        if (page < 0) return 127 | 127 << 8;
+        const int off = (k_lo + tile * KT + lane % KT) % a.page_size;
+        const uint8_t* s = a.scales + ((int64_t)page * 2 * a.G + g) * blocks + off / a.block;
+        return (int)__ldg(s) | (int)__ldg(s + (int64_t)a.G * blocks) << 8;
+    };
+    uint32_t kr[2 * KG][KSTEPS], vr[KG][4][VREGS];
+    auto fetch_keys = [&](uint32_t row) {         // (a key that is not there: some row of the cache, masked below)
+#pragma unroll
+        for (int i = 0; i < 2 * KG; ++i) {
+            const uint32_t at = __shfl_sync(0xffffffffu, row, n8 + 8 * i);
+            fetch<HD / 4>(a.pages + (size_t)(at == 0xffffffffu ? 0u : at) * HD + c4 * (HD / 4), kr[i]);
+        }
+    };
+    auto fetch_values = [&](uint32_t row) {       // (a value that is not there: zeros)
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t at = __shfl_sync(0xffffffffu, row, 16 * i + 2 * c4 + (k & 1) + 8 * (k >> 1));
+#pragma unroll
+                for (int w = 0; w < VREGS; ++w) vr[i][k][w] = 0u;
+                if (at != 0xffffffffu)
+                    fetch<HD / 8>(a.pages + ((size_t)at + v_rows) * HD + n8 * (HD / 8), vr[i][k]);
+            }
+    };
+
+    int tile = tile_begin + warp / wq;
+    int page = page_of(tile), page_next = page_of(tile + wk);
+    uint32_t row = row_of(tile, page), row_next = row_of(tile + wk, page_next);
+    int sc = scales_of(tile, page), sc_next = scales_of(tile + wk, page_next);
+    if (tile < tile_stop) {
+        fetch_keys(row);
+        fetch_values(row);
+    }
+    int page_after = page_of(tile + 2 * wk);
+
+    for (; tile < tile_stop; tile += wk) {
+        const int kt = k_lo + tile * KT;
+        // ---- scores, transposed: rows are keys, columns queries
+        float s[KG][NT][4];
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][nt][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+            uint32_t b[PARTS][NT][2];
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    if constexpr (F::Q_SHARED) {
+                        const uint2 w = q_sh[((part * NT + nt) * KSTEPS + ks) * 32];
+                        b[part][nt][0] = w.x; b[part][nt][1] = w.y;
+                    } else {
+                        b[part][nt][0] = qf[part][nt][ks][0]; b[part][nt][1] = qf[part][nt][ks][1];
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < KG; ++i) {
+                const uint32_t f[4] = {q8_half2(kr[2 * i][ks] & 0xffffu), q8_half2(kr[2 * i + 1][ks] & 0xffffu),
+                                       q8_half2(kr[2 * i][ks] >> 16), q8_half2(kr[2 * i + 1][ks] >> 16)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int part = PARTS - 1; part >= 0; --part) mma_f16(s[i][nt], f, b[part][nt][0], b[part][nt][1]);
+            }
+        }
+        const bool whole = __all_sync(0xffffffffu, row != 0xffffffffu) && kt + KT - 1 <= w_first &&
+                           (a.window <= 0 || kt > w_last - a.window);
+        uint32_t seen_rows = 0;
+        if (!whole) seen_rows = __ballot_sync(0xffffffffu, row != 0xffffffffu);
+        if (tile + wk < tile_stop) fetch_keys(row_next);
+
+        // ---- scaled scores, their maxima
+        float ev[KG][2];                  // the values' exponents of this lane's keys
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int key = 16 * i + 8 * k + n8;
+                const int both = __shfl_sync(0xffffffffu, sc, key);
+                const float fk = __int_as_float((both & 0xff) << 23);
+                ev[i][k] = (float)(both >> 8) - 127.f;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = s[i][nt][2 * k + e] * fq[nt][e] * fk;
+                        if (!whole) {
+                            const int kpos = kt + key;
+                            const bool ok = (seen_rows >> key & 1u) && kpos <= qpos[nt][e] &&
+                                            (a.window <= 0 || kpos > qpos[nt][e] - a.window);
+                            x = ok ? x : -INFINITY;
+                        }
+                        s[i][nt][2 * k + e] = x;
+                    }
+            }
+        bool moved = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int i = 0; i < KG; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float x = s[i][nt][2 * k + e];
+                        moved |= x > m[nt][e] + STALE || x + ev[i][k] > M[nt][e] + STALE;
+                    }
+        if (__any_sync(0xffffffffu, moved)) {
+            // (seldom after a row's first tiles: a maximum may lag by 2^8, which halves and sums hold)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = m[nt][e], Top = M[nt][e];
+#pragma unroll
+                    for (int i = 0; i < KG; ++i)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            top = fmaxf(top, s[i][nt][2 * k + e]);
+                            Top = fmaxf(Top, s[i][nt][2 * k + e] + ev[i][k]);
+                        }
+#pragma unroll
+                    for (int x = 4; x < 32; x *= 2) {
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                        Top = fmaxf(Top, __shfl_xor_sync(0xffffffffu, Top, x));
+                    }
+                    l[nt][e] *= ex2(m[nt][e] - top);
+                    const float keep = ex2(M[nt][e] - Top);
+                    m[nt][e] = top;
+                    M[nt][e] = Top;
+#pragma unroll
+                    for (int j = 0; j < KSTEPS; ++j) {
+                        o[j][nt][e] *= keep;
+                        o[j][nt][2 + e] *= keep;
+                    }
+                }
+        }
+        // ---- probabilities, as the second operand
+        uint32_t p[PARTS][KG][NT][2];
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float y[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float x = s[i][nt][2 * k + e];
+                        l[nt][e] += ex2(x - m[nt][e]);
+                        y[e] = ex2(x + (ev[i][k] + P_SHIFT - M[nt][e]));
+                    }
+                    const uint32_t h = halves(y[0], y[1]);
+                    p[0][i][nt][k] = transposed(h);
+                    if constexpr (PARTS == 2) p[1][i][nt][k] = transposed(halves_rest(y[0], y[1], h));
+                }
+        // ---- sums over the keys, transposed: rows are entries of a head
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+#pragma unroll
+            for (int j = 0; j < KSTEPS; ++j) {
+                constexpr uint32_t LOW = 0x5140, HIGH = 0x7362;
+                const int w = V_WORDS ? j / 2 : j;
+                const uint32_t pick = V_WORDS && (j & 1) ? HIGH : LOW;
+                const uint32_t x = __byte_perm(vr[i][0][w], vr[i][1][w], pick);
+                const uint32_t y = __byte_perm(vr[i][2][w], vr[i][3][w], pick);
+                const uint32_t f[4] = {q8_half2(x & 0xffffu), q8_half2(x >> 16), q8_half2(y & 0xffffu), q8_half2(y >> 16)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int part = PARTS - 1; part >= 0; --part)
+                        mma_f16(o[j][nt], f, p[part][i][nt][0], p[part][i][nt][1]);
+            }
+        if (tile + wk < tile_stop) fetch_values(row_next);
+        row = row_next;
+        sc = sc_next;
+        row_next = row_of(tile + 2 * wk, page_after);
+        sc_next = scales_of(tile + 2 * wk, page_after);
+        page_after = page_of(tile + 3 * wk);
+    }
+
+    // ---- the groups of keys meet
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+            if (n8 == 0) {
+                sm_m[warp][nt * 8 + 2 * c4 + e] = m[nt][e];
+                sm_l[warp][nt * 8 + 2 * c4 + e] = l[nt][e];
+            }
+        }
+    __syncthreads();                      // (and the queries in shared memory are done with)
+    float* sums = smem;                   // [WARPS][8 NT][LD]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int i = nt * 8 + 2 * c4 + e;
+            float top = LOWEST;
+            for (int w = warp % wq; w < WARPS; w += wq) top = fmaxf(top, sm_m[w][i]);
+            const float f = ex2(M[nt][e] - P_SHIFT - top);
+            float* to = sums + (warp * 8 * NT + i) * LD + n8 * (HD / 8);
+#pragma unroll
+            for (int j = 0; j < KSTEPS; ++j)
+                *reinterpret_cast<float2*>(to + 2 * j) = make_float2(o[j][nt][e] * f, o[j][nt][2 + e] * f);
+        }
+    __syncthreads();
+    const int64_t part_ld = HD + 2;
+    auto leave = [&](int i, int d, float sum, float top, float total) {       // query i's entry d
+        const int p = q0 + i, tok = p / GS, h = g * GS + p - tok * GS;
+        if (a.n_splits == 1) {
+            out[(int64_t)(t0 + tok) * a.out_stride + (int64_t)h * HD + d] = from_float<T>(total == 0.f ? 0.f : sum / total);
+        } else if (t0 + tok < a.part_tokens) {
+            float* part = a.part + (((int64_t)(t0 + tok) * a.H + h) * a.n_splits + split) * part_ld;
+            part[d] = sum;
+            if (d == 0) { part[HD] = top; part[HD + 1] = total; }
+        }
+    };
+    bool odd = false;
+    for (int idx = tid; idx < nq * HD; idx += THREADS) {
+        const int i = idx / HD, d = idx - i * HD, group = i / (8 * NT), j = i - group * 8 * NT;
+        float top = LOWEST, total = 0.f, sum = 0.f;
+        for (int w = group; w < WARPS; w += wq) top = fmaxf(top, sm_m[w][j]);
+        for (int w = group; w < WARPS; w += wq) {
+            total += sm_l[w][j] * ex2(sm_m[w][j] - top);
+            sum += sums[(w * 8 * NT + j) * LD + d];
+        }
+        odd |= isnan(sum) || isnan(total);
+        leave(i, d, sum, top, total);
+    }
+    // a NaN, and not all queries see the same keys: each of them by itself
+    if (__syncthreads_or(odd) && first_pos != last_pos) {
+        float* acc = smem + WARPS * HD;
+        static_assert((WARPS + 1) * HD <= WARPS * 8 * LD, "room for the scalar form");
+        for (int i = 0; i < nq; ++i) {
+            const int p = q0 + i, tok = p / GS, pos = pos0 + tok;
+            const int lo = max(k_lo + tile_begin * KT, a.window > 0 ? pos - a.window + 1 : 0);
+            const int hi = min(k_lo + tile_end * KT - 1, pos);
+            attend_scalar<T>(q + (int64_t)(t0 + tok) * a.q_stride + (int64_t)(g * GS + p - tok * GS) * HD, a, table, g, lo, hi,
+                             acc, sm_ml, smem);
+            for (int d = tid; d < HD; d += THREADS) leave(i, d, acc[d], sm_ml[2 * WARPS], sm_ml[2 * WARPS + 1]);
+            __syncthreads();
+        }
+    }
+}
+
+// Joins the splits: a warp per token and head.  grid (tokens of a row x heads / 4, rows).
+template <typename T>
+__global__ void __launch_bounds__(128) attn_q8_merge_kernel(T* __restrict__ out, const Q8Args a) {
+    pdl_wait();
+    pdl_trigger();
+    const int r = a.row_list ? a.row_list[blockIdx.y] : blockIdx.y, lane = threadIdx.x & 31;
+    const int at = blockIdx.x * 4 + threadIdx.x / 32, tok = at / a.H, h = at - tok * a.H;
+    const int t0 = a.row_start[r];
+    if (tok >= a.row_start[r + 1] - t0 || t0 + tok >= a.part_tokens) return;
+    const int64_t ld = HD + 2;
+    const float* part = a.part + ((int64_t)(t0 + tok) * a.H + h) * a.n_splits * ld;
+    float top = LOWEST, total = 0.f, sum[DPL];
+    for (int k = lane; k < a.n_splits; k += 32) top = fmaxf(top, part[k * ld + HD]);
+    top = warp_max(top);
+#pragma unroll
+    for (int c = 0; c < DPL; ++c) sum[c] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < a.n_splits; ++k) {
+        const float f = ex2(part[k * ld + HD] - top);
+        total += part[k * ld + HD + 1] * f;
+#pragma unroll
+        for (int c = 0; c < DPL; ++c)
+            if (lane + 32 * c < HD) sum[c] += part[k * ld + lane + 32 * c] * f;
+    }
 #pragma unroll
     for (int c = 0; c < DPL; ++c)
         if (lane + 32 * c < HD)
-            out[token * a.out_stride + (int64_t)h * HD + lane + 32 * c] = from_float<T>(l != 0.f ? o[c] / l : 0.f);
+            out[(int64_t)(t0 + tok) * a.out_stride + (int64_t)h * HD + lane + 32 * c] =
+                from_float<T>(total == 0.f ? 0.f : sum[c] / total);
+}
+
+template <typename T, int NT>
+static int launch(const T* q, T* out, const Q8Args& a, int n_list, int max_new, int q_tiles, cudaStream_t stream) {
+    const size_t smem = Form<T, NT>::smem();
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    e = sllm_launch_pdl(attn_q8_kernel<T, NT>, dim3(a.G, a.n_splits * q_tiles, n_list), dim3(THREADS), smem, stream, q, out, a);
+    if (e != cudaSuccess || a.n_splits == 1) return (int)e;
+    return (int)sllm_launch_pdl(attn_q8_merge_kernel<T>, dim3(((int64_t)max_new * a.H + 3) / 4, n_list), dim3(128), 0, stream,
+                                out, a);
+}
+
+template <typename T, int NT> static int slots() {
+    int device = 0, sms = 0, per = 0;
+    if (cudaGetDevice(&device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+        cudaFuncSetAttribute(attn_q8_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)Form<T, NT>::smem()) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attn_q8_kernel<T, NT>, THREADS, Form<T, NT>::smem()) !=
+            cudaSuccess)
+        return 0;
+    return sms * per;
 }
 
 }  // namespace sllm
 
 using namespace sllm;
 
+// CTAs that the device holds at once, of the form for 8 (nt = 1) or 16 (nt = 2) queries a warp; 0: not known.
+SLLM_EXPORT int sllm_attn_q8_slots(int dtype, int nt) {
+    if (dtype == 0) return nt == 1 ? slots<float, 1>() : slots<float, 2>();
+    return nt == 1 ? slots<__nv_bfloat16, 1>() : slots<__nv_bfloat16, 2>();
+}
+// keys of a warp's tile
+SLLM_EXPORT int sllm_attn_q8_tile(int dtype, int nt) {
+    if (dtype == 0) return nt == 1 ? Form<float, 1>::KT : Form<float, 2>::KT;
+    return nt == 1 ? Form<__nv_bfloat16, 1>::KT : Form<__nv_bfloat16, 2>::KT;
+}
+
+// nt: queries a warp / 8; wq: groups of queries of a CTA (1, 2 or 4).  part: n_splits > 1 only, float
+// [part_tokens, H, n_splits, HD + 2].
 SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages, const void* scales, const int* table,
                              int table_stride, int page_size, int block, const int* row_start, const int* row_pos0,
                              const int* row_list, int n_list, int max_new, void* out, int64_t out_stride, int H, int G,
-                             float scale, int window, int dtype, cudaStream_t stream) {
+                             float scale, int window, int dtype, int nt, int wq, int n_splits, float* part,
+                             int64_t part_tokens, cudaStream_t stream) {
     if (n_list <= 0 || max_new <= 0) return 0;
     if (H <= 0 || G <= 0 || H % G || page_size <= 0 || block <= 0 || page_size % block || window < 0 || n_list > 65535 ||
-        (dtype != 0 && dtype != 1))
+        (dtype != 0 && dtype != 1) || (nt != 1 && nt != 2) || (wq != 1 && wq != 2 && wq != 4) || n_splits < 1 ||
+        (n_splits > 1 && part == nullptr) || ((uintptr_t)pages & 15))
         return (int)cudaErrorInvalidValue;
+    const int64_t q_tiles = ((int64_t)max_new * (H / G) + 8 * nt * wq - 1) / (8 * nt * wq);
+    if (q_tiles * n_splits > 65535 || (int64_t)max_new * H > (1u << 30)) return (int)cudaErrorInvalidValue;
+    const int es = dtype == 0 ? 4 : 2;
+    const int q_vec = (uintptr_t)q % (4 * es) == 0 && q_stride % 4 == 0;
     const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
-                      table_stride, page_size, block, H, G, window, scale};
-    const dim3 grid(max_new, n_list, (H + 3) / 4);
+                      part, part_tokens, table_stride, page_size, block, H, G, window, n_splits, wq, q_vec, scale * LOG2E};
+    typedef __nv_bfloat16 bf16;
     if (dtype == 0)
-        return (int)sllm_launch_pdl(attn_q8_kernel<float>, grid, dim3(128), 0, stream, (const float*)q, (float*)out, a);
-    return (int)sllm_launch_pdl(attn_q8_kernel<__nv_bfloat16>, grid, dim3(128), 0, stream, (const __nv_bfloat16*)q,
-                                (__nv_bfloat16*)out, a);
+        return nt == 1 ? launch<float, 1>((const float*)q, (float*)out, a, n_list, max_new, (int)q_tiles, stream)
+                       : launch<float, 2>((const float*)q, (float*)out, a, n_list, max_new, (int)q_tiles, stream);
+    return nt == 1 ? launch<bf16, 1>((const bf16*)q, (bf16*)out, a, n_list, max_new, (int)q_tiles, stream)
+                   : launch<bf16, 2>((const bf16*)q, (bf16*)out, a, n_list, max_new, (int)q_tiles, stream);
 }

@@ -12,6 +12,7 @@ and a lazy dispatch table (src/scratch_llm/kernels/attention/dispatch.py:68-90).
 from __future__ import annotations
 
 import ctypes
+import functools
 from ctypes import c_float, c_int, c_int64, c_void_p
 from typing import Sequence
 
@@ -951,6 +952,8 @@ def _q8_cache(pages: torch.Tensor, scales: torch.Tensor, n_kv_heads: int, page_s
     block = page_size // scales.shape[3]
     if block * head_dim > Q8_MAX_BLOCK_ENTRIES:
         raise KernelError(f"blocks of {block} tokens of {head_dim} entries: at most {Q8_MAX_BLOCK_ENTRIES} entries")
+    if not 1 <= pages.shape[0] <= (1 << 32) // (2 * n_kv_heads * page_size) - 1:
+        raise KernelError(f"{pages.shape[0]} pages: from one page to 2^32 keys and values of a head are taken")
     if pages.data_ptr() % 16:
         raise KernelError("pages must start on a 16-byte boundary")
     return block
@@ -1030,6 +1033,35 @@ def kv_read_q8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Ten
     return out
 
 
+@functools.lru_cache(maxsize=64)
+def _attention_q8_form(device: int, head_dim: int, code: int, nt: int) -> tuple[int, int]:
+    """(CTAs that the device holds at once, keys of a warp's tile) of the form for ``8 * nt`` queries a warp."""
+    lib = _load(*attention_q8_library(head_dim))
+    slots = int(lib.sllm_attn_q8_slots(c_int(code), c_int(nt)))
+    if slots <= 0:
+        raise KernelError("the occupancy of the 8-bit attention kernel could not be read")
+    return slots, int(lib.sllm_attn_q8_tile(c_int(code), c_int(nt)))
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_new: int, max_context: int, n_heads: int,
+                       n_kv_heads: int, window: int) -> tuple[int, int, int]:
+    """How a launch is shared out: (queries a warp / 8, groups of queries of a CTA, CTAs along the keys)."""
+    packed = max_new * (n_heads // n_kv_heads)
+    nt = 1 if packed <= 8 else 2
+    wq = 1 if packed <= 8 * nt else 2 if packed <= 16 * nt else 4
+    slots, tile = _attention_q8_form(device, head_dim, code, nt)
+    base = n_list * n_kv_heads * -(-packed // (8 * nt * wq))
+    keys = min(max_context, window + max_new) if window else max_context
+    turns = max(1, -(-keys // (tile * (4 // wq))))        # tiles of a warp without splits
+    best, best_cost = 1, None
+    for n in range(1, min(64, turns) + 1):
+        cost = -(-base * n // slots) * (-(-turns // n) + 2) + (0.1 * n + 1 if n > 1 else 0)
+        if best_cost is None or cost < best_cost:
+            best, best_cost = n, cost
+    return nt, wq, best
+
+
 def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, page_size: int,
                  row_start: torch.Tensor, row_pos0: torch.Tensor, out: torch.Tensor, row_list: torch.Tensor | None,
                  n_list: int, max_new: int, max_context: int, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
@@ -1055,11 +1087,19 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
         raise KernelError(f"window must not be negative, got {window}")
     _here(q=q, pages=pages, scales=scales, block_table=block_table, row_start=row_start, row_pos0=row_pos0, out=out,
           row_list=row_list)
+    if n_list <= 0 or max_new <= 0:
+        return out
+    nt, wq, n_splits = _attention_q8_plan(q.get_device(), head_dim, _code(q.dtype), n_list, max_new, max_context, n_heads,
+                                          n_kv_heads, window or 0)
+    part = None
+    if n_splits > 1:
+        part = torch.empty(q.shape[0] * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
     _check(_load(*attention_q8_library(head_dim)).sllm_attn_q8(
         _ptr(q), c_int64(q.stride(0)), _ptr(pages), _ptr(scales), _ptr(block_table), c_int(block_table.stride(0)),
         c_int(page_size), c_int(block), _ptr(row_start), _ptr(row_pos0), _ptr(row_list), c_int(n_list), c_int(max_new),
         _ptr(out), c_int64(out.stride(0)), c_int(n_heads), c_int(n_kv_heads), c_float(scale), c_int(window or 0),
-        c_int(_code(q.dtype)), _stream()), "attention_q8")
+        c_int(_code(q.dtype)), c_int(nt), c_int(wq), c_int(n_splits), _ptr(part), c_int64(q.shape[0]), _stream()),
+        "attention_q8")
     return out
 
 
