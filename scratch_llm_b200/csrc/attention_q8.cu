@@ -4,9 +4,11 @@
 //   s_j = scale * q . k_j,   out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s)
 // Compiled once per head size: -DSLLM_HEAD_DIM=<multiple of 16, at most 256>.
 //
-// Numbers.  An e4m3 number is a half exactly, and one instruction turns two of them, so the products run on the tensor
-// cores' f16 form with the cache's numbers as they are; the blocks' powers of two join the scores (2^ek) and the
-// probabilities (2^ev) in 32 bits.  A query is brought into f16's range by a power of two of its own (largest entry
+// Numbers.  An e4m3 number's bits, moved to a half's places, are that number times 2^-8 (subnormal ones too), so the
+// products run on the tensor cores' f16 form with the cache's numbers as they are: seven bit operations for four of
+// them (the conversion instruction takes the special-function pipe for as long as eight: 64 rows of 4,096 keys, 32
+// heads of 128 on 8 kv heads, 225 us with it).  The blocks' powers of two join the scores (2^ek) and the probabilities
+// (2^ev) in 32 bits.  A NaN's bits would count as 480: a CTA that meets one takes its queries again key after key.  A query is brought into f16's range by a power of two of its own (largest entry
 // in [2^14, 2^15)): bfloat16 entries keep all their bits down to 2^-38 of the largest, 32-bit ones are split into two
 // halves (22 bits).  A probability is multiplied by its key's 2^ev before it becomes a half, against a running
 // maximum of its own, M = max(s + ev): what counts towards the output keeps 11 bits (22 in the 32-bit form) down
@@ -15,11 +17,14 @@
 // Layout.  The products are taken transposed, keys and then the values' entries as the 16 rows of mma.m16n8k16, queries as
 // its 8 columns: a decoded token's group of up to 8 query heads fills the instruction, and an output is spread over
 // half as many registers.  Which entry of a head stands in which k step is free as long as queries and keys agree:
-// a lane takes a quarter of each key's bytes as they lie, and of the values an eighth of four keys, so keys and values come
-// from global memory straight into the operands' registers, a whole line a request, with no shared memory between.
-// P becomes an operand by movmatrix.  The next tile's keys are requested once this tile's have met the queries, its
-// values once these are used: half of a warp's registers are always on their way.
+// a lane takes a quarter of each key's bytes as they lie, and of the values an eighth of four keys; P becomes an operand
+// by movmatrix.  Every warp fills a ring of its own in shared memory by TMA (one request per plane and tile where a
+// page holds whole tiles, else one per run of keys), so that no warp waits for another before the end, and 16 KB a warp
+// are on their way while it works (requested straight into registers, half a tile at a time, 64 rows of 4,096 keys
+// took 210 us: the loads' latency).  128-byte (heads of 64: 64-byte) swizzle: no two lanes of a read meet in a bank.
+// Other heads, and pages of no whole eights of tokens, come by untiled bulk copies, as they lie.
 #include "q8.cuh"
+#include "tc_common.cuh"
 
 #ifndef SLLM_HEAD_DIM
 #error "compile with -DSLLM_HEAD_DIM=<head size>"
@@ -39,14 +44,36 @@ constexpr float LOWEST = -1e30f;                         // below every score; f
 constexpr float STALE = 8.f;                             // how far a maximum may lag behind the scores (base 2)
 constexpr float P_SHIFT = 6.f;                           // probabilities become halves times 2^6: 2^14 at most
 
+// n / d for 0 <= n < 2^31: 2 n * ceil(2^(31 + s) / d) / 2^(32 + s), 2^s >= d
+struct Divisor {
+    uint32_t magic; int shift, d;
+    __device__ __forceinline__ int quotient(int n) const { return (int)(__umulhi(2u * (uint32_t)n, magic) >> shift); }
+};
+static Divisor divisor(int d) {
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s, d};
+}
+
 struct Q8Args {
     int64_t q_stride, out_stride;
     const uint8_t* pages; const uint8_t* scales; const int* table;
     const int* row_start; const int* row_pos0; const int* row_list;
     float* part; int64_t part_tokens;                    // [tokens, H, n_splits, HD + 2]: sums, maximum, denominator
-    int table_stride, page_size, block, H, G, window, n_splits, wq, q_vec;
+    int table_stride, page_size, block, H, G, window, n_splits, wq, q_vec, run, tiled;
     float scale_log2;
+    Divisor page_div, block_div;
 };
+
+constexpr bool WIDE = HD % 128 == 0;                     // a tile is columns of 128 bytes, each [KT][128]
+constexpr bool CAN_TILE = WIDE || HD == 64;
+constexpr int WIDTH = WIDE ? 128 : HD;
+// where byte b of a key (or value) lies in a tile of KT rows
+template <int KT> __device__ __forceinline__ int place(int row, int b, bool swizzled) {
+    if constexpr (WIDE) return (b / 128) * KT * 128 + row * 128 + ((b % 128 / 16 ^ (swizzled ? row & 7 : 0)) << 4) + b % 16;
+    else if constexpr (HD == 64) return row * 64 + ((b / 16 ^ (swizzled ? row >> 1 & 3 : 0)) << 4) + b % 16;
+    else return row * HD + b;
+}
 
 template <typename T, int NT> struct Form {
     static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;           // halves that an operand of T is split into
@@ -54,9 +81,14 @@ template <typename T, int NT> struct Form {
     static constexpr int Q_REGS = NT * PARTS * KSTEPS * 2;
     static constexpr bool Q_SHARED = Q_REGS > 32;
     static constexpr int LD = HD + 4;
-    static constexpr size_t merge_bytes() { return sizeof(float) * WARPS * 8 * NT * LD; }
-    static constexpr size_t q_bytes() { return Q_SHARED ? sizeof(uint32_t) * WARPS * 32 * Q_REGS : 0; }
-    static constexpr size_t smem() { return merge_bytes() > q_bytes() ? merge_bytes() : q_bytes(); }
+    static constexpr int STAGE = 2 * KT * HD;                     // bytes of a tile: keys, then values
+    static constexpr int STAGES = NT == 1 ? (STAGE >= 8192 ? 2 : 4) : (STAGE >= 8192 ? 3 : 4);
+    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int MERGE = (int)sizeof(float) * WARPS * 8 * NT * LD;
+    static constexpr int Q_BYTES = Q_SHARED ? (int)sizeof(uint32_t) * WARPS * 32 * Q_REGS : 0;
+    // the ring (at its end the meeting of the warps takes its place), then the queries
+    static constexpr int Q_AT = RING > MERGE ? RING : (MERGE + 1023) / 1024 * 1024;
+    static constexpr size_t smem() { return 1024 + Q_AT + Q_BYTES; }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -85,32 +117,50 @@ __device__ __forceinline__ uint32_t halves_rest(float a, float b, uint32_t h) {
     return halves(a - f.x, b - f.y);
 }
 
-// BYTES from global memory into words, in the widest loads that every lane's address allows
-template <int BYTES, int N> __device__ __forceinline__ void fetch(const uint8_t* p, uint32_t (&w)[N]) {
+// Bytes 1 and 3 of a word, and bytes 0 and 2, as pairs of halves: the numbers times 2^-8.  `top`: the largest
+// of their bits without the sign; a NaN's are 0x3f80, the largest number's 0x3f00.
+__device__ __forceinline__ void halves_of(uint32_t w, uint32_t& odd, uint32_t& even, uint32_t& top) {
+    const uint32_t a = w >> 1 & 0x3f803f80u, b = w << 7 & 0x3f803f80u;
+    odd = (w & 0x80008000u) | a;
+    even = (w << 8 & 0x80008000u) | b;
+    top = __vimax3_u16x2(top, a, b);
+}
+__device__ __forceinline__ bool any_nan(uint32_t top) { return (top & 0xffffu) >= 0x3f80u || top >> 16 >= 0x3f80u; }
+
+// BYTES of shared memory into words; where they lie in pieces of 16 bytes, piece i at p[i]
+template <int BYTES, int N> __device__ __forceinline__ void take(const uint8_t* const (&p)[(BYTES + 15) / 16], int off, uint32_t (&w)[N]) {
     if constexpr (BYTES % 16 == 0) {
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) {
-            const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            const uint4 x = *reinterpret_cast<const uint4*>(p[i] + off);
             w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
         }
     } else if constexpr (BYTES % 8 == 0) {
 #pragma unroll
         for (int i = 0; i < BYTES / 8; ++i) {
-            const uint2 x = __ldg(reinterpret_cast<const uint2*>(p) + i);
+            const uint2 x = *reinterpret_cast<const uint2*>(p[0] + off + 8 * i);
             w[2 * i] = x.x; w[2 * i + 1] = x.y;
         }
     } else if constexpr (BYTES % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < BYTES / 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+        for (int i = 0; i < BYTES / 4; ++i) w[i] = *reinterpret_cast<const uint32_t*>(p[0] + off + 4 * i);
     } else {
 #pragma unroll
-        for (int i = 0; i < BYTES / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint16_t*>(p) + i);
+        for (int i = 0; i < BYTES / 2; ++i) w[i] = *reinterpret_cast<const uint16_t*>(p[0] + off + 2 * i);
     }
 }
 
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
 // One query over the keys lo .. hi that it sees, key after key, by all warps of the CTA: sums relative to m (base 2) in
-// acc [HD], and (m, l).  For tiles in which a NaN came out: a tensor-core product multiplies also what a query does
-// not see by zero, and zero times a NaN is one.
+// acc [HD], and (m, l).  For tiles that hold a NaN: it belongs to the queries that see it and to no other.
 template <typename T>
 __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args& a, const int* __restrict__ table, int g,
                                            int lo, int hi, float* acc, float* ml, float* smem) {
@@ -166,11 +216,15 @@ __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args
 // grid (kv heads, splits x tiles of queries, rows), the tiles with the most keys first.
 template <typename T, int NT>
 __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
-attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
+attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_constant__ CUtensorMap map, const Q8Args a) {
     using F = Form<T, NT>;
-    constexpr int PARTS = F::PARTS, KT = F::KT, KG = KT / 16, LD = F::LD;
-    extern __shared__ __align__(16) float smem[];
+    constexpr int PARTS = F::PARTS, KT = F::KT, KG = KT / 16, LD = F::LD, STAGES = F::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    float* smem = reinterpret_cast<float*>(ring);
+    __shared__ uint64_t full[WARPS][STAGES];
     __shared__ float sm_m[WARPS][8 * NT], sm_l[WARPS][8 * NT], sm_ml[2 * WARPS + 2];
+    __shared__ int some_nan;
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n8 = lane >> 2, c4 = lane & 3;
@@ -192,8 +246,8 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
     const int w0 = q0 + (warp % wq) * 8 * NT, w_nq = min(8 * NT, q0 + nq - w0);     // (w_nq may be 0 or less)
     const int w_first = pos0 + w0 / GS, w_last = pos0 + (w0 + max(w_nq, 1) - 1) / GS;
     uint32_t qf[F::Q_SHARED ? 1 : PARTS][F::Q_SHARED ? 1 : NT][F::Q_SHARED ? 1 : KSTEPS][2];
-    uint2* q_sh = reinterpret_cast<uint2*>(smem) + warp * (F::Q_REGS / 2) * 32 + lane;   // [part][nt][ks][lane]
-    float fq[NT][2];                      // scale * log2 e / the query's power of two, of queries 2 c4 and 2 c4 + 1
+    uint2* q_sh = reinterpret_cast<uint2*>(ring + F::Q_AT) + warp * (F::Q_REGS / 2) * 32 + lane;   // [part][nt][ks][lane]
+    float fq[NT][2];                      // 2^8 * scale * log2 e / the query's power of two, of queries 2 c4 and 2 c4 + 1
     int qpos[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -227,7 +281,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
         // 2^k with top * 2^k in [2^14, 2^15); at most 2^100, so that its inverse times the scale is a normal number
         const int k = top > 0.f ? min(100, 14 + 127 - (__float_as_int(top) >> 23)) : 0;
         const float up = __int_as_float((k + 127) << 23);
-        const float own = a.scale_log2 * __int_as_float((127 - k) << 23);
+        const float own = a.scale_log2 * __int_as_float((127 + 8 - k) << 23);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             fq[nt][e] = __shfl_sync(0xffffffffu, own, (2 * c4 + e) * 4);
@@ -236,7 +290,8 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
         }
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks) {
-            const float y0 = x[4 * ks] * up, y1 = x[4 * ks + 1] * up, y2 = x[4 * ks + 2] * up, y3 = x[4 * ks + 3] * up;
+            // (the order in which a key's word gives its bytes)
+            const float y0 = x[4 * ks + 1] * up, y1 = x[4 * ks + 3] * up, y2 = x[4 * ks] * up, y3 = x[4 * ks + 2] * up;
             const uint32_t h0 = halves(y0, y1), h1 = halves(y2, y3);
             uint32_t r0 = 0, r1 = 0;
             if constexpr (PARTS == 2) {
@@ -264,59 +319,94 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
         for (int e = 0; e < 2; ++e) { m[nt][e] = M[nt][e] = LOWEST; l[nt][e] = 0.f; }
     }
 
-    // ---- where a tile's keys lie: lane i looks up key i (page, then its two scales) and tells the others
+    // ---- the ring: lane i looks up key i of a tile (its page, then its two scales); where a page holds whole tiles lane
+    // 0 requests them, else lane i the i-th run of `run` keys
     const int blocks = a.page_size / a.block;
-    const uint32_t v_rows = (uint32_t)a.G * a.page_size;
     int tile_stop = tile_end;             // this warp's queries see nothing from here on
     if (w_nq <= 0) tile_stop = tile_begin;
     else tile_stop = min(tile_stop, (w_last - k_lo) / KT + 1);
+    uint8_t* stages = ring + warp * STAGES * F::STAGE;
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) mbar_init(&full[warp][i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    }
+    if (tid == 0) some_nan = 0;
+    __syncwarp();
     auto page_of = [&](int tile) {
         const int kpos = k_lo + tile * KT + lane % KT;
-        return tile < tile_stop && kpos <= w_last ? __ldg(table + kpos / a.page_size) : -1;
+        return tile < tile_stop && kpos <= w_last ? __ldg(table + a.page_div.quotient(kpos)) : -1;
     };
-    auto row_of = [&](int tile, int page) {       // the key's row among all rows of HD bytes (at most 2^32 - 2), ~0: none
-        const int off = (k_lo + tile * KT + lane % KT) % a.page_size;
-        return page >= 0 ? ((uint32_t)page * 2u * a.G + g) * a.page_size + off : 0xffffffffu;
-    };
-    auto scales_of = [&](int tile, int page) {
-        if (page < 0) return 127 | 127 << 8;
-        const int off = (k_lo + tile * KT + lane % KT) % a.page_size;
-        const uint8_t* s = a.scales + ((int64_t)page * 2 * a.G + g) * blocks + off / a.block;
+    // requests a tile and returns the bytes of this lane's two scales; -1: no such key
+    auto request = [&](int tile, int page, int stage) {
+        const int kpos = k_lo + tile * KT + lane % KT, off = kpos - a.page_div.quotient(kpos) * a.page_size;
+        const int from = lane * a.run % KT;                    // the first key of this lane's run
+        const int run_page = __shfl_sync(0xffffffffu, page, from), run_off = __shfl_sync(0xffffffffu, off, from);
+        const bool mine = lane * a.run < KT && run_page >= 0;
+        const uint32_t asked = __ballot_sync(0xffffffffu, mine);
+        const uint32_t bar = smem_u32(&full[warp][stage]);
+        if (lane == 0) mbar_expect_tx(&full[warp][stage], (uint32_t)__popc(asked) * 2u * a.run * HD);
+        __syncwarp();
+        if (mine) {
+            const uint32_t dst = smem_u32(stages + stage * F::STAGE) + lane * a.run * WIDTH;
+            const int plane = run_page * 2 * a.G + g;
+            if (CAN_TILE && a.tiled) {
+#pragma unroll
+                for (int x = 0; x < HD; x += WIDTH) {
+                    tma_load_3d(dst + x * KT, &map, bar, x, run_off, plane);
+                    tma_load_3d(dst + x * KT + KT * HD, &map, bar, x, run_off, plane + a.G);
+                }
+            } else {
+                const uint8_t* src = a.pages + ((int64_t)plane * a.page_size + run_off) * HD;
+                const int64_t v_off = (int64_t)a.G * a.page_size * HD;
+                if constexpr (HD == WIDTH) {
+                    bulk_load(dst, src, a.run * HD, bar);
+                    bulk_load(dst + KT * HD, src + v_off, a.run * HD, bar);
+                } else {
+                    for (int i = 0; i < a.run; ++i)
+#pragma unroll
+                        for (int x = 0; x < HD; x += WIDTH) {
+                            bulk_load(dst + x * KT + i * WIDTH, src + i * HD + x, WIDTH, bar);
+                            bulk_load(dst + x * KT + i * WIDTH + KT * HD, src + v_off + i * HD + x, WIDTH, bar);
+                        }
+                }
+            }
+        }
+        if (page < 0) return -1;
+        const uint8_t* s = a.scales + ((int64_t)page * 2 * a.G + g) * blocks + a.block_div.quotient(off);
         return (int)__ldg(s) | (int)__ldg(s + (int64_t)a.G * blocks) << 8;
     };
-    uint32_t kr[2 * KG][KSTEPS], vr[KG][4][VREGS];
-    auto fetch_keys = [&](uint32_t row) {         // (a key that is not there: some row of the cache, masked below)
+    // where this lane's pieces of a key (rows n8 + 8 i) and of a value (rows 2 c4, 2 c4 + 1, and 8 i on) lie in a stage
+    const uint8_t* k_at[(HD / 4 + 15) / 16];
+    const uint8_t* v_at[2][(HD / 8 + 15) / 16];
 #pragma unroll
-        for (int i = 0; i < 2 * KG; ++i) {
-            const uint32_t at = __shfl_sync(0xffffffffu, row, n8 + 8 * i);
-            fetch<HD / 4>(a.pages + (size_t)(at == 0xffffffffu ? 0u : at) * HD + c4 * (HD / 4), kr[i]);
-        }
-    };
-    auto fetch_values = [&](uint32_t row) {       // (a value that is not there: zeros)
+    for (int i = 0; i < (HD / 4 + 15) / 16; ++i) k_at[i] = stages + place<KT>(n8, c4 * (HD / 4) + 16 * i, a.tiled);
 #pragma unroll
-        for (int i = 0; i < KG; ++i)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t at = __shfl_sync(0xffffffffu, row, 16 * i + 2 * c4 + (k & 1) + 8 * (k >> 1));
-#pragma unroll
-                for (int w = 0; w < VREGS; ++w) vr[i][k][w] = 0u;
-                if (at != 0xffffffffu)
-                    fetch<HD / 8>(a.pages + ((size_t)at + v_rows) * HD + n8 * (HD / 8), vr[i][k]);
-            }
-    };
+        for (int i = 0; i < (HD / 8 + 15) / 16; ++i)
+            v_at[k][i] = stages + KT * HD + place<KT>(2 * c4 + k, n8 * (HD / 8) + 16 * i, a.tiled);
+    constexpr int EIGHT = 8 * WIDTH;         // eight rows
 
-    int tile = tile_begin + warp / wq;
-    int page = page_of(tile), page_next = page_of(tile + wk);
-    uint32_t row = row_of(tile, page), row_next = row_of(tile + wk, page_next);
-    int sc = scales_of(tile, page), sc_next = scales_of(tile + wk, page_next);
-    if (tile < tile_stop) {
-        fetch_keys(row);
-        fetch_values(row);
+    int tile = tile_begin + warp / wq, sc[STAGES];
+    bool nan_seen = false, ok = true;
+    {
+        int page[STAGES];
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) page[i] = page_of(tile + i * wk);
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i)
+            sc[i] = tile + i * wk < tile_stop ? request(tile + i * wk, page[i], i) : -1;
     }
-    int page_after = page_of(tile + 2 * wk);
+    int page_after = page_of(tile + STAGES * wk), stage = 0, parity = 0;
 
     for (; tile < tile_stop; tile += wk) {
         const int kt = k_lo + tile * KT;
+        ok = mbar_wait(&full[warp][stage], parity, 1);
+        if (!ok) break;
+        const int at = stage * F::STAGE;
+        uint32_t top_bits = 0u;
         // ---- scores, transposed: rows are keys, columns queries
         float s[KG][NT][4];
 #pragma unroll
@@ -325,6 +415,9 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[i][nt][e] = 0.f;
+        uint32_t kr[2 * KG][KSTEPS];
+#pragma unroll
+        for (int i = 0; i < 2 * KG; ++i) take<HD / 4>(k_at, at + i * EIGHT, kr[i]);
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks) {
             uint32_t b[PARTS][NT][2];
@@ -341,19 +434,19 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
                 }
 #pragma unroll
             for (int i = 0; i < KG; ++i) {
-                const uint32_t f[4] = {q8_half2(kr[2 * i][ks] & 0xffffu), q8_half2(kr[2 * i + 1][ks] & 0xffffu),
-                                       q8_half2(kr[2 * i][ks] >> 16), q8_half2(kr[2 * i + 1][ks] >> 16)};
+                uint32_t f[4];
+                halves_of(kr[2 * i][ks], f[0], f[2], top_bits);
+                halves_of(kr[2 * i + 1][ks], f[1], f[3], top_bits);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int part = PARTS - 1; part >= 0; --part) mma_f16(s[i][nt], f, b[part][nt][0], b[part][nt][1]);
             }
         }
-        const bool whole = __all_sync(0xffffffffu, row != 0xffffffffu) && kt + KT - 1 <= w_first &&
-                           (a.window <= 0 || kt > w_last - a.window);
+        const bool there = sc[0] >= 0;
+        const bool whole = __all_sync(0xffffffffu, there) && kt + KT - 1 <= w_first && (a.window <= 0 || kt > w_last - a.window);
         uint32_t seen_rows = 0;
-        if (!whole) seen_rows = __ballot_sync(0xffffffffu, row != 0xffffffffu);
-        if (tile + wk < tile_stop) fetch_keys(row_next);
+        if (!whole) seen_rows = __ballot_sync(0xffffffffu, there);
 
         // ---- scaled scores, their maxima
         float ev[KG][2];                  // the values' exponents of this lane's keys
@@ -362,9 +455,9 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int key = 16 * i + 8 * k + n8;
-                const int both = __shfl_sync(0xffffffffu, sc, key);
+                const int both = __shfl_sync(0xffffffffu, sc[0], key);
                 const float fk = __int_as_float((both & 0xff) << 23);
-                ev[i][k] = (float)(both >> 8) - 127.f;
+                ev[i][k] = (float)(both >> 8 & 0xff) - 127.f;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -442,27 +535,45 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
                 }
         // ---- sums over the keys, transposed: rows are entries of a head
 #pragma unroll
-        for (int i = 0; i < KG; ++i)
+        for (int i = 0; i < KG; ++i) {
+            uint32_t vr[4][VREGS];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) take<HD / 8>(v_at[k & 1], at + (2 * i + (k >> 1)) * EIGHT, vr[k]);
 #pragma unroll
             for (int j = 0; j < KSTEPS; ++j) {
-                constexpr uint32_t LOW = 0x5140, HIGH = 0x7362;
+                // (bytes 1 and 3: entry 2 j of two keys, bytes 0 and 2: entry 2 j + 1)
+                constexpr uint32_t LOW = 0x4501, HIGH = 0x6723;
                 const int w = V_WORDS ? j / 2 : j;
                 const uint32_t pick = V_WORDS && (j & 1) ? HIGH : LOW;
-                const uint32_t x = __byte_perm(vr[i][0][w], vr[i][1][w], pick);
-                const uint32_t y = __byte_perm(vr[i][2][w], vr[i][3][w], pick);
-                const uint32_t f[4] = {q8_half2(x & 0xffffu), q8_half2(x >> 16), q8_half2(y & 0xffffu), q8_half2(y >> 16)};
+                const uint32_t x = __byte_perm(vr[0][w], vr[1][w], pick);
+                const uint32_t y = __byte_perm(vr[2][w], vr[3][w], pick);
+                uint32_t f[4];
+                halves_of(x, f[0], f[1], top_bits);
+                halves_of(y, f[2], f[3], top_bits);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int part = PARTS - 1; part >= 0; --part)
                         mma_f16(o[j][nt], f, p[part][i][nt][0], p[part][i][nt][1]);
             }
-        if (tile + wk < tile_stop) fetch_values(row_next);
-        row = row_next;
-        sc = sc_next;
-        row_next = row_of(tile + 2 * wk, page_after);
-        sc_next = scales_of(tile + 2 * wk, page_after);
-        page_after = page_of(tile + 3 * wk);
+        }
+        if (__any_sync(0xffffffffu, any_nan(top_bits))) {
+            // (the tile's places without a key may hold anything: what counts are this lane's own keys)
+            if (whole) nan_seen = true;
+            else if (there && lane < KT)
+                for (int b = 0; b < HD; b += 2)
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        const uint32_t w = *reinterpret_cast<const uint16_t*>(stages + at + v * KT * HD + place<KT>(lane, b, a.tiled));
+                        nan_seen |= (w & 0x7f) == 0x7f || (w >> 8 & 0x7f) == 0x7f;
+                    }
+        }
+        __syncwarp();                     // (the stage is read)
+#pragma unroll
+        for (int i = 0; i + 1 < STAGES; ++i) sc[i] = sc[i + 1];
+        sc[STAGES - 1] = tile + STAGES * wk < tile_stop ? request(tile + STAGES * wk, page_after, stage) : -1;
+        page_after = page_of(tile + (STAGES + 1) * wk);
+        if (++stage == STAGES) { stage = 0; parity ^= 1; }
     }
 
     // ---- the groups of keys meet
@@ -477,7 +588,8 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
                 sm_l[warp][nt * 8 + 2 * c4 + e] = l[nt][e];
             }
         }
-    __syncthreads();                      // (and the queries in shared memory are done with)
+    __syncthreads();                      // (all rings are done with)
+    if (nan_seen) some_nan = 1;
     float* sums = smem;                   // [WARPS][8 NT][LD]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -486,7 +598,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
             const int i = nt * 8 + 2 * c4 + e;
             float top = LOWEST;
             for (int w = warp % wq; w < WARPS; w += wq) top = fmaxf(top, sm_m[w][i]);
-            const float f = ex2(M[nt][e] - P_SHIFT - top);
+            const float f = ex2(M[nt][e] + (8.f - P_SHIFT) - top);
             float* to = sums + (warp * 8 * NT + i) * LD + n8 * (HD / 8);
 #pragma unroll
             for (int j = 0; j < KSTEPS; ++j)
@@ -504,7 +616,6 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
             if (d == 0) { part[HD] = top; part[HD + 1] = total; }
         }
     };
-    bool odd = false;
     for (int idx = tid; idx < nq * HD; idx += THREADS) {
         const int i = idx / HD, d = idx - i * HD, group = i / (8 * NT), j = i - group * 8 * NT;
         float top = LOWEST, total = 0.f, sum = 0.f;
@@ -513,11 +624,10 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const Q8Args a) {
             total += sm_l[w][j] * ex2(sm_m[w][j] - top);
             sum += sums[(w * 8 * NT + j) * LD + d];
         }
-        odd |= isnan(sum) || isnan(total);
         leave(i, d, sum, top, total);
     }
-    // a NaN, and not all queries see the same keys: each of them by itself
-    if (__syncthreads_or(odd) && first_pos != last_pos) {
+    __syncthreads();
+    if (some_nan) {                       // each query by itself
         float* acc = smem + WARPS * HD;
         static_assert((WARPS + 1) * HD <= WARPS * 8 * LD, "room for the scalar form");
         for (int i = 0; i < nq; ++i) {
@@ -563,12 +673,46 @@ __global__ void __launch_bounds__(128) attn_q8_merge_kernel(T* __restrict__ out,
                 from_float<T>(total == 0.f ? 0.f : sum[c] / total);
 }
 
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encode_fn() {
+    static EncodeFn fn = nullptr;
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) == cudaSuccess &&
+            found == cudaDriverEntryPointSuccess)
+            fn = (EncodeFn)p;
+    }
+    return fn;
+}
+
 template <typename T, int NT>
-static int launch(const T* q, T* out, const Q8Args& a, int n_list, int max_new, int q_tiles, cudaStream_t stream) {
+static int launch(const T* q, T* out, Q8Args a, int64_t n_pages, int n_list, int max_new, int q_tiles, cudaStream_t stream) {
+    constexpr int KT = Form<T, NT>::KT;
     const size_t smem = Form<T, NT>::smem();
+    // runs of keys that lie in a page and start a tile's share of it
+    a.run = KT;
+    while (a.page_size % a.run) a.run /= 2;
+    // tiles by TMA: boxes that start on a whole pattern of the swizzle (eight rows), of the cache as (byte of a head, place
+    // in a page, page and plane and head)
+    a.tiled = CAN_TILE && a.run >= 8;
+    CUtensorMap map = {};
+    if (a.tiled) {
+        const EncodeFn encode = encode_fn();
+        if (!encode) return (int)cudaErrorNotSupported;
+        const cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)a.page_size, (cuuint64_t)n_pages * 2 * a.G};
+        const cuuint64_t strides[2] = {(cuuint64_t)HD, (cuuint64_t)HD * a.page_size};
+        const cuuint32_t box[3] = {(cuuint32_t)WIDTH, (cuuint32_t)a.run, 1u}, one[3] = {1u, 1u, 1u};
+        if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(a.pages), dims, strides, box, one,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, WIDE ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return (int)cudaErrorInvalidValue;
+    }
     cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    e = sllm_launch_pdl(attn_q8_kernel<T, NT>, dim3(a.G, a.n_splits * q_tiles, n_list), dim3(THREADS), smem, stream, q, out, a);
+    e = sllm_launch_pdl(attn_q8_kernel<T, NT>, dim3(a.G, a.n_splits * q_tiles, n_list), dim3(THREADS), smem, stream, q, out, map, a);
     if (e != cudaSuccess || a.n_splits == 1) return (int)e;
     return (int)sllm_launch_pdl(attn_q8_merge_kernel<T>, dim3(((int64_t)max_new * a.H + 3) / 4, n_list), dim3(128), 0, stream,
                                 out, a);
@@ -601,10 +745,18 @@ SLLM_EXPORT int sllm_attn_q8_tile(int dtype, int nt) {
     return nt == 1 ? Form<__nv_bfloat16, 1>::KT : Form<__nv_bfloat16, 2>::KT;
 }
 
+// The code of a wait that was given up since the last call, 0 if none was (synchronises the device).
+SLLM_EXPORT int sllm_attn_q8_error() {
+    int code = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&code, g_tc_error, sizeof(int)) != cudaSuccess) return -1;
+    if (code) cudaMemcpyToSymbol(g_tc_error, &zero, sizeof(int));
+    return code;
+}
+
 // nt: queries a warp / 8; wq: groups of queries of a CTA (1, 2 or 4).  part: n_splits > 1 only, float
 // [part_tokens, H, n_splits, HD + 2].
-SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages, const void* scales, const int* table,
-                             int table_stride, int page_size, int block, const int* row_start, const int* row_pos0,
+SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages, int64_t n_pages, const void* scales,
+                             const int* table, int table_stride, int page_size, int block, const int* row_start, const int* row_pos0,
                              const int* row_list, int n_list, int max_new, void* out, int64_t out_stride, int H, int G,
                              float scale, int window, int dtype, int nt, int wq, int n_splits, float* part,
                              int64_t part_tokens, cudaStream_t stream) {
@@ -618,11 +770,12 @@ SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages,
     const int es = dtype == 0 ? 4 : 2;
     const int q_vec = (uintptr_t)q % (4 * es) == 0 && q_stride % 4 == 0;
     const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
-                      part, part_tokens, table_stride, page_size, block, H, G, window, n_splits, wq, q_vec, scale * LOG2E};
+                      part, part_tokens, table_stride, page_size, block, H, G, window, n_splits, wq, q_vec, 0, 0, scale * LOG2E,
+                      divisor(page_size), divisor(block)};
     typedef __nv_bfloat16 bf16;
     if (dtype == 0)
-        return nt == 1 ? launch<float, 1>((const float*)q, (float*)out, a, n_list, max_new, (int)q_tiles, stream)
-                       : launch<float, 2>((const float*)q, (float*)out, a, n_list, max_new, (int)q_tiles, stream);
-    return nt == 1 ? launch<bf16, 1>((const bf16*)q, (bf16*)out, a, n_list, max_new, (int)q_tiles, stream)
-                   : launch<bf16, 2>((const bf16*)q, (bf16*)out, a, n_list, max_new, (int)q_tiles, stream);
+        return nt == 1 ? launch<float, 1>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream)
+                       : launch<float, 2>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
+    return nt == 1 ? launch<bf16, 1>((const bf16*)q, (bf16*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream)
+                   : launch<bf16, 2>((const bf16*)q, (bf16*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
 }

@@ -893,7 +893,8 @@ def check_kernel_errors() -> None:
     device: call it where the host waits anyway (the end of a request batch, of a trace)."""
     found = []
     for name, lib in list(_loaded.items()):
-        for symbol in ("sllm_gemm_tc_error", "sllm_gemv_tma_error", "sllm_attn_tc_error"):
+        for symbol in ("sllm_gemm_tc_error", "sllm_gemv_tma_error", "sllm_attn_tc_error",
+                       "sllm_attn_q8_error"):
             if hasattr(lib, symbol):
                 code = int(getattr(lib, symbol)())
                 if code:
@@ -952,8 +953,8 @@ def _q8_cache(pages: torch.Tensor, scales: torch.Tensor, n_kv_heads: int, page_s
     block = page_size // scales.shape[3]
     if block * head_dim > Q8_MAX_BLOCK_ENTRIES:
         raise KernelError(f"blocks of {block} tokens of {head_dim} entries: at most {Q8_MAX_BLOCK_ENTRIES} entries")
-    if not 1 <= pages.shape[0] <= (1 << 32) // (2 * n_kv_heads * page_size) - 1:
-        raise KernelError(f"{pages.shape[0]} pages: from one page to 2^32 keys and values of a head are taken")
+    if not 1 <= pages.shape[0] <= ((1 << 31) - 1) // (2 * n_kv_heads):
+        raise KernelError(f"{pages.shape[0]} pages: from 1 to {((1 << 31) - 1) // (2 * n_kv_heads)} are taken")
     if pages.data_ptr() % 16:
         raise KernelError("pages must start on a 16-byte boundary")
     return block
@@ -1095,8 +1096,8 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     if n_splits > 1:
         part = torch.empty(q.shape[0] * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
     _check(_load(*attention_q8_library(head_dim)).sllm_attn_q8(
-        _ptr(q), c_int64(q.stride(0)), _ptr(pages), _ptr(scales), _ptr(block_table), c_int(block_table.stride(0)),
-        c_int(page_size), c_int(block), _ptr(row_start), _ptr(row_pos0), _ptr(row_list), c_int(n_list), c_int(max_new),
+        _ptr(q), c_int64(q.stride(0)), _ptr(pages), c_int64(pages.shape[0]), _ptr(scales), _ptr(block_table),
+        c_int(block_table.stride(0)), c_int(page_size), c_int(block), _ptr(row_start), _ptr(row_pos0), _ptr(row_list), c_int(n_list), c_int(max_new),
         _ptr(out), c_int64(out.stride(0)), c_int(n_heads), c_int(n_kv_heads), c_float(scale), c_int(window or 0),
         c_int(_code(q.dtype)), c_int(nt), c_int(wq), c_int(n_splits), _ptr(part), c_int64(q.shape[0]), _stream()),
         "attention_q8")
