@@ -4,11 +4,10 @@
 //   s_j = scale * q . k_j,   out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s)
 // Compiled once per head size: -DSLLM_HEAD_DIM=<multiple of 16, at most 256>.
 //
-// Numbers.  An e4m3 number's bits, moved to a half's places, are that number times 2^-8 (subnormal ones too), so the
-// products run on the tensor cores' f16 form with the cache's numbers as they are: seven bit operations for four of
-// them (the conversion instruction takes the special-function pipe for as long as eight: 64 rows of 4,096 keys, 32
-// heads of 128 on 8 kv heads, 225 us with it).  The blocks' powers of two join the scores (2^ek) and the probabilities
-// (2^ev) in 32 bits.  A NaN's bits would count as 480: a CTA that meets one takes its queries again key after key.  A query is brought into f16's range by a power of two of its own (largest entry
+// Numbers.  An e4m3 number is a half exactly, and one instruction turns two of them, so the products run on the tensor
+// cores' f16 form with the cache's numbers as they are (by bit operations, seven for four numbers, 64 rows of 4,096
+// keys took 141 us instead of 124).  The blocks' powers of two join the scores (2^ek) and the probabilities (2^ev) in 32
+// bits.  A query is brought into f16's range by a power of two of its own (largest entry
 // in [2^14, 2^15)): bfloat16 entries keep all their bits down to 2^-38 of the largest, 32-bit ones are split into two
 // halves (22 bits).  A probability is multiplied by its key's 2^ev before it becomes a half, against a running
 // maximum of its own, M = max(s + ev): what counts towards the output keeps 11 bits (22 in the 32-bit form) down
@@ -18,11 +17,15 @@
 // its 8 columns: a decoded token's group of up to 8 query heads fills the instruction, and an output is spread over
 // half as many registers.  Which entry of a head stands in which k step is free as long as queries and keys agree:
 // a lane takes a quarter of each key's bytes as they lie, and of the values an eighth of four keys; P becomes an operand
-// by movmatrix.  Every warp fills a ring of its own in shared memory by TMA (one request per plane and tile where a
-// page holds whole tiles, else one per run of keys), so that no warp waits for another before the end, and 16 KB a warp
-// are on their way while it works (requested straight into registers, half a tile at a time, 64 rows of 4,096 keys
-// took 210 us: the loads' latency).  128-byte (heads of 64: 64-byte) swizzle: no two lanes of a read meet in a bank.
-// Other heads, and pages of no whole eights of tokens, come by untiled bulk copies, as they lie.
+// by movmatrix.  Every warp fetches tiles of its own into shared memory by TMA (one request per plane and tile where a
+// page holds whole tiles, else one per run of keys), so that no warp waits for another before the end.  One tile a warp
+// is on its way or worked on, four warps a scheduler cover the wait: 64 rows of 4,096 keys, 32 heads of 128 on 8 kv heads,
+// take 99 us (5.4 TB/s); two tiles in turn for three warps a scheduler took 121 us, the keys of the next tile requested as
+// soon as this one's are read 111, loads straight into registers 210: what counts is instructions and the warps that are
+// there to issue them.  128-byte (heads of 64: 64-byte) swizzle: no two lanes of a read meet in a bank.  Other
+// heads, and pages of no whole eights of tokens, come by untiled bulk copies, as they lie.
+#include <cooperative_groups.h>
+
 #include "q8.cuh"
 #include "tc_common.cuh"
 
@@ -42,6 +45,7 @@ constexpr int DPL = (HD + 31) / 32;                      // entries of a head a 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LOWEST = -1e30f;                         // below every score; finite, so that differences are numbers
 constexpr float STALE = 8.f;                             // how far a maximum may lag behind the scores (base 2)
+constexpr int MAX_CLUSTER = 8;                           // CTAs of a cluster, on every device of the kind
 constexpr float P_SHIFT = 6.f;                           // probabilities become halves times 2^6: 2^14 at most
 
 // n / d for 0 <= n < 2^31: 2 n * ceil(2^(31 + s) / d) / 2^(32 + s), 2^s >= d
@@ -60,7 +64,7 @@ struct Q8Args {
     const uint8_t* pages; const uint8_t* scales; const int* table;
     const int* row_start; const int* row_pos0; const int* row_list;
     float* part; int64_t part_tokens;                    // [tokens, H, n_splits, HD + 2]: sums, maximum, denominator
-    int table_stride, page_size, block, H, G, window, n_splits, wq, q_vec, run, tiled;
+    int table_stride, page_size, block, H, G, window, n_splits, wq, q_vec, run, tiled, cluster;
     float scale_log2;
     Divisor page_div, block_div;
 };
@@ -81,13 +85,13 @@ template <typename T, int NT> struct Form {
     static constexpr int Q_REGS = NT * PARTS * KSTEPS * 2;
     static constexpr bool Q_SHARED = Q_REGS > 32;
     static constexpr int LD = HD + 4;
-    static constexpr int STAGE = 2 * KT * HD;                     // bytes of a tile: keys, then values
-    static constexpr int STAGES = NT == 1 ? (STAGE >= 8192 ? 2 : 4) : (STAGE >= 8192 ? 3 : 4);
-    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int TILE = 2 * KT * HD;                      // bytes of a tile: keys, then values
+    static constexpr int TILES = WARPS * TILE;
     static constexpr int MERGE = (int)sizeof(float) * WARPS * 8 * NT * LD;
     static constexpr int Q_BYTES = Q_SHARED ? (int)sizeof(uint32_t) * WARPS * 32 * Q_REGS : 0;
-    // the ring (at its end the meeting of the warps takes its place), then the queries
-    static constexpr int Q_AT = RING > MERGE ? RING : (MERGE + 1023) / 1024 * 1024;
+    // the tiles (at the end the meeting of the warps takes their place), then the queries
+    static constexpr int SCALAR = (int)sizeof(float) * (WARPS + 1) * HD;     // (behind the meeting: the scalar form's)
+    static constexpr int Q_AT = ((TILES > MERGE + SCALAR ? TILES : MERGE + SCALAR) + 1023) / 1024 * 1024;
     static constexpr size_t smem() { return 1024 + Q_AT + Q_BYTES; }
 };
 
@@ -117,15 +121,11 @@ __device__ __forceinline__ uint32_t halves_rest(float a, float b, uint32_t h) {
     return halves(a - f.x, b - f.y);
 }
 
-// Bytes 1 and 3 of a word, and bytes 0 and 2, as pairs of halves: the numbers times 2^-8.  `top`: the largest
-// of their bits without the sign; a NaN's are 0x3f80, the largest number's 0x3f00.
-__device__ __forceinline__ void halves_of(uint32_t w, uint32_t& odd, uint32_t& even, uint32_t& top) {
-    const uint32_t a = w >> 1 & 0x3f803f80u, b = w << 7 & 0x3f803f80u;
-    odd = (w & 0x80008000u) | a;
-    even = (w << 8 & 0x80008000u) | b;
-    top = __vimax3_u16x2(top, a, b);
+// bytes 0 and 1 of a word, and bytes 2 and 3, as pairs of halves
+__device__ __forceinline__ void halves_of(uint32_t w, uint32_t& low, uint32_t& high) {
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+        : "=r"(low), "=r"(high) : "r"(w));
 }
-__device__ __forceinline__ bool any_nan(uint32_t top) { return (top & 0xffffu) >= 0x3f80u || top >> 16 >= 0x3f80u; }
 
 // BYTES of shared memory into words; where they lie in pieces of 16 bytes, piece i at p[i]
 template <int BYTES, int N> __device__ __forceinline__ void take(const uint8_t* const (&p)[(BYTES + 15) / 16], int off, uint32_t (&w)[N]) {
@@ -160,7 +160,8 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 }
 
 // One query over the keys lo .. hi that it sees, key after key, by all warps of the CTA: sums relative to m (base 2) in
-// acc [HD], and (m, l).  For tiles that hold a NaN: it belongs to the queries that see it and to no other.
+// acc [HD], and (m, l).  For tiles in which a NaN came out: a product on the tensor cores multiplies also what a query does
+// not see, by zero, and zero times a NaN is one.
 template <typename T>
 __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args& a, const int* __restrict__ table, int g,
                                            int lo, int hi, float* acc, float* ml, float* smem) {
@@ -212,19 +213,24 @@ __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args
 
 // The queries of a row and kv head are packed: p = token * GS + j is the row's token `token` and query head g GS + j.  A
 // CTA takes 8 NT wq packed queries over a share of the keys; its warps are wq groups of queries by 4 / wq groups of keys,
-// which take turns at the tiles.  A CTA with fewer queries than the launch allows has fewer groups of queries.
+// which take turns at the tiles.  A CTA with fewer queries than the launch allows has fewer groups of queries.  Up to
+// eight splits can be a cluster, whose CTAs merge their sums through distributed shared memory (one row of 1,000 keys: 10.3
+// us against 12.4 with a merge kernel); in launches that fill the device clusters find less room than CTAs by themselves (24
+// rows of 4,096 keys of 64, three splits: 47 against 37), and the splits' sums meet in attn_q8_merge_kernel.
 // grid (kv heads, splits x tiles of queries, rows), the tiles with the most keys first.
 template <typename T, int NT>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2)
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 2)
 attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_constant__ CUtensorMap map, const Q8Args a) {
     using F = Form<T, NT>;
-    constexpr int PARTS = F::PARTS, KT = F::KT, KG = KT / 16, LD = F::LD, STAGES = F::STAGES;
+    constexpr int PARTS = F::PARTS, KT = F::KT, KG = KT / 16, LD = F::LD;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    float* smem = reinterpret_cast<float*>(ring);
-    __shared__ uint64_t full[WARPS][STAGES];
+    uint8_t* tiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    float* smem = reinterpret_cast<float*>(tiles);
+    __shared__ uint64_t full[WARPS];
     __shared__ float sm_m[WARPS][8 * NT], sm_l[WARPS][8 * NT], sm_ml[2 * WARPS + 2];
-    __shared__ int some_nan;
+    __shared__ float all_top[WARPS * 8 * NT], all_total[WARPS * 8 * NT];      // of the CTA, for the cluster
+
+    if (threadIdx.x == 0 && a.tiled) asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n8 = lane >> 2, c4 = lane & 3;
@@ -242,12 +248,94 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     const int per_split = (n_tiles + a.n_splits - 1) / a.n_splits;
     const int tile_begin = min(n_tiles, split * per_split), tile_end = min(n_tiles, tile_begin + per_split);
 
-    // ---- this warp's queries
+    // ---- this warp's queries: which they are
     const int w0 = q0 + (warp % wq) * 8 * NT, w_nq = min(8 * NT, q0 + nq - w0);     // (w_nq may be 0 or less)
     const int w_first = pos0 + w0 / GS, w_last = pos0 + (w0 + max(w_nq, 1) - 1) / GS;
+    // ---- tiles: lane i looks up key i (its page, then its two scales); where a page holds whole tiles lane 0 requests
+    // them, else lane i the i-th run of `run` keys
+    const int blocks = a.page_size / a.block;
+    int tile_stop = tile_end;             // this warp's queries see nothing from here on
+    if (w_nq <= 0) tile_stop = tile_begin;
+    else tile_stop = min(tile_stop, (w_last - k_lo) / KT + 1);
+    uint8_t* mine_at = tiles + warp * F::TILE;
+    if (lane == 0) {
+        mbar_init(&full[warp], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    }
+    __syncwarp();
+    auto page_of = [&](int tile) {
+        const int kpos = k_lo + tile * KT + lane % KT;
+        return tile < tile_stop && kpos <= w_last ? __ldg(table + a.page_div.quotient(kpos)) : -1;
+    };
+    // requests a tile and returns the bytes of this lane's key's two scales; -1: no such key
+    auto request = [&](int tile, int page) {
+        const int kpos = k_lo + tile * KT + lane % KT, off = kpos - a.page_div.quotient(kpos) * a.page_size;
+        const uint32_t bar = smem_u32(&full[warp]), dst = smem_u32(mine_at);
+        if (CAN_TILE && a.run == KT) {                         // (one page: lane 0's key is the tile's first)
+            if (lane == 0) {
+                mbar_expect_tx(&full[warp], page >= 0 ? F::TILE : 0);
+                if (page >= 0)
+#pragma unroll
+                    for (int x = 0; x < HD; x += WIDTH) {
+                        tma_load_3d(dst + x * KT, &map, bar, x, off, page * 2 * a.G + g);
+                        tma_load_3d(dst + x * KT + KT * HD, &map, bar, x, off, (page * 2 + 1) * a.G + g);
+                    }
+            }
+        } else {
+            const int from = lane * a.run % KT;                // the first key of this lane's run
+            const int run_page = __shfl_sync(0xffffffffu, page, from), run_off = __shfl_sync(0xffffffffu, off, from);
+            const bool mine = lane * a.run < KT && run_page >= 0;
+            const uint32_t asked = __ballot_sync(0xffffffffu, mine);
+            if (lane == 0) mbar_expect_tx(&full[warp], (uint32_t)__popc(asked) * 2u * a.run * HD);
+            __syncwarp();
+            if (mine) {
+                const uint32_t to = dst + lane * a.run * WIDTH;
+                const int plane = run_page * 2 * a.G + g;
+                if (CAN_TILE && a.tiled) {
+#pragma unroll
+                    for (int x = 0; x < HD; x += WIDTH) {
+                        tma_load_3d(to + x * KT, &map, bar, x, run_off, plane);
+                        tma_load_3d(to + x * KT + KT * HD, &map, bar, x, run_off, plane + a.G);
+                    }
+                } else {
+                    const uint8_t* src = a.pages + ((int64_t)plane * a.page_size + run_off) * HD;
+                    const int64_t v_off = (int64_t)a.G * a.page_size * HD;
+                    const int rows = HD == WIDTH ? 1 : a.run, bytes = HD == WIDTH ? a.run * HD : WIDTH;
+                    for (int i = 0; i < rows; ++i)
+#pragma unroll
+                        for (int x = 0; x < HD; x += WIDTH) {
+                            bulk_load(to + x * KT + i * WIDTH, src + i * HD + x, bytes, bar);
+                            bulk_load(to + x * KT + i * WIDTH + KT * HD, src + v_off + i * HD + x, bytes, bar);
+                        }
+                }
+            }
+        }
+        if (page < 0) return -1;
+        const uint8_t* s = a.scales + ((int64_t)page * 2 * a.G + g) * blocks + a.block_div.quotient(off);
+        return (int)__ldg(s) | (int)__ldg(s + (int64_t)a.G * blocks) << 8;
+    };
+    // where this lane's pieces of a key (rows n8 + 8 i) and of a value (rows 2 c4, 2 c4 + 1, and 8 i on) lie in a tile
+    const uint8_t* k_at[(HD / 4 + 15) / 16];
+    const uint8_t* v_at[2][(HD / 8 + 15) / 16];
+#pragma unroll
+    for (int i = 0; i < (HD / 4 + 15) / 16; ++i) k_at[i] = mine_at + place<KT>(n8, c4 * (HD / 4) + 16 * i, a.tiled);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < (HD / 8 + 15) / 16; ++i)
+            v_at[k][i] = mine_at + KT * HD + place<KT>(2 * c4 + k, n8 * (HD / 8) + 16 * i, a.tiled);
+    constexpr int EIGHT = 8 * WIDTH;         // eight rows
+
+    int tile = tile_begin + warp / wq, page = page_of(tile), sc = -1, parity = 0;
+    bool ok = true;
+    if (tile < tile_stop) sc = request(tile, page);
+    page = page_of(tile + wk);
+
+    // ---- its queries, while the first tile is on its way
     uint32_t qf[F::Q_SHARED ? 1 : PARTS][F::Q_SHARED ? 1 : NT][F::Q_SHARED ? 1 : KSTEPS][2];
-    uint2* q_sh = reinterpret_cast<uint2*>(ring + F::Q_AT) + warp * (F::Q_REGS / 2) * 32 + lane;   // [part][nt][ks][lane]
-    float fq[NT][2];                      // 2^8 * scale * log2 e / the query's power of two, of queries 2 c4 and 2 c4 + 1
+    uint2* q_sh = reinterpret_cast<uint2*>(tiles + F::Q_AT) + warp * (F::Q_REGS / 2) * 32 + lane;   // [part][nt][ks][lane]
+    float fq[NT][2];                      // scale * log2 e / the query's power of two, of queries 2 c4 and 2 c4 + 1
     int qpos[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -281,7 +369,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         // 2^k with top * 2^k in [2^14, 2^15); at most 2^100, so that its inverse times the scale is a normal number
         const int k = top > 0.f ? min(100, 14 + 127 - (__float_as_int(top) >> 23)) : 0;
         const float up = __int_as_float((k + 127) << 23);
-        const float own = a.scale_log2 * __int_as_float((127 + 8 - k) << 23);
+        const float own = a.scale_log2 * __int_as_float((127 - k) << 23);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             fq[nt][e] = __shfl_sync(0xffffffffu, own, (2 * c4 + e) * 4);
@@ -290,8 +378,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         }
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks) {
-            // (the order in which a key's word gives its bytes)
-            const float y0 = x[4 * ks + 1] * up, y1 = x[4 * ks + 3] * up, y2 = x[4 * ks] * up, y3 = x[4 * ks + 2] * up;
+            const float y0 = x[4 * ks] * up, y1 = x[4 * ks + 1] * up, y2 = x[4 * ks + 2] * up, y3 = x[4 * ks + 3] * up;
             const uint32_t h0 = halves(y0, y1), h1 = halves(y2, y3);
             uint32_t r0 = 0, r1 = 0;
             if constexpr (PARTS == 2) {
@@ -319,94 +406,10 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         for (int e = 0; e < 2; ++e) { m[nt][e] = M[nt][e] = LOWEST; l[nt][e] = 0.f; }
     }
 
-    // ---- the ring: lane i looks up key i of a tile (its page, then its two scales); where a page holds whole tiles lane
-    // 0 requests them, else lane i the i-th run of `run` keys
-    const int blocks = a.page_size / a.block;
-    int tile_stop = tile_end;             // this warp's queries see nothing from here on
-    if (w_nq <= 0) tile_stop = tile_begin;
-    else tile_stop = min(tile_stop, (w_last - k_lo) / KT + 1);
-    uint8_t* stages = ring + warp * STAGES * F::STAGE;
-    if (lane == 0) {
-#pragma unroll
-        for (int i = 0; i < STAGES; ++i) mbar_init(&full[warp][i], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    }
-    if (tid == 0) some_nan = 0;
-    __syncwarp();
-    auto page_of = [&](int tile) {
-        const int kpos = k_lo + tile * KT + lane % KT;
-        return tile < tile_stop && kpos <= w_last ? __ldg(table + a.page_div.quotient(kpos)) : -1;
-    };
-    // requests a tile and returns the bytes of this lane's two scales; -1: no such key
-    auto request = [&](int tile, int page, int stage) {
-        const int kpos = k_lo + tile * KT + lane % KT, off = kpos - a.page_div.quotient(kpos) * a.page_size;
-        const int from = lane * a.run % KT;                    // the first key of this lane's run
-        const int run_page = __shfl_sync(0xffffffffu, page, from), run_off = __shfl_sync(0xffffffffu, off, from);
-        const bool mine = lane * a.run < KT && run_page >= 0;
-        const uint32_t asked = __ballot_sync(0xffffffffu, mine);
-        const uint32_t bar = smem_u32(&full[warp][stage]);
-        if (lane == 0) mbar_expect_tx(&full[warp][stage], (uint32_t)__popc(asked) * 2u * a.run * HD);
-        __syncwarp();
-        if (mine) {
-            const uint32_t dst = smem_u32(stages + stage * F::STAGE) + lane * a.run * WIDTH;
-            const int plane = run_page * 2 * a.G + g;
-            if (CAN_TILE && a.tiled) {
-#pragma unroll
-                for (int x = 0; x < HD; x += WIDTH) {
-                    tma_load_3d(dst + x * KT, &map, bar, x, run_off, plane);
-                    tma_load_3d(dst + x * KT + KT * HD, &map, bar, x, run_off, plane + a.G);
-                }
-            } else {
-                const uint8_t* src = a.pages + ((int64_t)plane * a.page_size + run_off) * HD;
-                const int64_t v_off = (int64_t)a.G * a.page_size * HD;
-                if constexpr (HD == WIDTH) {
-                    bulk_load(dst, src, a.run * HD, bar);
-                    bulk_load(dst + KT * HD, src + v_off, a.run * HD, bar);
-                } else {
-                    for (int i = 0; i < a.run; ++i)
-#pragma unroll
-                        for (int x = 0; x < HD; x += WIDTH) {
-                            bulk_load(dst + x * KT + i * WIDTH, src + i * HD + x, WIDTH, bar);
-                            bulk_load(dst + x * KT + i * WIDTH + KT * HD, src + v_off + i * HD + x, WIDTH, bar);
-                        }
-                }
-            }
-        }
-        if (page < 0) return -1;
-        const uint8_t* s = a.scales + ((int64_t)page * 2 * a.G + g) * blocks + a.block_div.quotient(off);
-        return (int)__ldg(s) | (int)__ldg(s + (int64_t)a.G * blocks) << 8;
-    };
-    // where this lane's pieces of a key (rows n8 + 8 i) and of a value (rows 2 c4, 2 c4 + 1, and 8 i on) lie in a stage
-    const uint8_t* k_at[(HD / 4 + 15) / 16];
-    const uint8_t* v_at[2][(HD / 8 + 15) / 16];
-#pragma unroll
-    for (int i = 0; i < (HD / 4 + 15) / 16; ++i) k_at[i] = stages + place<KT>(n8, c4 * (HD / 4) + 16 * i, a.tiled);
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int i = 0; i < (HD / 8 + 15) / 16; ++i)
-            v_at[k][i] = stages + KT * HD + place<KT>(2 * c4 + k, n8 * (HD / 8) + 16 * i, a.tiled);
-    constexpr int EIGHT = 8 * WIDTH;         // eight rows
-
-    int tile = tile_begin + warp / wq, sc[STAGES];
-    bool nan_seen = false, ok = true;
-    {
-        int page[STAGES];
-#pragma unroll
-        for (int i = 0; i < STAGES; ++i) page[i] = page_of(tile + i * wk);
-#pragma unroll
-        for (int i = 0; i < STAGES; ++i)
-            sc[i] = tile + i * wk < tile_stop ? request(tile + i * wk, page[i], i) : -1;
-    }
-    int page_after = page_of(tile + STAGES * wk), stage = 0, parity = 0;
-
     for (; tile < tile_stop; tile += wk) {
         const int kt = k_lo + tile * KT;
-        ok = mbar_wait(&full[warp][stage], parity, 1);
+        ok = mbar_wait(&full[warp], parity, 1);
         if (!ok) break;
-        const int at = stage * F::STAGE;
-        uint32_t top_bits = 0u;
         // ---- scores, transposed: rows are keys, columns queries
         float s[KG][NT][4];
 #pragma unroll
@@ -417,7 +420,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
                 for (int e = 0; e < 4; ++e) s[i][nt][e] = 0.f;
         uint32_t kr[2 * KG][KSTEPS];
 #pragma unroll
-        for (int i = 0; i < 2 * KG; ++i) take<HD / 4>(k_at, at + i * EIGHT, kr[i]);
+        for (int i = 0; i < 2 * KG; ++i) take<HD / 4>(k_at, i * EIGHT, kr[i]);
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks) {
             uint32_t b[PARTS][NT][2];
@@ -435,15 +438,15 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
 #pragma unroll
             for (int i = 0; i < KG; ++i) {
                 uint32_t f[4];
-                halves_of(kr[2 * i][ks], f[0], f[2], top_bits);
-                halves_of(kr[2 * i + 1][ks], f[1], f[3], top_bits);
+                halves_of(kr[2 * i][ks], f[0], f[2]);
+                halves_of(kr[2 * i + 1][ks], f[1], f[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int part = PARTS - 1; part >= 0; --part) mma_f16(s[i][nt], f, b[part][nt][0], b[part][nt][1]);
             }
         }
-        const bool there = sc[0] >= 0;
+        const bool there = sc >= 0;
         const bool whole = __all_sync(0xffffffffu, there) && kt + KT - 1 <= w_first && (a.window <= 0 || kt > w_last - a.window);
         uint32_t seen_rows = 0;
         if (!whole) seen_rows = __ballot_sync(0xffffffffu, there);
@@ -455,7 +458,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int key = 16 * i + 8 * k + n8;
-                const int both = __shfl_sync(0xffffffffu, sc[0], key);
+                const int both = __shfl_sync(0xffffffffu, sc, key);
                 const float fk = __int_as_float((both & 0xff) << 23);
                 ev[i][k] = (float)(both >> 8 & 0xff) - 127.f;
 #pragma unroll
@@ -538,18 +541,23 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         for (int i = 0; i < KG; ++i) {
             uint32_t vr[4][VREGS];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) take<HD / 8>(v_at[k & 1], at + (2 * i + (k >> 1)) * EIGHT, vr[k]);
+            for (int k = 0; k < 4; ++k) {
+                take<HD / 8>(v_at[k & 1], (2 * i + (k >> 1)) * EIGHT, vr[k]);
+                if (!whole && !(seen_rows >> (16 * i + 2 * c4 + (k & 1) + 8 * (k >> 1)) & 1u))
+#pragma unroll
+                    for (int w = 0; w < VREGS; ++w) vr[k][w] = 0u;         // (a place without a key may hold a NaN)
+            }
 #pragma unroll
             for (int j = 0; j < KSTEPS; ++j) {
-                // (bytes 1 and 3: entry 2 j of two keys, bytes 0 and 2: entry 2 j + 1)
-                constexpr uint32_t LOW = 0x4501, HIGH = 0x6723;
+                // (bytes 0 and 1: entry 2 j of two keys, bytes 2 and 3: entry 2 j + 1)
+                constexpr uint32_t LOW = 0x5140, HIGH = 0x7362;
                 const int w = V_WORDS ? j / 2 : j;
                 const uint32_t pick = V_WORDS && (j & 1) ? HIGH : LOW;
                 const uint32_t x = __byte_perm(vr[0][w], vr[1][w], pick);
                 const uint32_t y = __byte_perm(vr[2][w], vr[3][w], pick);
                 uint32_t f[4];
-                halves_of(x, f[0], f[1], top_bits);
-                halves_of(y, f[2], f[3], top_bits);
+                halves_of(x, f[0], f[1]);
+                halves_of(y, f[2], f[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -557,23 +565,10 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
                         mma_f16(o[j][nt], f, p[part][i][nt][0], p[part][i][nt][1]);
             }
         }
-        if (__any_sync(0xffffffffu, any_nan(top_bits))) {
-            // (the tile's places without a key may hold anything: what counts are this lane's own keys)
-            if (whole) nan_seen = true;
-            else if (there && lane < KT)
-                for (int b = 0; b < HD; b += 2)
-#pragma unroll
-                    for (int v = 0; v < 2; ++v) {
-                        const uint32_t w = *reinterpret_cast<const uint16_t*>(stages + at + v * KT * HD + place<KT>(lane, b, a.tiled));
-                        nan_seen |= (w & 0x7f) == 0x7f || (w >> 8 & 0x7f) == 0x7f;
-                    }
-        }
-        __syncwarp();                     // (the stage is read)
-#pragma unroll
-        for (int i = 0; i + 1 < STAGES; ++i) sc[i] = sc[i + 1];
-        sc[STAGES - 1] = tile + STAGES * wk < tile_stop ? request(tile + STAGES * wk, page_after, stage) : -1;
-        page_after = page_of(tile + (STAGES + 1) * wk);
-        if (++stage == STAGES) { stage = 0; parity ^= 1; }
+        __syncwarp();                     // (the tile is read)
+        if (tile + wk < tile_stop) sc = request(tile + wk, page);
+        page = page_of(tile + 2 * wk);
+        parity ^= 1;
     }
 
     // ---- the groups of keys meet
@@ -588,8 +583,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
                 sm_l[warp][nt * 8 + 2 * c4 + e] = l[nt][e];
             }
         }
-    __syncthreads();                      // (all rings are done with)
-    if (nan_seen) some_nan = 1;
+    __syncthreads();                      // (all tiles are done with)
     float* sums = smem;                   // [WARPS][8 NT][LD]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -598,24 +592,31 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
             const int i = nt * 8 + 2 * c4 + e;
             float top = LOWEST;
             for (int w = warp % wq; w < WARPS; w += wq) top = fmaxf(top, sm_m[w][i]);
-            const float f = ex2(M[nt][e] + (8.f - P_SHIFT) - top);
+            const float f = ex2(M[nt][e] - P_SHIFT - top);
             float* to = sums + (warp * 8 * NT + i) * LD + n8 * (HD / 8);
 #pragma unroll
             for (int j = 0; j < KSTEPS; ++j)
                 *reinterpret_cast<float2*>(to + 2 * j) = make_float2(o[j][nt][e] * f, o[j][nt][2 + e] * f);
         }
     __syncthreads();
-    const int64_t part_ld = HD + 2;
-    auto leave = [&](int i, int d, float sum, float top, float total) {       // query i's entry d
+    auto to_out = [&](int i, int d, float sum, float total) {                 // query i's entry d
+        const int p = q0 + i, tok = p / GS, h = g * GS + p - tok * GS;
+        out[(int64_t)(t0 + tok) * a.out_stride + (int64_t)h * HD + d] = from_float<T>(total == 0.f ? 0.f : sum / total);
+    };
+    auto leave = [&](int i, int d, float sum, float top, float total) {
         const int p = q0 + i, tok = p / GS, h = g * GS + p - tok * GS;
         if (a.n_splits == 1) {
-            out[(int64_t)(t0 + tok) * a.out_stride + (int64_t)h * HD + d] = from_float<T>(total == 0.f ? 0.f : sum / total);
+            to_out(i, d, sum, total);
+        } else if (a.cluster) {
+            sums[i * LD + d] = sum;                      // (query i's place of the first group of keys)
+            if (d == 0) { all_top[i] = top; all_total[i] = total; }
         } else if (t0 + tok < a.part_tokens) {
-            float* part = a.part + (((int64_t)(t0 + tok) * a.H + h) * a.n_splits + split) * part_ld;
+            float* part = a.part + (((int64_t)(t0 + tok) * a.H + h) * a.n_splits + split) * (HD + 2);
             part[d] = sum;
             if (d == 0) { part[HD] = top; part[HD + 1] = total; }
         }
     };
+    bool odd = false;
     for (int idx = tid; idx < nq * HD; idx += THREADS) {
         const int i = idx / HD, d = idx - i * HD, group = i / (8 * NT), j = i - group * 8 * NT;
         float top = LOWEST, total = 0.f, sum = 0.f;
@@ -624,21 +625,45 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
             total += sm_l[w][j] * ex2(sm_m[w][j] - top);
             sum += sums[(w * 8 * NT + j) * LD + d];
         }
+        odd |= isnan(sum) || isnan(total);
         leave(i, d, sum, top, total);
     }
-    __syncthreads();
-    if (some_nan) {                       // each query by itself
-        float* acc = smem + WARPS * HD;
-        static_assert((WARPS + 1) * HD <= WARPS * 8 * LD, "room for the scalar form");
+    // a NaN, and not all queries see the same keys: each of them by itself
+    if (__syncthreads_or(odd) && first_pos != last_pos) {
+        float* scratch = reinterpret_cast<float*>(tiles + F::MERGE);
+        float* acc = scratch + WARPS * HD;
         for (int i = 0; i < nq; ++i) {
             const int p = q0 + i, tok = p / GS, pos = pos0 + tok;
             const int lo = max(k_lo + tile_begin * KT, a.window > 0 ? pos - a.window + 1 : 0);
             const int hi = min(k_lo + tile_end * KT - 1, pos);
             attend_scalar<T>(q + (int64_t)(t0 + tok) * a.q_stride + (int64_t)(g * GS + p - tok * GS) * HD, a, table, g, lo, hi,
-                             acc, sm_ml, smem);
+                             acc, sm_ml, scratch);
             for (int d = tid; d < HD; d += THREADS) leave(i, d, acc[d], sm_ml[2 * WARPS], sm_ml[2 * WARPS + 1]);
             __syncthreads();
         }
+    }
+    if (a.n_splits > 1 && a.cluster) {
+        // every CTA merges a share of the entries, in the splits' order
+        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        cluster.sync();
+        for (int idx = split * THREADS + tid; idx < nq * HD; idx += a.n_splits * THREADS) {
+            const int i = idx / HD, d = idx - i * HD;
+            float tops[MAX_CLUSTER], top = LOWEST, total = 0.f, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < MAX_CLUSTER; ++k) {
+                tops[k] = k < a.n_splits ? cluster.map_shared_rank(all_top, k)[i] : LOWEST;
+                top = fmaxf(top, tops[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < MAX_CLUSTER; ++k) {
+                if (k >= a.n_splits) continue;
+                const float f = ex2(tops[k] - top);
+                total += cluster.map_shared_rank(all_total, k)[i] * f;
+                sum += cluster.map_shared_rank(sums, k)[i * LD + d] * f;
+            }
+            to_out(i, d, sum, total);
+        }
+        cluster.sync();                   // (nobody leaves while others read)
     }
 }
 
@@ -712,8 +737,20 @@ static int launch(const T* q, T* out, Q8Args a, int64_t n_pages, int n_list, int
     }
     cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    e = sllm_launch_pdl(attn_q8_kernel<T, NT>, dim3(a.G, a.n_splits * q_tiles, n_list), dim3(THREADS), smem, stream, q, out, map, a);
-    if (e != cudaSuccess || a.n_splits == 1) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.G, a.n_splits * q_tiles, n_list);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {1u, (unsigned)a.n_splits, 1u};
+    cfg.attrs = attr;
+    cfg.numAttrs = a.cluster ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, attn_q8_kernel<T, NT>, q, out, map, (const Q8Args)a);
+    if (e != cudaSuccess || a.n_splits == 1 || a.cluster) return (int)e;
     return (int)sllm_launch_pdl(attn_q8_merge_kernel<T>, dim3(((int64_t)max_new * a.H + 3) / 4, n_list), dim3(128), 0, stream,
                                 out, a);
 }
@@ -753,24 +790,24 @@ SLLM_EXPORT int sllm_attn_q8_error() {
     return code;
 }
 
-// nt: queries a warp / 8; wq: groups of queries of a CTA (1, 2 or 4).  part: n_splits > 1 only, float
-// [part_tokens, H, n_splits, HD + 2].
+// nt: queries a warp / 8; wq: groups of queries of a CTA (1, 2 or 4).  cluster: up to 8 splits are merged inside the kernel; else
+// part, float [part_tokens, H, n_splits, HD + 2], takes the splits' sums.
 SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages, int64_t n_pages, const void* scales,
                              const int* table, int table_stride, int page_size, int block, const int* row_start, const int* row_pos0,
                              const int* row_list, int n_list, int max_new, void* out, int64_t out_stride, int H, int G,
                              float scale, int window, int dtype, int nt, int wq, int n_splits, float* part,
-                             int64_t part_tokens, cudaStream_t stream) {
+                             int64_t part_tokens, int cluster, cudaStream_t stream) {
     if (n_list <= 0 || max_new <= 0) return 0;
     if (H <= 0 || G <= 0 || H % G || page_size <= 0 || block <= 0 || page_size % block || window < 0 || n_list > 65535 ||
         (dtype != 0 && dtype != 1) || (nt != 1 && nt != 2) || (wq != 1 && wq != 2 && wq != 4) || n_splits < 1 ||
-        (n_splits > 1 && part == nullptr) || ((uintptr_t)pages & 15))
+        (cluster ? n_splits > MAX_CLUSTER : n_splits > 1 && part == nullptr) || ((uintptr_t)pages & 15))
         return (int)cudaErrorInvalidValue;
     const int64_t q_tiles = ((int64_t)max_new * (H / G) + 8 * nt * wq - 1) / (8 * nt * wq);
     if (q_tiles * n_splits > 65535 || (int64_t)max_new * H > (1u << 30)) return (int)cudaErrorInvalidValue;
     const int es = dtype == 0 ? 4 : 2;
     const int q_vec = (uintptr_t)q % (4 * es) == 0 && q_stride % 4 == 0;
     const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
-                      part, part_tokens, table_stride, page_size, block, H, G, window, n_splits, wq, q_vec, 0, 0, scale * LOG2E,
+                      part, part_tokens, table_stride, page_size, block, H, G, window, n_splits, wq, q_vec, 0, 0, cluster && n_splits > 1, scale * LOG2E,
                       divisor(page_size), divisor(block)};
     typedef __nv_bfloat16 bf16;
     if (dtype == 0)

@@ -1046,8 +1046,9 @@ def _attention_q8_form(device: int, head_dim: int, code: int, nt: int) -> tuple[
 
 @functools.lru_cache(maxsize=4096)
 def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_new: int, max_context: int, n_heads: int,
-                       n_kv_heads: int, window: int) -> tuple[int, int, int]:
-    """How a launch is shared out: (queries a warp / 8, groups of queries of a CTA, CTAs along the keys)."""
+                       n_kv_heads: int, window: int) -> tuple[int, int, int, bool]:
+    """How a launch is shared out: (queries a warp / 8, groups of queries of a CTA, CTAs along the keys, whether these
+    are a cluster that merges by itself)."""
     packed = max_new * (n_heads // n_kv_heads)
     nt = 1 if packed <= 8 else 2
     wq = 1 if packed <= 8 * nt else 2 if packed <= 16 * nt else 4
@@ -1060,7 +1061,7 @@ def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_n
         cost = -(-base * n // slots) * (-(-turns // n) + 2) + (0.1 * n + 1 if n > 1 else 0)
         if best_cost is None or cost < best_cost:
             best, best_cost = n, cost
-    return nt, wq, best
+    return nt, wq, best, best <= 8 and base * best <= _sm_count(device)
 
 
 def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, page_size: int,
@@ -1090,17 +1091,17 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
           row_list=row_list)
     if n_list <= 0 or max_new <= 0:
         return out
-    nt, wq, n_splits = _attention_q8_plan(q.get_device(), head_dim, _code(q.dtype), n_list, max_new, max_context, n_heads,
+    nt, wq, n_splits, cluster = _attention_q8_plan(q.get_device(), head_dim, _code(q.dtype), n_list, max_new, max_context, n_heads,
                                           n_kv_heads, window or 0)
     part = None
-    if n_splits > 1:
+    if n_splits > 1 and not cluster:
         part = torch.empty(q.shape[0] * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
     _check(_load(*attention_q8_library(head_dim)).sllm_attn_q8(
         _ptr(q), c_int64(q.stride(0)), _ptr(pages), c_int64(pages.shape[0]), _ptr(scales), _ptr(block_table),
         c_int(block_table.stride(0)), c_int(page_size), c_int(block), _ptr(row_start), _ptr(row_pos0), _ptr(row_list), c_int(n_list), c_int(max_new),
         _ptr(out), c_int64(out.stride(0)), c_int(n_heads), c_int(n_kv_heads), c_float(scale), c_int(window or 0),
-        c_int(_code(q.dtype)), c_int(nt), c_int(wq), c_int(n_splits), _ptr(part), c_int64(q.shape[0]), _stream()),
-        "attention_q8")
+        c_int(_code(q.dtype)), c_int(nt), c_int(wq), c_int(n_splits), _ptr(part), c_int64(q.shape[0]),
+        c_int(int(cluster)), _stream()), "attention_q8")
     return out
 
 
