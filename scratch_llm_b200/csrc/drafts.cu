@@ -12,73 +12,189 @@
 // All of it in 64 bits: products and differences of 32-bit numbers are exact there, and a sum of 128,256 of them
 // in another order moves by 1e-16 of itself, where a token's share of it is 1e-5: in 32 bits a draw in a
 // hundred would fall on another token.
+//
+// A row needs its drafts' own entries (one warp, a draft a lane) and then one pass over the distribution that decides: a
+// cluster of eight CTAs per row, every warp with a run of the vocabulary of its own.  Sums of runs go through shared
+// memory, sums of CTAs through distributed shared memory; the warp whose run holds the goal walks it once more (a
+// few KB that the SM has just read).  One CTA per row, every pass by itself, took 155 us for 4 rows of 128,256 entries.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace sllm {
 
-constexpr int VERIFY_THREADS = 1024;
+constexpr int VERIFY_THREADS = 512, VERIFY_WARPS = VERIFY_THREADS / 32, VERIFY_RANKS = 8;
+constexpr int VERIFY_BATCH = 4;         // strips of 128 entries that a warp requests at a time
 
 __device__ __forceinline__ double weight(float p, float q) {
     const double w = (double)p - (double)q;
     return w > 0.0 ? w : 0.0;           // (a NaN too)
 }
 
-__global__ void __launch_bounds__(VERIFY_THREADS)
+// What a row draws from: max(p - q, 0), without the entry `hot`; q may be null.
+struct Weights {
+    const float* p; const float* q;
+    int hot;
+    bool vec;                           // whole 16-byte words
+    // of the entries j .. j + 3 below `end`
+    __device__ __forceinline__ void load(int j, int end, float4& a, float4& b) const {
+        b = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (vec && j + 4 <= end) {
+            a = __ldg(reinterpret_cast<const float4*>(p + j));
+            if (q) b = __ldg(reinterpret_cast<const float4*>(q + j));
+        } else {
+            a = b;
+            float* x = reinterpret_cast<float*>(&a);
+            float* y = reinterpret_cast<float*>(&b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (j + i < end) {
+                    x[i] = __ldg(p + j + i);
+                    if (q) y[i] = __ldg(q + j + i);
+                }
+        }
+    }
+    __device__ __forceinline__ void of(int j, const float4& a, const float4& b, double (&w)[4]) const {
+        w[0] = j == hot ? 0.0 : weight(a.x, b.x);
+        w[1] = j + 1 == hot ? 0.0 : weight(a.y, b.y);
+        w[2] = j + 2 == hot ? 0.0 : weight(a.z, b.z);
+        w[3] = j + 3 == hot ? 0.0 : weight(a.w, b.w);
+    }
+};
+
+__global__ void __cluster_dims__(VERIFY_RANKS, 1, 1) __launch_bounds__(VERIFY_THREADS)
 verify_drafts_kernel(const float* __restrict__ probs, int64_t p_stride, const float* __restrict__ draft_probs,
                      int64_t q_stride, const int* __restrict__ drafts, const int* __restrict__ start,
                      const float* __restrict__ uniforms, int V, int* __restrict__ tokens, int* __restrict__ accepted) {
-    __shared__ double part[VERIFY_THREADS];
-    __shared__ int found;
+    __shared__ double warp_sum[VERIFY_WARPS], cta_sum[2];
+    __shared__ int n_accepted;
     pdl_wait();
     pdl_trigger();
-    const int r = blockIdx.x, tid = threadIdx.x;
-    const int d0 = start[r], k = start[r + 1] - d0, p0 = d0 + r;
-    int n = 0;
-    for (; n < k; ++n) {
-        const int x = drafts[d0 + n];
-        if (x < 0 || x >= V) break;
-        const double q = draft_probs ? (double)draft_probs[(d0 + n) * q_stride + x] : 1.0;
-        if (!((double)uniforms[p0 + n] * q < (double)probs[(p0 + n) * p_stride + x])) break;
-    }
-    const float* p = probs + (p0 + n) * p_stride;
-    const float* q = draft_probs && n < k ? draft_probs + (d0 + n) * q_stride : nullptr;
-    const int hot = !draft_probs && n < k ? drafts[d0 + n] : -1;
-    const int per = (V + VERIFY_THREADS - 1) / VERIFY_THREADS, begin = min(V, tid * per), end = min(V, begin + per);
-    int token = -1;
-    for (int turn = 0; turn < 2 && token < 0; ++turn) {       // the weights, or p itself
-        auto w = [&](int j) { return j == hot && !turn ? 0.0 : weight(p[j], q && !turn ? q[j] : 0.f); };
-        double mine = 0.0;
-        int last = -1;
-        for (int j = begin; j < end; ++j) {
-            const double x = w(j);
-            mine += x;
-            if (x > 0.0) last = j;
-        }
-        __syncthreads();
-        part[tid] = mine;
-        if (tid == 0) found = -1;
-        __syncthreads();
-        double before = 0.0, total = 0.0;
-        for (int t = 0; t < VERIFY_THREADS; ++t) {
-            if (t == tid) before = total;
-            total += part[t];
-        }
-        const double goal = (double)uniforms[p0 + k] * total;
-        if (last >= 0 && before <= goal) {                      // (the last such thread has it, or one after it none)
-            double run = before;
-            int pick = last;
-            for (int j = begin; j < end; ++j) {
-                run += w(j);
-                if (run > goal) { pick = j; break; }
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int rank = (int)cluster.block_rank(), r = blockIdx.x / VERIFY_RANKS;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int d0 = start[r], k = start[r + 1] - d0;
+    const int64_t p0 = (int64_t)d0 + r;
+    const double u = (double)uniforms[p0 + k];
+    if (warp == 0) {
+        int n = 0;
+        for (; n < k; n += 32) {
+            const int i = n + lane;
+            bool kept = i < k;
+            if (kept) {
+                const int x = drafts[d0 + i];
+                kept = x >= 0 && x < V;
+                if (kept) {
+                    const double q = draft_probs ? (double)draft_probs[(int64_t)(d0 + i) * q_stride + x] : 1.0;
+                    kept = (double)uniforms[p0 + i] * q < (double)probs[(p0 + i) * p_stride + x];
+                }
             }
-            atomicMax(&found, pick);
+            const uint32_t refused = __ballot_sync(0xffffffffu, !kept);
+            if (refused) { n += __ffs(refused) - 1; break; }
         }
-        __syncthreads();
-        token = found;
+        if (lane == 0) n_accepted = min(n, k);
     }
-    for (int i = tid; i <= k; i += VERIFY_THREADS)
-        tokens[p0 + i] = i < n ? drafts[d0 + i] : i == n ? token : -1;
-    if (tid == 0) accepted[r] = n;
+    __syncthreads();
+    const int n = n_accepted;
+    Weights w = {probs + (p0 + n) * p_stride, draft_probs && n < k ? draft_probs + (int64_t)(d0 + n) * q_stride : nullptr,
+                 !draft_probs && n < k ? drafts[d0 + n] : -1, false};
+    // this warp's run: a share of the vocabulary, in whole fours
+    const int run = ((V + VERIFY_RANKS * VERIFY_WARPS - 1) / (VERIFY_RANKS * VERIFY_WARPS) + 3) / 4 * 4;
+    const int64_t run0 = (int64_t)(rank * VERIFY_WARPS + warp) * run;
+    const int begin = (int)min((int64_t)V, run0), end = (int)min((int64_t)V, run0 + run);
+    bool found = false;
+    for (int turn = 0; turn < 2 && !found; ++turn) {          // the weights, or p itself (the same turn in all CTAs)
+        if (turn) { w.q = nullptr; w.hot = -1; }
+        w.vec = (((uintptr_t)w.p | (uintptr_t)w.q) & 15) == 0;
+        double mine = 0.0;
+        for (int j0 = begin; j0 < end; j0 += 128 * VERIFY_BATCH) {
+            float4 a[VERIFY_BATCH], b[VERIFY_BATCH];
+#pragma unroll
+            for (int t = 0; t < VERIFY_BATCH; ++t) w.load(j0 + 128 * t + 4 * lane, end, a[t], b[t]);
+#pragma unroll
+            for (int t = 0; t < VERIFY_BATCH; ++t) {
+                double x[4];
+                w.of(j0 + 128 * t + 4 * lane, a[t], b[t], x);
+                mine += (x[0] + x[1]) + (x[2] + x[3]);
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        if (lane == 0) warp_sum[warp] = mine;
+        __syncthreads();
+        if (tid == 0) {
+            double sum = 0.0;
+            for (int i = 0; i < VERIFY_WARPS; ++i) sum += warp_sum[i];
+            cta_sum[turn] = sum;
+        }
+        cluster.sync();
+        double total = 0.0, before = 0.0, sums[VERIFY_RANKS];
+#pragma unroll
+        for (int i = 0; i < VERIFY_RANKS; ++i) sums[i] = cluster.map_shared_rank(cta_sum, i)[turn];
+#pragma unroll
+        for (int i = 0; i < VERIFY_RANKS; ++i) total += sums[i];
+        found = total > 0.0;
+        if (!found) continue;
+        // the first CTA whose end lies past the goal, or the last one with any weight
+        const double goal = u * total;
+        int owner = -1;
+        double upto = 0.0, after = 0.0;
+#pragma unroll
+        for (int i = 0; i < VERIFY_RANKS; ++i) {
+            if ((owner < 0 || after <= goal) && sums[i] > 0.0) { owner = i; before = upto; after = upto + sums[i]; }
+            upto += sums[i];
+        }
+        if (owner != rank) continue;
+        // likewise its warp
+        int own_warp = -1;
+        double start_at = 0.0;
+        upto = before;
+        for (int i = 0; i < VERIFY_WARPS; ++i) {
+            if ((own_warp < 0 || after <= goal) && warp_sum[i] > 0.0) { own_warp = i; start_at = upto; after = upto + warp_sum[i]; }
+            upto += warp_sum[i];
+        }
+        if (own_warp != warp) continue;
+        // and its entry, a strip of 128 at a time
+        int token = -1;
+        double past = start_at;
+        for (int j0 = begin; j0 < end; j0 += 128) {
+            const int j = j0 + 4 * lane;
+            float4 a, b;
+            double x[4];
+            w.load(j, end, a, b);
+            w.of(j, a, b, x);
+            double scan = (x[0] + x[1]) + (x[2] + x[3]);
+            const double own = scan;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double up = __shfl_up_sync(0xffffffffu, scan, o);
+                if (lane >= o) scan += up;
+            }
+            // the lane whose entries pass the goal, and which of them; the last one of any weight stands in
+            double at = past + (scan - own);
+            int pick = -1, last = -1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                at += x[i];
+                if (x[i] > 0.0) last = j + i;
+                if (x[i] > 0.0 && pick < 0 && at > goal) pick = j + i;
+            }
+            const uint32_t hits = __ballot_sync(0xffffffffu, pick >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
+            if (hits) {
+                token = __shfl_sync(0xffffffffu, pick, __ffs(hits) - 1);
+                break;
+            }
+            if (any) token = __shfl_sync(0xffffffffu, last, 31 - __clz(any));
+            past += __shfl_sync(0xffffffffu, scan, 31);
+        }
+        if (lane == 0) tokens[p0 + n] = token;
+    }
+    if (rank == 0) {
+        for (int i = tid; i <= k; i += VERIFY_THREADS)
+            if (i != n || !found) tokens[p0 + i] = i < n ? drafts[d0 + i] : -1;
+        if (tid == 0) accepted[r] = n;
+    }
+    cluster.sync();                       // (nobody leaves while others read its sum)
 }
 
 }  // namespace sllm
@@ -89,7 +205,7 @@ SLLM_EXPORT int sllm_verify_drafts(const float* probs, int64_t p_stride, const f
                                    const int* drafts, const int* start, const float* uniforms, int n_rows, int V,
                                    int* tokens, int* accepted, cudaStream_t stream) {
     if (n_rows <= 0) return 0;
-    if (V <= 0) return (int)cudaErrorInvalidValue;
-    return (int)sllm_launch_pdl(verify_drafts_kernel, dim3(n_rows), dim3(VERIFY_THREADS), 0, stream, probs, p_stride,
+    if (V <= 0 || n_rows > 0x7fffffff / VERIFY_RANKS) return (int)cudaErrorInvalidValue;
+    return (int)sllm_launch_pdl(verify_drafts_kernel, dim3(n_rows * VERIFY_RANKS), dim3(VERIFY_THREADS), 0, stream, probs, p_stride,
                                 draft_probs, q_stride, drafts, start, uniforms, V, tokens, accepted);
 }
