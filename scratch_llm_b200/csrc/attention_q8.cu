@@ -90,8 +90,7 @@ template <typename T, int NT> struct Form {
     static constexpr int MERGE = (int)sizeof(float) * WARPS * 8 * NT * LD;
     static constexpr int Q_BYTES = Q_SHARED ? (int)sizeof(uint32_t) * WARPS * 32 * Q_REGS : 0;
     // the tiles (at the end the meeting of the warps takes their place), then the queries
-    static constexpr int SCALAR = (int)sizeof(float) * (WARPS + 1) * HD;     // (behind the meeting: the scalar form's)
-    static constexpr int Q_AT = ((TILES > MERGE + SCALAR ? TILES : MERGE + SCALAR) + 1023) / 1024 * 1024;
+    static constexpr int Q_AT = ((TILES > MERGE ? TILES : MERGE) + 1023) / 1024 * 1024;
     static constexpr size_t smem() { return 1024 + Q_AT + Q_BYTES; }
 };
 
@@ -159,21 +158,22 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
-// One query over the keys lo .. hi that it sees, key after key, by all warps of the CTA: sums relative to m (base 2) in
-// acc [HD], and (m, l).  For tiles in which a NaN came out: a product on the tensor cores multiplies also what a query does
-// not see, by zero, and zero times a NaN is one.
+// One query over the keys lo .. hi that it sees, key after key, by a warp: sums relative to m (base 2) in o (entry
+// lane + 32 c), and (m, l).  For tiles in which a NaN came out: a product on the tensor cores multiplies also what a query
+// does not see, by zero, and zero times a NaN is one.
 template <typename T>
 __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args& a, const int* __restrict__ table, int g,
-                                           int lo, int hi, float* acc, float* ml, float* smem) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int blocks = a.page_size / a.block;
-    float x[DPL], o[DPL], m = LOWEST, l = 0.f;
+                                           int lo, int hi, float* o, float& m, float& l) {
+    const int lane = threadIdx.x & 31, blocks = a.page_size / a.block;
+    float x[DPL];
+    m = LOWEST;
+    l = 0.f;
 #pragma unroll
     for (int c = 0; c < DPL; ++c) {
         x[c] = lane + 32 * c < HD ? to_float(q[lane + 32 * c]) * a.scale_log2 : 0.f;
         o[c] = 0.f;
     }
-    for (int j = lo + warp; j <= hi; j += WARPS) {
+    for (int j = lo; j <= hi; ++j) {
         const int page = table[j / a.page_size], off = j % a.page_size;
         if (page < 0) continue;
         const int64_t k_plane = (int64_t)page * 2 * a.G + g, v_plane = k_plane + a.G;
@@ -192,23 +192,6 @@ __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args
         for (int c = 0; c < DPL; ++c)
             if (lane + 32 * c < HD) o[c] = o[c] * keep + pv * q8_float2(v[lane + 32 * c]).x;
     }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < DPL; ++c)
-        if (lane + 32 * c < HD) smem[warp * HD + lane + 32 * c] = o[c];
-    if (lane == 0) { ml[2 * warp] = m; ml[2 * warp + 1] = l; }
-    __syncthreads();
-    float top = LOWEST, total = 0.f;
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[2 * w]);
-    for (int w = 0; w < WARPS; ++w) total += ml[2 * w + 1] * exp2f(ml[2 * w] - top);
-    for (int d = threadIdx.x; d < HD; d += THREADS) {
-        float sum = 0.f;
-        for (int w = 0; w < WARPS; ++w) sum += smem[w * HD + d] * exp2f(ml[2 * w] - top);
-        acc[d] = sum;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) { ml[2 * WARPS] = top; ml[2 * WARPS + 1] = total; }
-    __syncthreads();
 }
 
 // The queries of a row and kv head are packed: p = token * GS + j is the row's token `token` and query head g GS + j.  A
@@ -227,7 +210,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     uint8_t* tiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     float* smem = reinterpret_cast<float*>(tiles);
     __shared__ uint64_t full[WARPS];
-    __shared__ float sm_m[WARPS][8 * NT], sm_l[WARPS][8 * NT], sm_ml[2 * WARPS + 2];
+    __shared__ float sm_m[WARPS][8 * NT], sm_l[WARPS][8 * NT];
     __shared__ float all_top[WARPS * 8 * NT], all_total[WARPS * 8 * NT];      // of the CTA, for the cluster
 
     if (threadIdx.x == 0 && a.tiled) asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
@@ -630,16 +613,16 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     }
     // a NaN, and not all queries see the same keys: each of them by itself
     if (__syncthreads_or(odd) && first_pos != last_pos) {
-        float* scratch = reinterpret_cast<float*>(tiles + F::MERGE);
-        float* acc = scratch + WARPS * HD;
-        for (int i = 0; i < nq; ++i) {
+        for (int i = warp; i < nq; i += WARPS) {
             const int p = q0 + i, tok = p / GS, pos = pos0 + tok;
             const int lo = max(k_lo + tile_begin * KT, a.window > 0 ? pos - a.window + 1 : 0);
             const int hi = min(k_lo + tile_end * KT - 1, pos);
+            float sum[DPL], top, total;
             attend_scalar<T>(q + (int64_t)(t0 + tok) * a.q_stride + (int64_t)(g * GS + p - tok * GS) * HD, a, table, g, lo, hi,
-                             acc, sm_ml, scratch);
-            for (int d = tid; d < HD; d += THREADS) leave(i, d, acc[d], sm_ml[2 * WARPS], sm_ml[2 * WARPS + 1]);
-            __syncthreads();
+                             sum, top, total);
+#pragma unroll
+            for (int c = 0; c < DPL; ++c)
+                if (lane + 32 * c < HD) leave(i, lane + 32 * c, sum[c], top, total);
         }
     }
     if (a.n_splits > 1 && a.cluster) {
@@ -696,6 +679,39 @@ __global__ void __launch_bounds__(128) attn_q8_merge_kernel(T* __restrict__ out,
         if (lane + 32 * c < HD)
             out[(int64_t)(t0 + tok) * a.out_stride + (int64_t)h * HD + lane + 32 * c] =
                 from_float<T>(total == 0.f ? 0.f : sum[c] / total);
+}
+
+// After portions were attended to in 16 bits: where their keys or values hold a NaN (a byte of `odd` is set) every query by
+// itself, a warp at a time; else nothing.
+template <typename T>
+__global__ void __launch_bounds__(128) attn_q8_odd_kernel(const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ odd,
+                                                          int64_t n_odd, int n_list, const Q8Args a) {
+    pdl_wait();
+    pdl_trigger();
+    bool any = false;
+    const int64_t head = min(n_odd, (int64_t)((16 - ((uintptr_t)odd & 15)) & 15)), words = (n_odd - head) / 16;
+    for (int64_t i = threadIdx.x; i < words; i += 128) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(odd + head) + i);
+        any |= (x.x | x.y | x.z | x.w) != 0u;
+    }
+    for (int64_t i = threadIdx.x; i < head; i += 128) any |= odd[i] != 0;
+    for (int64_t i = head + words * 16 + threadIdx.x; i < n_odd; i += 128) any |= odd[i] != 0;
+    if (!__syncthreads_or(any)) return;
+    const int lane = threadIdx.x & 31, GS = a.H / a.G;
+    for (int k = 0; k < n_list; ++k) {
+        const int r = a.row_list ? a.row_list[k] : k, t0 = a.row_start[r], n_new = a.row_start[r + 1] - t0;
+        for (int64_t i = blockIdx.x * 4 + threadIdx.x / 32; i < (int64_t)n_new * a.H; i += gridDim.x * 4) {
+            const int tok = (int)(i / a.H), h = (int)(i - (int64_t)tok * a.H), pos = a.row_pos0[r] + tok;
+            float sum[DPL], top, total;
+            attend_scalar<T>(q + (int64_t)(t0 + tok) * a.q_stride + (int64_t)h * HD, a, a.table + (int64_t)r * a.table_stride, h / GS,
+                             a.window > 0 ? max(0, pos - a.window + 1) : 0, pos, sum, top, total);
+#pragma unroll
+            for (int c = 0; c < DPL; ++c)
+                if (lane + 32 * c < HD)
+                    out[(int64_t)(t0 + tok) * a.out_stride + (int64_t)h * HD + lane + 32 * c] =
+                        from_float<T>(total == 0.f ? 0.f : sum[c] / total);
+        }
+    }
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -815,4 +831,18 @@ SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages,
                        : launch<float, 2>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
     return nt == 1 ? launch<bf16, 1>((const bf16*)q, (bf16*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream)
                    : launch<bf16, 2>((const bf16*)q, (bf16*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
+}
+
+// See attn_q8_odd_kernel; odd: n_odd bytes.
+SLLM_EXPORT int sllm_attn_q8_odd(const void* q, int64_t q_stride, const void* pages, const void* scales, const int* table,
+                                 int table_stride, int page_size, int block, const int* row_start, const int* row_pos0,
+                                 const int* row_list, int n_list, void* out, int64_t out_stride, int H, int G, float scale,
+                                 int window, const uint8_t* odd, int64_t n_odd, cudaStream_t stream) {
+    if (n_list <= 0 || n_odd <= 0) return 0;
+    if (H <= 0 || G <= 0 || H % G || page_size <= 0 || block <= 0 || page_size % block) return (int)cudaErrorInvalidValue;
+    const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
+                      nullptr, 0, table_stride, page_size, block, H, G, window, 1, 1, 0, 0, 0, 0, scale * LOG2E,
+                      divisor(page_size), divisor(block)};
+    return (int)sllm_launch_pdl(attn_q8_odd_kernel<__nv_bfloat16>, dim3(148), dim3(128), 0, stream, (const __nv_bfloat16*)q,
+                                (__nv_bfloat16*)out, odd, n_odd, n_list, a);
 }

@@ -240,38 +240,66 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
     }
 }
 
-// The values of positions row_from[r] .. row_to[r] - 1 of every row, into pages of T through a table of their
-// own.  A page is one run of bytes; a thread takes READ_PIECES pieces of 16.  grid (pieces of a page, pages of a
-// row, rows).
+// Reading back: the values of positions from .. to - 1 of a row, into pages of T through a table of their own.  A page is
+// one run of bytes; a thread takes READ_PIECES pieces of 16.  grid (pieces of a page, pages of a row, rows).
 constexpr int READ_THREADS = 256, READ_PIECES = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(READ_THREADS)
-kv_read_q8_kernel(const uint8_t* __restrict__ pages, const uint8_t* __restrict__ scales, const int* __restrict__ table,
-                  int table_stride, const int* __restrict__ row_from, const int* __restrict__ row_to, T* __restrict__ out,
-                  const int* __restrict__ out_table, int out_stride, int page_size, int block, int G, int hd, int first_row) {
+struct ReadArgs {
+    const uint8_t* pages; const uint8_t* scales; const int* table; int table_stride;
+    int page_size, block, G, hd, first_row;
+    // positions [row_from[r], row_to[r]) of row r through out_table, or, where row_start is given: everything that the
+    // queries of the listed rows see, page p of the i-th of them to page i * listed_pages + p, which the kernel writes
+    // into out_table[r] itself (-1 where a page is not needed); odd[i * listed_pages + p, blockIdx.x] is set to whether
+    // the CTA met a NaN
+    const int* row_from; const int* row_to;
+    const int* row_start; const int* row_pos0; const int* row_list; int window, listed_pages;
+    int* out_table; int out_stride; uint8_t* odd;
+};
+
+template <typename T, bool LISTED>
+__global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict__ out, const ReadArgs a) {
     pdl_wait();
     pdl_trigger();
-    const int r = first_row + blockIdx.z;
-    const int from = max(row_from[r], 0), to = row_to[r];
-    const int pieces = 2 * G * page_size * hd / 16;
-    for (int64_t p = from / page_size + (int64_t)blockIdx.y; p * page_size < to; p += gridDim.y) {
-        const int page = table[(int64_t)r * table_stride + p], out_page = out_table[(int64_t)r * out_stride + p];
-        if (page < 0 || out_page < 0) continue;
-        const uint8_t* src = pages + (int64_t)page * pieces * 16;
-        const uint8_t* sc = scales + (int64_t)page * (2 * G * (page_size / block));
+    const int i = a.first_row + blockIdx.z, r = a.row_list ? a.row_list[i] : i;
+    const int page_size = a.page_size, pieces = 2 * a.G * page_size * a.hd / 16;
+    constexpr bool listed = LISTED;
+    int from, to;
+    if (listed) {
+        const int n_new = a.row_start[r + 1] - a.row_start[r], pos0 = a.row_pos0[r];
+        to = n_new > 0 ? pos0 + n_new : 0;
+        // (whole pages: what the first one holds in front of the window meets a probability of zero)
+        from = a.window > 0 ? max(0, pos0 - a.window + 1) / page_size * page_size : 0;
+    } else {
+        from = max(a.row_from[r], 0);
+        to = a.row_to[r];
+    }
+    const int64_t p_end = listed ? a.listed_pages : ((int64_t)to + page_size - 1) / page_size;
+    for (int64_t p = (listed ? 0 : from / page_size) + (int64_t)blockIdx.y; p < p_end; p += gridDim.y) {
+        const bool needed = p >= from / page_size && p * page_size < to;
+        const int page = needed ? a.table[(int64_t)r * a.table_stride + p] : -1;
+        int out_page;
+        if (listed) {
+            out_page = page >= 0 ? (int)(i * (int64_t)a.listed_pages + p) : -1;
+            if (blockIdx.x == 0 && threadIdx.x == 0) a.out_table[(int64_t)r * a.out_stride + p] = out_page;
+        } else {
+            out_page = needed ? a.out_table[(int64_t)r * a.out_stride + p] : -1;
+        }
+        if (!listed && (page < 0 || out_page < 0)) continue;
+        const uint8_t* src = a.pages + (int64_t)page * pieces * 16;
+        const uint8_t* sc = a.scales + (int64_t)page * (2 * a.G * (page_size / a.block));
         T* dst = out + (int64_t)out_page * pieces * 16;
         const int c0 = blockIdx.x * READ_THREADS * READ_PIECES + threadIdx.x;
         uint4 x[READ_PIECES];
         int b[READ_PIECES];
+        bool odd = false;
 #pragma unroll
         for (int k = 0; k < READ_PIECES; ++k) {
-            const int c = c0 + k * READ_THREADS, row = c * 16 / hd;         // of the page's 2 G page_size rows
+            const int c = c0 + k * READ_THREADS, row = c * 16 / a.hd;       // of the page's 2 G page_size rows
             const int64_t pos = p * page_size + row % page_size;
             b[k] = -1;
-            if (c < pieces && pos >= from && pos < to) {
+            if (out_page >= 0 && c < pieces && pos >= from && pos < to) {
                 x[k] = __ldg(reinterpret_cast<const uint4*>(src) + c);
-                b[k] = sc[row / block];
+                b[k] = sc[row / a.block];
             }
         }
 #pragma unroll
@@ -282,6 +310,7 @@ kv_read_q8_kernel(const uint8_t* __restrict__ pages, const uint8_t* __restrict__
             float v[16];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                if (listed) odd |= ((w[j] & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u) != 0u;
                 const float2 lo = q8_float2(w[j] & 0xffffu), hi = q8_float2(w[j] >> 16);
                 v[4 * j] = lo.x * power;
                 v[4 * j + 1] = lo.y * power;
@@ -289,6 +318,10 @@ kv_read_q8_kernel(const uint8_t* __restrict__ pages, const uint8_t* __restrict__
                 v[4 * j + 3] = hi.y * power;
             }
             store_w<T, 16>(dst + (int64_t)(c0 + k * READ_THREADS) * 16, v);
+        }
+        if (listed) {
+            const int any = __syncthreads_or(odd);
+            if (threadIdx.x == 0) a.odd[(i * (int64_t)a.listed_pages + p) * gridDim.x + blockIdx.x] = any != 0;
         }
     }
 }
@@ -350,28 +383,54 @@ SLLM_EXPORT int sllm_rope_kv_write_q8(const void* qkv, void* q_out, const int* r
                 : launch_write<__nv_bfloat16, 1>(qkv, q_out, a, kv_ctas + q_ctas, threads, stream);
 }
 
-SLLM_EXPORT int sllm_kv_read_q8(const void* pages, const void* scales, const int* table, int table_stride,
-                                const int* row_from, const int* row_to, void* out, const int* out_table, int out_stride,
-                                int n_rows, int max_tokens, int page_size, int block, int G, int hd, int dtype,
-                                cudaStream_t stream) {
-    if (n_rows <= 0 || max_tokens <= 0) return 0;
-    if (G <= 0 || hd <= 0 || hd % 16 || page_size <= 0 || block <= 0 || page_size % block ||
-        (int64_t)G * page_size * hd > (1 << 27) || (((uintptr_t)pages | (uintptr_t)out) & 15) || (dtype != 0 && dtype != 1))
+static int launch_read(void* out, ReadArgs a, int n_rows, int64_t most, int dtype, cudaStream_t stream) {
+    if (a.G <= 0 || a.hd <= 0 || a.hd % 16 || a.page_size <= 0 || a.block <= 0 || a.page_size % a.block ||
+        (int64_t)a.G * a.page_size * a.hd > (1 << 27) || (((uintptr_t)a.pages | (uintptr_t)out) & 15) ||
+        (dtype != 0 && dtype != 1))
         return (int)cudaErrorInvalidValue;
-    const int pieces = 2 * G * page_size * hd / 16, per = READ_THREADS * READ_PIECES;
-    // (max_tokens positions that start anywhere touch this many pages)
-    int64_t most = (int64_t)(max_tokens - 1) / page_size + 2;
+    const int pieces = 2 * a.G * a.page_size * a.hd / 16, per = READ_THREADS * READ_PIECES;
     if (most > 65535) most = 65535;
     for (int r = 0; r < n_rows; r += 65535) {
+        a.first_row = r;
         const dim3 grid((pieces + per - 1) / per, (unsigned)most, n_rows - r < 65535 ? n_rows - r : 65535);
-        const cudaError_t e = dtype == 0
-            ? sllm_launch_pdl(kv_read_q8_kernel<float>, grid, dim3(READ_THREADS), 0, stream, (const uint8_t*)pages,
-                              (const uint8_t*)scales, table, table_stride, row_from, row_to, (float*)out, out_table,
-                              out_stride, page_size, block, G, hd, r)
-            : sllm_launch_pdl(kv_read_q8_kernel<__nv_bfloat16>, grid, dim3(READ_THREADS), 0, stream, (const uint8_t*)pages,
-                              (const uint8_t*)scales, table, table_stride, row_from, row_to, (__nv_bfloat16*)out, out_table,
-                              out_stride, page_size, block, G, hd, r);
+        const cudaError_t e =
+            a.row_start && dtype == 1 ? sllm_launch_pdl(kv_read_q8_kernel<__nv_bfloat16, true>, grid, dim3(READ_THREADS), 0,
+                                                        stream, (__nv_bfloat16*)out, a)
+            : a.row_start ? cudaErrorInvalidValue
+            : dtype == 0 ? sllm_launch_pdl(kv_read_q8_kernel<float, false>, grid, dim3(READ_THREADS), 0, stream, (float*)out, a)
+                         : sllm_launch_pdl(kv_read_q8_kernel<__nv_bfloat16, false>, grid, dim3(READ_THREADS), 0, stream,
+                                           (__nv_bfloat16*)out, a);
         if (e != cudaSuccess) return (int)e;
     }
     return 0;
+}
+
+SLLM_EXPORT int sllm_kv_read_q8(const void* pages, const void* scales, const int* table, int table_stride,
+                                const int* row_from, const int* row_to, void* out, int* out_table, int out_stride,
+                                int n_rows, int max_tokens, int page_size, int block, int G, int hd, int dtype,
+                                cudaStream_t stream) {
+    if (n_rows <= 0 || max_tokens <= 0) return 0;
+    if (page_size <= 0) return (int)cudaErrorInvalidValue;
+    const ReadArgs a = {(const uint8_t*)pages, (const uint8_t*)scales, table, table_stride, page_size, block, G, hd, 0,
+                        row_from, row_to, nullptr, nullptr, nullptr, 0, 0, out_table, out_stride, nullptr};
+    // (max_tokens positions that start anywhere touch this many pages)
+    return launch_read(out, a, n_rows, (int64_t)(max_tokens - 1) / page_size + 2, dtype, stream);
+}
+
+SLLM_EXPORT int sllm_kv_read_q8_shares(int page_size, int G, int hd) {
+    return (int)(((int64_t)2 * G * page_size * hd / 16 + READ_THREADS * READ_PIECES - 1) / (READ_THREADS * READ_PIECES));
+}
+
+// What the queries of the listed rows see (row_list null: rows 0 .. n_list - 1), at most listed_pages pages a row, into
+// out [n_list * listed_pages, 2, G, page_size, hd]; row r's part of out_table names the pages.  odd: a byte for each page and
+// sllm_kv_read_q8_shares() of it, not 0 where a NaN was met.  bfloat16 only.
+SLLM_EXPORT int sllm_kv_read_q8_listed(const void* pages, const void* scales, const int* table, int table_stride,
+                                       const int* row_start, const int* row_pos0, const int* row_list, int n_list,
+                                       int window, int listed_pages, void* out, int* out_table, int out_stride, uint8_t* odd,
+                                       int page_size, int block, int G, int hd, cudaStream_t stream) {
+    if (n_list <= 0 || listed_pages <= 0) return 0;
+    if ((int64_t)n_list * listed_pages > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    const ReadArgs a = {(const uint8_t*)pages, (const uint8_t*)scales, table, table_stride, page_size, block, G, hd, 0,
+                        nullptr, nullptr, row_start, row_pos0, row_list, window, listed_pages, out_table, out_stride, odd};
+    return launch_read(out, a, n_list, listed_pages, 1, stream);
 }

@@ -1064,6 +1064,43 @@ def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_n
     return nt, wq, best, best <= 8 and base * best <= _sm_count(device)
 
 
+#: from this many packed queries (new tokens x query heads of a kv head) in a row on, bfloat16 portions are read back into
+#: pages of 16 bits and attended to by the tcgen05 kernel
+Q8_TC_MIN_PACKED_QUERIES = 128
+#: what the portions' keys and values in 16 bits may take at once; rows beyond it follow in launches of their own
+Q8_WORKSPACE_BYTES = 1 << 30
+
+
+def _attention_q8_portions(q, pages, scales, block_table, page_size, block, row_start, row_pos0, out, row_list, n_list,
+                           max_new, max_context, n_heads, n_kv_heads, head_dim, scale, window) -> None:
+    width = -(-max_context // page_size)
+    page_bytes = 4 * n_kv_heads * page_size * head_dim
+    shares = int(_core("sllm_kv_q8").sllm_kv_read_q8_shares(c_int(page_size), c_int(n_kv_heads), c_int(head_dim)))
+    at_once = max(1, min(n_list, Q8_WORKSPACE_BYTES // (width * page_bytes)))
+    n_rows = n_list if row_list is None else row_start.numel() - 1
+    for first in range(0, n_list, at_once):
+        n = min(at_once, n_list - first)
+        # (all rows in order: the ones of this launch by themselves; else the list's part of it)
+        if row_list is None:
+            rows, listed, starts, pos0, table = n, None, row_start[first:], row_pos0[first:], block_table[first:]
+        else:
+            rows, listed, starts, pos0, table = n_rows, row_list[first:first + n], row_start, row_pos0, block_table
+        plain = torch.empty((n * width, 2, n_kv_heads, page_size, head_dim), dtype=q.dtype, device=q.device)
+        plain_table = torch.empty((rows, width), dtype=torch.int32, device=q.device)
+        odd = torch.empty(n * width * shares, dtype=torch.uint8, device=q.device)
+        _check(_core("sllm_kv_q8").sllm_kv_read_q8_listed(
+            _ptr(pages), _ptr(scales), _ptr(table), c_int(table.stride(0)), _ptr(starts), _ptr(pos0), _ptr(listed), c_int(n),
+            c_int(window or 0), c_int(width), _ptr(plain), _ptr(plain_table), c_int(width), _ptr(odd), c_int(page_size), c_int(block),
+            c_int(n_kv_heads), c_int(head_dim), _stream()), "kv_read_q8")
+        attention_tc(q, plain, plain_table, page_size, starts, pos0, out, listed, n, max_new, n_heads, n_kv_heads, head_dim,
+                     scale, window)
+        _check(_load(*attention_q8_library(head_dim)).sllm_attn_q8_odd(
+            _ptr(q), c_int64(q.stride(0)), _ptr(pages), _ptr(scales), _ptr(table), c_int(table.stride(0)), c_int(page_size),
+            c_int(block), _ptr(starts), _ptr(pos0), _ptr(listed), c_int(n), _ptr(out), c_int64(out.stride(0)), c_int(n_heads),
+            c_int(n_kv_heads), c_float(scale), c_int(window or 0), _ptr(odd), c_int64(odd.numel()), _stream()),
+            "attention_q8")
+
+
 def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, page_size: int,
                  row_start: torch.Tensor, row_pos0: torch.Tensor, out: torch.Tensor, row_list: torch.Tensor | None,
                  n_list: int, max_new: int, max_context: int, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
@@ -1090,6 +1127,12 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     _here(q=q, pages=pages, scales=scales, block_table=block_table, row_start=row_start, row_pos0=row_pos0, out=out,
           row_list=row_list)
     if n_list <= 0 or max_new <= 0:
+        return out
+    if q.dtype == torch.bfloat16 and max_new * (n_heads // n_kv_heads) >= Q8_TC_MIN_PACKED_QUERIES \
+            and attention_tc_supports(n_heads, n_kv_heads, head_dim, page_size, window, biased=bool(window)) \
+            and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0:
+        _attention_q8_portions(q, pages, scales, block_table, page_size, block, row_start, row_pos0, out, row_list, n_list,
+                               max_new, max_context, n_heads, n_kv_heads, head_dim, scale, window)
         return out
     nt, wq, n_splits, cluster = _attention_q8_plan(q.get_device(), head_dim, _code(q.dtype), n_list, max_new, max_context, n_heads,
                                           n_kv_heads, window or 0)

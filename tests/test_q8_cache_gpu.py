@@ -217,15 +217,22 @@ def attend_on_device(c, q, rows, dev, H, scale, window=0, row_list=None, out=Non
                             context or max(b + m for b, m in listed), H, c.G, c.hd, scale, window or None)
 
 
-def tolerance(dtype, hd, want, spread, reach):
-    """The result's rounding; the probabilities' before they multiply v (11 bits, or 21 in the 32-bit form); a score's
-    error, at most hd roundings of 32-bit sums (of 2^-22 each on the tensor cores) of the sum of its products' sizes, which
+def tolerance(dtype, hd, want, spread, reach, portion=False):
+    """The result's rounding; the probabilities' before they multiply v (11 bits, or 21 in the 32-bit form; in portions
+    that the tcgen05 kernel takes 8 bits, a bfloat16 of them: off by at most 2^-8 of each, sum_j 2^-8 p_j |v_j|, and as
+    much again for the denominator where it sums the rounded ones); a score's error, at most hd roundings of 32-bit sums (of 2^-22 each on the tensor cores) of the sum of its products' sizes, which
     moves its probability by as much; and the 32-bit sums over the keys."""
     H = reach.shape[1]
     moved = (2.0 ** -22 * hd * reach).expand(-1, -1, hd).reshape(want.shape)
     if dtype == torch.bfloat16:
-        return 2.0 ** -8 * want.abs() + (2.0 ** -10 + 2 * moved) * spread
+        return 2.0 ** -8 * want.abs() + ((2.0 ** -7 if portion else 2.0 ** -10) + 2 * moved) * spread
     return 2.0 ** -23 * want.abs() + (2.0 ** -19 + 2 * moved) * spread
+
+
+def is_portion(c, rows, dtype, H):
+    from scratch_llm_b200.kernels import ops
+    return dtype == torch.bfloat16 and max(m for _, m in rows) * (H // c.G) >= ops.Q8_TC_MIN_PACKED_QUERIES and \
+        ops.attention_tc_supports(H, c.G, c.hd, c.page, None)
 
 
 def check(c, q, rows, dtype, H, window=0, n=None, **kw):
@@ -235,7 +242,7 @@ def check(c, q, rows, dtype, H, window=0, n=None, **kw):
     want, spread, reach = plain.attend(q, c.pages, c.scales, c.table, rows, c.page, H, c.G, c.hd, scale, window)
     n = want.shape[0]
     far = (got[:n].double().cpu() - want).abs()
-    tol = tolerance(dtype, c.hd, want, spread, reach)
+    tol = tolerance(dtype, c.hd, want, spread, reach, is_portion(c, rows, dtype, H))
     assert not got[:n].isnan().any()
     assert (far <= tol).all(), f"worst {(far / tol.clamp(min=1e-300)).max():.3g} of the tolerance"
     assert (got[n:] == 7).all()
@@ -314,8 +321,36 @@ def test_attention_values_that_are_no_numbers(dtype, H, G, hd, rows):
     assert torch.equal(got.isnan(), want.isnan())
     assert want.isnan().any() and not want[:2].isnan().any()
     fine = ~want.isnan()
-    tol = tolerance(dtype, hd, want, spread, reach)
+    tol = tolerance(dtype, hd, want, spread, reach, is_portion(c, rows, dtype, H))
     assert ((got - want).abs() <= tol)[fine].all()
+
+
+@pytest.mark.parametrize("window", [0, 150])
+def test_attention_portions_in_several_launches(window, monkeypatch):
+    """Portions whose keys and values in 16 bits do not fit the workspace at once, all rows and listed ones; what lies
+    behind a window may have been given back."""
+    from scratch_llm_b200.kernels import ops
+    H, G, hd, page = 8, 2, 64, 16
+    rows = [(300, 40), (20, 70), (0, 33), (511, 128), (7, 0), (64, 35)]
+    gen = torch.Generator().manual_seed(11)
+    c = Cache(G, hd, page, 8, [b + m for b, m in rows], gen).fill([(b + m, 0) for b, m in rows], gen, 0.5)
+    q = torch.randn(sum(m for _, m in rows), H * hd, generator=gen).bfloat16()
+    if window:
+        for r, (b, _) in enumerate(rows):
+            c.table[r, :max(0, b - window + 1) // page] = -1
+    monkeypatch.setattr(ops, "Q8_WORKSPACE_BYTES", 2 * 4 * G * 640 * hd)
+    dev, s = c.device(), starts(rows)
+    want, spread, reach = plain.attend(q, c.pages, c.scales, c.table, rows, page, H, G, hd, hd ** -0.5, window)
+    tol = tolerance(torch.bfloat16, hd, want, spread, reach, True)
+    got = attend_on_device(c, q.to(DEV), rows, dev, H, hd ** -0.5, window).double().cpu()
+    assert ((got - want).abs() <= tol).all()
+    got = attend_on_device(c, q.to(DEV), rows, dev, H, hd ** -0.5, window, row_list=[3, 0, 5, 1]).double().cpu()
+    for r in range(len(rows)):
+        part = slice(s[r], s[r + 1])
+        if r in (0, 1, 3, 5):
+            assert ((got[part] - want[part]).abs() <= tol[part]).all()
+        else:
+            assert (got[part] == 7).all()
 
 
 def test_attention_far_scales():
