@@ -918,46 +918,85 @@ Q8_MAX_HEAD_DIM = 256
 Q8_MAX_BLOCK_ENTRIES = 32768
 
 
-def _here(**tensors: torch.Tensor | None) -> None:
-    """Every tensor lies on the current device, whose stream the kernel is launched on."""
-    device = torch.cuda.current_device()
-    for name, t in tensors.items():
-        if t is not None and t.get_device() != device:
-            raise KernelError(f"{name} is on {t.device}, the current device is cuda:{device}")
+def _device() -> int:
+    """The current device, on whose stream kernels are launched."""
+    return _current_device() if _current_device is not None else torch.cuda.current_device()
 
 
-def _i32_rows(t: torch.Tensor, n: int, name: str) -> None:
-    _need(t, torch.int32, name)
-    if t.dim() != 1 or t.numel() < n:
-        raise KernelError(f"{name} must have {n} entries")
+def _stream_of(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def _table(t: torch.Tensor, n_rows: int, name: str) -> None:
-    _need(t, torch.int32, name, contiguous=False)
-    if t.dim() != 2 or t.shape[0] < n_rows or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise KernelError(f"{name} must have {n_rows} contiguous rows")
+# The operators below are called for every layer of every step: what a call checks is one expression per tensor, and only
+# a tensor that fails it is asked what is wrong (_refuse).
+
+def _is(t: torch.Tensor, dtype: torch.dtype, device: int) -> bool:
+    return t.dtype is dtype and t.get_device() == device and t.is_contiguous()
 
 
-def _q8_cache(pages: torch.Tensor, scales: torch.Tensor, n_kv_heads: int, page_size: int, head_dim: int) -> int:
-    """Checks a cache in 8 bits and returns the tokens of its blocks."""
-    _need(pages, Q8_DTYPE, "pages")
-    _need(scales, Q8_SCALE_DTYPE, "scales")
-    if pages.dim() != 5 or pages.shape[1:] != (2, n_kv_heads, page_size, head_dim):
-        raise KernelError(f"pages must be [n_pages, 2, {n_kv_heads}, {page_size}, {head_dim}], got {list(pages.shape)}")
-    if scales.dim() != 4 or scales.shape[:3] != (pages.shape[0], 2, n_kv_heads) or scales.shape[3] < 1 \
-            or page_size % scales.shape[3]:
-        raise KernelError(f"scales must be [{pages.shape[0]}, 2, {n_kv_heads}, blocks of a page] with blocks that divide "
-                          f"the page's {page_size} tokens, got {list(scales.shape)}")
+def _is_rows(t: torch.Tensor, device: int, n: int) -> bool:
+    return t.dtype is torch.int32 and t.get_device() == device and t.is_contiguous() and t.dim() == 1 and t.numel() >= n
+
+
+def _is_table(t: torch.Tensor, device: int, n_rows: int) -> bool:
+    return t.dtype is torch.int32 and t.get_device() == device and t.dim() == 2 and t.size(0) >= n_rows \
+        and (t.size(1) <= 1 or t.stride(1) == 1)
+
+
+def _is_matrix(t: torch.Tensor, dtype: torch.dtype, device: int, rows: int, columns: int) -> bool:
+    return t.dtype is dtype and t.get_device() == device and t.dim() == 2 and t.size(0) == rows and t.size(1) == columns \
+        and (columns <= 1 or t.stride(1) == 1)
+
+
+def _refuse(t: torch.Tensor, name: str, dtype: torch.dtype | None, device: int, wanted: str) -> None:
+    _need(t, dtype, name, contiguous=False)
+    if t.get_device() != device:
+        raise KernelError(f"{name} is on {t.device}, the current device is cuda:{device}")
+    raise KernelError(f"{name} must be {wanted}, got {list(t.shape)} with strides {list(t.stride())}")
+
+
+@functools.lru_cache(maxsize=256)
+def _q8_block(n_pages: int, g: int, page_size: int, head_dim: int, scales: tuple) -> int:
+    """The tokens of a block of a cache in 8 bits of these sizes; refuses what the kernels do not take."""
+    if len(scales) != 4 or scales[:3] != (n_pages, 2, g) or scales[3] < 1 or page_size % scales[3]:
+        raise KernelError(f"scales must be [{n_pages}, 2, {g}, blocks of a page] with blocks that divide the page's "
+                          f"{page_size} tokens, got {list(scales)}")
     if head_dim % 16 or not 16 <= head_dim <= Q8_MAX_HEAD_DIM:
         raise KernelError(f"head size {head_dim}: a cache in 8 bits takes multiples of 16 up to {Q8_MAX_HEAD_DIM}")
-    block = page_size // scales.shape[3]
+    block = page_size // scales[3]
     if block * head_dim > Q8_MAX_BLOCK_ENTRIES:
         raise KernelError(f"blocks of {block} tokens of {head_dim} entries: at most {Q8_MAX_BLOCK_ENTRIES} entries")
-    if not 1 <= pages.shape[0] <= ((1 << 31) - 1) // (2 * n_kv_heads):
-        raise KernelError(f"{pages.shape[0]} pages: from 1 to {((1 << 31) - 1) // (2 * n_kv_heads)} are taken")
+    if g * page_size * head_dim > 1 << 27:
+        raise KernelError(f"pages of {page_size} tokens, {g} heads of {head_dim}: at most 2^27 entries a plane")
+    if not 1 <= n_pages <= ((1 << 31) - 1) // (2 * g):
+        raise KernelError(f"{n_pages} pages: from 1 to {((1 << 31) - 1) // (2 * g)} are taken")
+    return block
+
+
+def _q8_cache(pages: torch.Tensor, scales: torch.Tensor, n_kv_heads: int, page_size: int, head_dim: int,
+              device: int) -> int:
+    """Checks a cache in 8 bits and returns the tokens of its blocks."""
+    shape = pages.shape
+    if not (_is(pages, Q8_DTYPE, device) and len(shape) == 5 and shape[1] == 2 and shape[2] == n_kv_heads
+            and shape[3] == page_size and shape[4] == head_dim):
+        _refuse(pages, "pages", Q8_DTYPE, device, f"contiguous [n_pages, 2, {n_kv_heads}, {page_size}, {head_dim}]")
+    if not _is(scales, Q8_SCALE_DTYPE, device):
+        _refuse(scales, "scales", Q8_SCALE_DTYPE, device, "contiguous [n_pages, 2, kv heads, blocks of a page]")
+    block = _q8_block(shape[0], n_kv_heads, page_size, head_dim, tuple(scales.shape))
     if pages.data_ptr() % 16:
         raise KernelError("pages must start on a 16-byte boundary")
     return block
+
+
+@functools.lru_cache(maxsize=None)
+def _q8_function(name: str, head_dim: int, signature: str):
+    """An entry of the 8-bit cache's libraries (of the attention's where ``head_dim`` is given) that takes plain numbers:
+    p a pointer, i an int, l a 64-bit int, f a float."""
+    lib = _load(*attention_q8_library(head_dim)) if head_dim else \
+        _core("sllm_drafts" if name == "sllm_verify_drafts" else "sllm_kv_q8")
+    function = getattr(lib, name)
+    function.argtypes = [{"p": c_void_p, "i": c_int, "l": c_int64, "f": c_float}[c] for c in signature]
+    return function
 
 
 def rope_kv_write_q8(qkv: torch.Tensor, row_start: torch.Tensor, row_pos0: torch.Tensor, n_rows: int, max_new: int,
@@ -972,38 +1011,41 @@ def rope_kv_write_q8(qkv: torch.Tensor, row_start: torch.Tensor, row_pos0: torch
     earlier tokens keeps its scale or takes a larger one, at which the earlier tokens' numbers are rounded again.
     Infinities and NaN are stored as NaN.  Two rows of a step share no block.  Tables of fewer than ``head_dim / 2``
     columns rotate only the first ``2 * columns`` entries of a head; ``cos`` None rotates nothing."""
-    _need(qkv, None, "qkv")
-    _need(q_out, qkv.dtype, "q_out")
-    block = _q8_cache(pages, scales, n_kv_heads, page_size, head_dim)
-    n = qkv.shape[0]
-    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim:
-        raise KernelError("qkv width does not match the head counts")
-    if q_out.shape != (n, n_heads * head_dim):
-        raise KernelError(f"q_out must be [{n}, {n_heads * head_dim}], got {list(q_out.shape)}")
-    _i32_rows(row_start, n_rows + 1, "row_start")
-    _i32_rows(row_pos0, n_rows, "row_pos0")
-    _table(block_table, n_rows, "block_table")
-    rot = 0
+    device, dtype = _device(), qkv.dtype
+    code = _code(dtype)
+    block = _q8_cache(pages, scales, n_kv_heads, page_size, head_dim, device)
+    n, width = qkv.size(0), (n_heads + 2 * n_kv_heads) * head_dim
+    if not (_is(qkv, dtype, device) and qkv.dim() == 2 and qkv.size(1) == width):
+        _refuse(qkv, "qkv", None, device, f"contiguous [tokens, {width}]")
+    if not (_is(q_out, dtype, device) and q_out.dim() == 2 and q_out.size(0) == n and q_out.size(1) == n_heads * head_dim):
+        _refuse(q_out, "q_out", dtype, device, f"contiguous [{n}, {n_heads * head_dim}]")
+    if not _is_rows(row_start, device, n_rows + 1):
+        _refuse(row_start, "row_start", torch.int32, device, f"{n_rows + 1} entries")
+    if not _is_rows(row_pos0, device, n_rows):
+        _refuse(row_pos0, "row_pos0", torch.int32, device, f"{n_rows} entries")
+    if not _is_table(block_table, device, n_rows):
+        _refuse(block_table, "block_table", torch.int32, device, f"{n_rows} contiguous rows")
+    rot, cos_at, sin_at, bias_at = 0, 0, 0, 0
     if cos is not None:
-        _need(cos, torch.float32, "cos")
-        _need(sin, torch.float32, "sin")
-        if cos.dim() != 2 or not 1 <= cos.shape[1] <= head_dim // 2 or sin.shape != cos.shape:
-            raise KernelError("rotary table width")
-        rot = 2 * cos.shape[1]
+        rot = 2 * cos.size(-1)
+        if not (_is(cos, torch.float32, device) and cos.dim() == 2 and 2 <= rot <= head_dim):
+            _refuse(cos, "cos", torch.float32, device, f"contiguous [positions, 1 to {head_dim // 2}]")
+        if sin is None or not (_is(sin, torch.float32, device) and sin.shape == cos.shape):
+            _refuse(cos if sin is None else sin, "sin", torch.float32, device, "a table like cos")
+        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
     if bias is not None:
-        _need(bias, torch.float32, "bias")
-        if bias.numel() != qkv.shape[1]:
-            raise KernelError("bias must have one entry per column of qkv")
-    _here(qkv=qkv, q_out=q_out, row_start=row_start, row_pos0=row_pos0, cos=cos, sin=sin, pages=pages, scales=scales,
-          block_table=block_table, bias=bias)
-    for t, name in ((qkv, "qkv"), (q_out, "q_out"), (cos, "cos"), (sin, "sin"), (bias, "bias")):
-        if t is not None and t.data_ptr() % 16:
-            raise KernelError(f"{name} must start on a 16-byte boundary")
-    _check(_core("sllm_kv_q8").sllm_rope_kv_write_q8(
-        _ptr(qkv), _ptr(q_out), _ptr(row_start), _ptr(row_pos0), c_int(n_rows), c_int(n), c_int(max_new), _ptr(cos),
-        _ptr(sin), c_int(rot), c_int(int(interleaved)), _ptr(bias), _ptr(pages), _ptr(scales), _ptr(block_table),
-        c_int(block_table.stride(0)), c_int(page_size), c_int(block), c_int(n_heads), c_int(n_kv_heads), c_int(head_dim),
-        c_int(int(write)), c_int(_code(qkv.dtype)), _stream()), "rope_kv_write_q8")
+        if not (_is(bias, torch.float32, device) and bias.numel() == width):
+            _refuse(bias, "bias", torch.float32, device, f"{width} entries, one per column of qkv")
+        bias_at = bias.data_ptr()
+    q_at, out_at = qkv.data_ptr(), q_out.data_ptr()
+    if (q_at | out_at | cos_at | sin_at | bias_at) % 16:
+        raise KernelError("qkv, q_out, cos, sin and bias must start on 16-byte boundaries")
+    if q_at == out_at and n > 0:
+        raise KernelError("q_out must be memory of its own: qkv stays as it is")
+    _check(_q8_function("sllm_rope_kv_write_q8", 0, "ppppiiippiippppiiiiiiiip")(
+        q_at, out_at, row_start.data_ptr(), row_pos0.data_ptr(), n_rows, n, max_new, cos_at, sin_at, rot, int(interleaved),
+        bias_at, pages.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), page_size, block,
+        n_heads, n_kv_heads, head_dim, int(write), code, _stream_of(device)), "rope_kv_write_q8")
 
 
 def kv_read_q8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, page_size: int,
@@ -1012,25 +1054,29 @@ def kv_read_q8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Ten
     """Reads a cache in 8 bits back: the keys and values at the positions ``row_from[r]`` to ``row_to[r] - 1`` of every
     row (at most ``max_tokens``) go to the same places of the pages that ``out_table`` names, ``out``
     [n, 2, G, page_size, hd] in bfloat16 or float32, in which they are exact.  All other places are left alone."""
-    _need(out, None, "out")
-    if out.dim() != 5:
-        raise KernelError(f"out must be [n, 2, kv heads, {page_size}, head size], got {list(out.shape)}")
-    _, _, g, _, hd = out.shape
-    block = _q8_cache(pages, scales, g, page_size, hd)
-    if out.shape[1:] != pages.shape[1:]:
-        raise KernelError(f"out must have pages like the cache's {list(pages.shape[1:])}, got {list(out.shape[1:])}")
-    _i32_rows(row_from, n_rows, "row_from")
-    _i32_rows(row_to, n_rows, "row_to")
-    _table(block_table, n_rows, "block_table")
-    _table(out_table, n_rows, "out_table")
-    _here(pages=pages, scales=scales, block_table=block_table, row_from=row_from, row_to=row_to, out=out,
-          out_table=out_table)
-    if out.data_ptr() % 16:
+    device, dtype, shape = _device(), out.dtype, out.shape
+    code = _code(dtype)
+    if not (_is(out, dtype, device) and len(shape) == 5):
+        _refuse(out, "out", None, device, f"contiguous [n, 2, kv heads, {page_size}, head size]")
+    g, hd = shape[2], shape[4]
+    block = _q8_cache(pages, scales, g, page_size, hd, device)
+    if shape[1] != 2 or shape[3] != page_size:
+        _refuse(out, "out", None, device, f"pages like the cache's, [n, 2, {g}, {page_size}, {hd}]")
+    if not _is_rows(row_from, device, n_rows):
+        _refuse(row_from, "row_from", torch.int32, device, f"{n_rows} entries")
+    if not _is_rows(row_to, device, n_rows):
+        _refuse(row_to, "row_to", torch.int32, device, f"{n_rows} entries")
+    if not _is_table(block_table, device, n_rows):
+        _refuse(block_table, "block_table", torch.int32, device, f"{n_rows} contiguous rows")
+    if not _is_table(out_table, device, n_rows):
+        _refuse(out_table, "out_table", torch.int32, device, f"{n_rows} contiguous rows")
+    at = out.data_ptr()
+    if at % 16:
         raise KernelError("out must start on a 16-byte boundary")
-    _check(_core("sllm_kv_q8").sllm_kv_read_q8(
-        _ptr(pages), _ptr(scales), _ptr(block_table), c_int(block_table.stride(0)), _ptr(row_from), _ptr(row_to), _ptr(out),
-        _ptr(out_table), c_int(out_table.stride(0)), c_int(n_rows), c_int(max_tokens), c_int(page_size), c_int(block),
-        c_int(g), c_int(hd), c_int(_code(out.dtype)), _stream()), "kv_read_q8")
+    _check(_q8_function("sllm_kv_read_q8", 0, "pppippppiiiiiiiip")(
+        pages.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), row_from.data_ptr(),
+        row_to.data_ptr(), at, out_table.data_ptr(), out_table.stride(0), n_rows, max_tokens, page_size, block, g, hd, code,
+        _stream_of(device)), "kv_read_q8")
     return out
 
 
@@ -1072,10 +1118,10 @@ Q8_WORKSPACE_BYTES = 1 << 30
 
 
 def _attention_q8_portions(q, pages, scales, block_table, page_size, block, row_start, row_pos0, out, row_list, n_list,
-                           max_new, max_context, n_heads, n_kv_heads, head_dim, scale, window) -> None:
+                           max_new, max_context, n_heads, n_kv_heads, head_dim, scale, window, stream) -> None:
     width = -(-max_context // page_size)
     page_bytes = 4 * n_kv_heads * page_size * head_dim
-    shares = int(_core("sllm_kv_q8").sllm_kv_read_q8_shares(c_int(page_size), c_int(n_kv_heads), c_int(head_dim)))
+    shares = _q8_function("sllm_kv_read_q8_shares", 0, "iii")(page_size, n_kv_heads, head_dim)
     at_once = max(1, min(n_list, Q8_WORKSPACE_BYTES // (width * page_bytes)))
     n_rows = n_list if row_list is None else row_start.numel() - 1
     for first in range(0, n_list, at_once):
@@ -1088,17 +1134,17 @@ def _attention_q8_portions(q, pages, scales, block_table, page_size, block, row_
         plain = torch.empty((n * width, 2, n_kv_heads, page_size, head_dim), dtype=q.dtype, device=q.device)
         plain_table = torch.empty((rows, width), dtype=torch.int32, device=q.device)
         odd = torch.empty(n * width * shares, dtype=torch.uint8, device=q.device)
-        _check(_core("sllm_kv_q8").sllm_kv_read_q8_listed(
-            _ptr(pages), _ptr(scales), _ptr(table), c_int(table.stride(0)), _ptr(starts), _ptr(pos0), _ptr(listed), c_int(n),
-            c_int(window or 0), c_int(width), _ptr(plain), _ptr(plain_table), c_int(width), _ptr(odd), c_int(page_size), c_int(block),
-            c_int(n_kv_heads), c_int(head_dim), _stream()), "kv_read_q8")
+        listed_at = 0 if listed is None else listed.data_ptr()
+        _check(_q8_function("sllm_kv_read_q8_listed", 0, "pppipppiiippipiiiip")(
+            pages.data_ptr(), scales.data_ptr(), table.data_ptr(), table.stride(0), starts.data_ptr(), pos0.data_ptr(),
+            listed_at, n, window, width, plain.data_ptr(), plain_table.data_ptr(), width, odd.data_ptr(), page_size, block,
+            n_kv_heads, head_dim, stream), "kv_read_q8")
         attention_tc(q, plain, plain_table, page_size, starts, pos0, out, listed, n, max_new, n_heads, n_kv_heads, head_dim,
-                     scale, window)
-        _check(_load(*attention_q8_library(head_dim)).sllm_attn_q8_odd(
-            _ptr(q), c_int64(q.stride(0)), _ptr(pages), _ptr(scales), _ptr(table), c_int(table.stride(0)), c_int(page_size),
-            c_int(block), _ptr(starts), _ptr(pos0), _ptr(listed), c_int(n), _ptr(out), c_int64(out.stride(0)), c_int(n_heads),
-            c_int(n_kv_heads), c_float(scale), c_int(window or 0), _ptr(odd), c_int64(odd.numel()), _stream()),
-            "attention_q8")
+                     scale, window or None)
+        _check(_q8_function("sllm_attn_q8_odd", head_dim, "plpppiiipppipliifiplp")(
+            q.data_ptr(), q.stride(0), pages.data_ptr(), scales.data_ptr(), table.data_ptr(), table.stride(0), page_size, block,
+            starts.data_ptr(), pos0.data_ptr(), listed_at, n, out.data_ptr(), out.stride(0), n_heads, n_kv_heads, scale,
+            window, odd.data_ptr(), odd.numel(), stream), "attention_q8")
 
 
 def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, page_size: int,
@@ -1109,42 +1155,47 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     bits (:func:`rope_kv_write_q8`), for single tokens, drafted tokens and portions of prompts alike.  ``q`` [N, H * hd] may be
     a column slice; bfloat16 or float32, and ``out`` likewise.  No row brings more than ``max_new`` tokens, and no query
     stands at a position of ``max_context`` or more."""
-    _need(q, None, "q", contiguous=False)
-    _need(out, q.dtype, "out", contiguous=False)
-    block = _q8_cache(pages, scales, n_kv_heads, page_size, head_dim)
-    if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] != n_heads * head_dim or out.shape != q.shape or out.stride(1) != 1:
-        raise KernelError("attention q/out layout")
+    device, dtype, n, width = _device(), q.dtype, q.size(0), n_heads * head_dim
+    code = _code(dtype)
+    block = _q8_cache(pages, scales, n_kv_heads, page_size, head_dim, device)
+    if not _is_matrix(q, dtype, device, n, width):
+        _refuse(q, "q", None, device, f"[tokens, {width}] with contiguous rows")
+    if not _is_matrix(out, dtype, device, n, width):
+        _refuse(out, "out", dtype, device, f"[{n}, {width}] with contiguous rows")
     if n_heads % n_kv_heads:
         raise KernelError(f"{n_heads} query heads do not group evenly over {n_kv_heads} kv heads")
-    if row_list is not None:
-        _i32_rows(row_list, n_list, "row_list")
-    need = n_list if row_list is None else 1
-    _i32_rows(row_start, need + 1, "row_start")
-    _i32_rows(row_pos0, need, "row_pos0")
-    _table(block_table, need, "block_table")
-    if window is not None and window < 0:
+    rows = n_list if row_list is None else 1
+    if row_list is not None and not _is_rows(row_list, device, n_list):
+        _refuse(row_list, "row_list", torch.int32, device, f"{n_list} entries")
+    if not _is_rows(row_start, device, rows + 1):
+        _refuse(row_start, "row_start", torch.int32, device, f"{rows + 1} entries")
+    if not _is_rows(row_pos0, device, rows):
+        _refuse(row_pos0, "row_pos0", torch.int32, device, f"{rows} entries")
+    if not _is_table(block_table, device, rows):
+        _refuse(block_table, "block_table", torch.int32, device, f"{rows} contiguous rows")
+    window = window or 0
+    if window < 0:
         raise KernelError(f"window must not be negative, got {window}")
-    _here(q=q, pages=pages, scales=scales, block_table=block_table, row_start=row_start, row_pos0=row_pos0, out=out,
-          row_list=row_list)
     if n_list <= 0 or max_new <= 0:
         return out
-    if q.dtype == torch.bfloat16 and max_new * (n_heads // n_kv_heads) >= Q8_TC_MIN_PACKED_QUERIES \
+    stream = _stream_of(device)
+    if code == 1 and max_new * (n_heads // n_kv_heads) >= Q8_TC_MIN_PACKED_QUERIES \
             and attention_tc_supports(n_heads, n_kv_heads, head_dim, page_size, window, biased=bool(window)) \
             and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0:
         _attention_q8_portions(q, pages, scales, block_table, page_size, block, row_start, row_pos0, out, row_list, n_list,
-                               max_new, max_context, n_heads, n_kv_heads, head_dim, scale, window)
+                               max_new, max_context, n_heads, n_kv_heads, head_dim, scale, window, stream)
         return out
-    nt, wq, n_splits, cluster = _attention_q8_plan(q.get_device(), head_dim, _code(q.dtype), n_list, max_new, max_context, n_heads,
-                                          n_kv_heads, window or 0)
+    nt, wq, n_splits, cluster = _attention_q8_plan(device, head_dim, code, n_list, max_new, max_context, n_heads, n_kv_heads,
+                                                   window)
     part = None
     if n_splits > 1 and not cluster:
-        part = torch.empty(q.shape[0] * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
-    _check(_load(*attention_q8_library(head_dim)).sllm_attn_q8(
-        _ptr(q), c_int64(q.stride(0)), _ptr(pages), c_int64(pages.shape[0]), _ptr(scales), _ptr(block_table),
-        c_int(block_table.stride(0)), c_int(page_size), c_int(block), _ptr(row_start), _ptr(row_pos0), _ptr(row_list), c_int(n_list), c_int(max_new),
-        _ptr(out), c_int64(out.stride(0)), c_int(n_heads), c_int(n_kv_heads), c_float(scale), c_int(window or 0),
-        c_int(_code(q.dtype)), c_int(nt), c_int(wq), c_int(n_splits), _ptr(part), c_int64(q.shape[0]),
-        c_int(int(cluster)), _stream()), "attention_q8")
+        part = torch.empty(n * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
+    _check(_q8_function("sllm_attn_q8", head_dim, "plplppiiipppiipliifiiiiiplip")(
+        q.data_ptr(), q.stride(0), pages.data_ptr(), pages.size(0), scales.data_ptr(), block_table.data_ptr(),
+        block_table.stride(0), page_size, block, row_start.data_ptr(), row_pos0.data_ptr(),
+        0 if row_list is None else row_list.data_ptr(), n_list, max_new, out.data_ptr(), out.stride(0), n_heads, n_kv_heads,
+        scale, window, code, nt, wq, n_splits, 0 if part is None else part.data_ptr(), n, int(cluster), stream),
+        "attention_q8")
     return out
 
 
@@ -1164,30 +1215,30 @@ def verify_drafts(probs: torch.Tensor, drafts: torch.Tensor, draft_start: torch.
     drawn token and -1 behind it, ``accepted`` (int32 [n]) how many drafts that are.  A NaN counts as no probability, as
     does a draft outside the vocabulary; where no weight is left the row draws from ``p_i``, and a row of no probability at
     all gets the token -1.  Sums are formed in 64 bits."""
-    _need(probs, torch.float32, "probs", contiguous=False)
-    _need(uniforms, torch.float32, "uniforms")
-    for t, name in ((drafts, "drafts"), (draft_start, "draft_start"), (tokens, "tokens"), (accepted, "accepted")):
-        _need(t, torch.int32, name)
-    n, k = accepted.numel(), drafts.numel()
-    if probs.dim() != 2 or probs.shape[0] != k + n or probs.shape[1] < 1 or (probs.shape[1] > 1 and probs.stride(1) != 1):
-        raise KernelError(f"probs must be [{k + n}, V] with contiguous rows, got {list(probs.shape)}")
-    if draft_start.numel() != n + 1 or uniforms.numel() != k + n or tokens.numel() != k + n:
-        raise KernelError(f"{k} drafts in {n} rows need {n + 1} starts and {k + n} uniforms and tokens")
-    if draft_probs is not None:
-        _need(draft_probs, torch.float32, "draft_probs", contiguous=False)
-        if draft_probs.shape != (k, probs.shape[1]) or (probs.shape[1] > 1 and draft_probs.stride(1) != 1):
-            raise KernelError(f"draft_probs must be [{k}, {probs.shape[1]}] with contiguous rows, got "
-                              f"{list(draft_probs.shape)}")
+    device, n, k = _device(), accepted.numel(), drafts.numel()
+    if not _is_rows(drafts, device, 0):
+        _refuse(drafts, "drafts", torch.int32, device, "a vector")
+    if not _is_rows(accepted, device, 0):
+        _refuse(accepted, "accepted", torch.int32, device, "a vector")
+    v = probs.size(-1)
+    if v < 1 or not _is_matrix(probs, torch.float32, device, k + n, v):
+        _refuse(probs, "probs", torch.float32, device, f"[{k + n}, V] with contiguous rows")
+    if not (_is_rows(draft_start, device, 0) and draft_start.numel() == n + 1):
+        _refuse(draft_start, "draft_start", torch.int32, device, f"{n + 1} entries for {n} rows")
+    if not (_is(uniforms, torch.float32, device) and uniforms.numel() == k + n):
+        _refuse(uniforms, "uniforms", torch.float32, device, f"{k + n} entries for {k} drafts in {n} rows")
+    if not (_is_rows(tokens, device, 0) and tokens.numel() == k + n):
+        _refuse(tokens, "tokens", torch.int32, device, f"{k + n} entries for {k} drafts in {n} rows")
+    if draft_probs is not None and not _is_matrix(draft_probs, torch.float32, device, k, v):
+        _refuse(draft_probs, "draft_probs", torch.float32, device, f"[{k}, {v}] with contiguous rows")
     if max_drafts < 0:
         raise KernelError(f"max_drafts must not be negative, got {max_drafts}")
-    _here(probs=probs, drafts=drafts, draft_start=draft_start, uniforms=uniforms, tokens=tokens, accepted=accepted,
-          draft_probs=draft_probs)
     if n == 0:
         return
-    _check(_core("sllm_drafts").sllm_verify_drafts(
-        _ptr(probs), c_int64(probs.stride(0)), _ptr(draft_probs),
-        c_int64(draft_probs.stride(0) if draft_probs is not None else 0), _ptr(drafts), _ptr(draft_start), _ptr(uniforms),
-        c_int(n), c_int(probs.shape[1]), _ptr(tokens), _ptr(accepted), _stream()), "verify_drafts")
+    _check(_q8_function("sllm_verify_drafts", 0, "plplpppiippp")(
+        probs.data_ptr(), probs.stride(0), 0 if draft_probs is None else draft_probs.data_ptr(),
+        0 if draft_probs is None else draft_probs.stride(0), drafts.data_ptr(), draft_start.data_ptr(), uniforms.data_ptr(), n,
+        v, tokens.data_ptr(), accepted.data_ptr(), _stream_of(device)), "verify_drafts")
 
 
 def argmax_scratch_bytes(n_rows: int) -> int:
