@@ -26,9 +26,7 @@ struct WriteArgs {
     int64_t n_tasks, n_q_items;
 };
 
-// a thread keeps up to 64 entries in registers
-constexpr int WRITE_THREADS = 512;
-template <int W> constexpr int WRITE_UNITS = 32 / W;
+constexpr int WRITE_THREADS = 256;
 
 // Unit u of a head: 2 W entries, W at e0 and W at e1; turned pairs are (e0 + i, e1 + i), or, where neighbours
 // pair, the pairs within 2 W neighbouring entries.  Entries that do not turn come 2 W neighbours at a time.
@@ -51,7 +49,15 @@ template <typename T, int W> __device__ __forceinline__ void load_w(const T* p, 
 }
 template <typename T, int W> __device__ __forceinline__ void store_w(T* p, const float* v) {
     if constexpr (W == 1) p[0] = from_float<T>(v[0]);
-    else {
+    else if constexpr (W < Vec<T>::N) {
+        uint32_t w[W / 2];
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
 #pragma unroll
         for (int i = 0; i < W; i += Vec<T>::N) Vec<T>::store(p + i, v + i);
     }
@@ -64,12 +70,39 @@ __device__ __forceinline__ void load_angles(const WriteArgs& a, const Unit<W>& u
     load_w<float, W>(a.sin_t + (int64_t)pos * (a.rot / 2) + u.pair0, s);
 }
 
-// One unit of a head: loaded, with the bias, turned.  v[0 .. W): the entries at e0, v[W .. 2 W): those at e1.
+// One unit of a head as it lies in memory: of a thread's units all are requested before the first is worked on.
+template <typename T, int W> struct Raw {
+    static constexpr int WORDS = (2 * W * (int)sizeof(T) + 3) / 4, HALF = W * (int)sizeof(T);
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const T* head, const Unit<W>& u) {
+        if constexpr (HALF == 16) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(head + u.e0)), y = __ldg(reinterpret_cast<const uint4*>(head + u.e1));
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+            w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+        } else if constexpr (HALF == 8) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>(head + u.e0)), y = __ldg(reinterpret_cast<const uint2*>(head + u.e1));
+            w[0] = x.x; w[1] = x.y; w[2] = y.x; w[3] = y.y;
+        } else if constexpr (HALF == 4) {
+            w[0] = __float_as_uint(to_float(__ldg(head + u.e0)));
+            w[1] = __float_as_uint(to_float(__ldg(head + u.e1)));
+        } else {
+            w[0] = (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(head) + u.e0) |
+                   (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(head) + u.e1) << 16;
+        }
+    }
+    // v[0 .. W): the entries at e0, v[W .. 2 W): those at e1
+    __device__ __forceinline__ void values(float* v) const {
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i)
+            v[i] = sizeof(T) == 4 ? __uint_as_float(w[i]) : __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+};
+
+// A unit's values with the bias, turned.
 template <typename T, int W>
-__device__ __forceinline__ void load_unit(const WriteArgs& a, const T* head, const float* bias, const Unit<W>& u,
-                                          bool turns, const float* c, const float* s, float* v) {
-    load_w<T, W>(head + u.e0, v);
-    load_w<T, W>(head + u.e1, v + W);
+__device__ __forceinline__ void unit_values(const WriteArgs& a, const Raw<T, W>& raw, const float* bias, const Unit<W>& u,
+                                            bool turns, const float* c, const float* s, float* v) {
+    raw.values(v);
     if (bias != nullptr) {
         float b[2 * W];
         load_w<float, W>(bias + u.e0, b);
@@ -93,48 +126,69 @@ __device__ __forceinline__ void load_unit(const WriteArgs& a, const T* head, con
     }
 }
 
-// the row of token n: the last one that starts at or before it and is not empty
-__device__ __forceinline__ int row_of(const WriteArgs& a, int n) {
-    int lo = 0, hi = a.n_rows - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (a.row_start[mid] <= n) lo = mid; else hi = mid - 1;
+// The last row r with row_start[r] < bound - step * r (the left side grows with r, the right one does not): 16 rows a
+// look, whose loads do not wait for one another.
+__device__ __forceinline__ int last_row(const WriteArgs& a, int64_t bound, int step) {
+    int lo = 0, n = a.n_rows;
+    while (n > 1) {
+        const int stride = (n + 15) / 16;
+        int past = 0;
+#pragma unroll
+        for (int j = 1; j < 16; ++j)
+            if (j * stride < n) past += (int64_t)a.row_start[lo + j * stride] < bound - (int64_t)step * (lo + j * stride);
+        lo += past * stride;
+        n = min(stride, n - past * stride);
     }
     return lo;
 }
+// the row of token n: the last one that starts at or before it
+__device__ __forceinline__ int row_of(const WriteArgs& a, int n) { return last_row(a, (int64_t)n + 1, 0); }
 
-// CTAs 0 .. kv_ctas - 1: a group of a.lanes threads takes one block of the cache (what a row stores in it), for
-// one plane and kv head.  Row r has the slots from row_start[r] / block + 2 r on, at least as many as it touches
-// blocks: n new tokens touch at most n / block + 2.  The other CTAs turn the queries.
+// CTAs 0 .. kv_ctas - 1: a group of a.lanes threads takes one block of the cache (what a row stores in it), for one
+// plane and kv head, twice: for its largest value, then, from L1, to store it: blocks of any size, and room for the warps
+// that its chain of look-ups and two reads wants.  8,192 tokens of 32 + 8 + 8 heads of 128, blocks of 16, with the queries:
+// 53 us (29 at the copy rate); 1,581 tokens of 3 x 40 heads, blocks of 64, in 32 bits with biases: 52 (22).  With the block
+// in registers 49 and 60, eight entries at a time instead of four 52 and 55, several heads a group in a row 42 and 68.
+// Row r has the slots from
+// row_start[r] / block + 2 r on, at least as many as it touches blocks: n new tokens touch at most n / block + 2.  The
+// other CTAs turn the queries.
 template <typename T, int W>
-__global__ void __launch_bounds__(WRITE_THREADS)
+__global__ void __launch_bounds__(WRITE_THREADS, 4)
 rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const WriteArgs a) {
-    __shared__ float warp_top[WRITE_THREADS / 32];
+    __shared__ float warp_top[2][WRITE_THREADS / 32];
     pdl_wait();
     pdl_trigger();
     const int heads = a.H + 2 * a.G, upt = a.hd / (2 * W);
     if ((int)blockIdx.x >= a.kv_ctas) {
-        // ---- queries: a thread takes a unit of a token and walks a share of the token's heads with it
+        // ---- queries: a thread takes a unit of a token and walks a share of the token's heads with it (an item: a token's
+        // share of heads)
         const int per_group = (a.H + a.q_groups - 1) / a.q_groups;
-        for (int64_t i = (int64_t)(blockIdx.x - a.kv_ctas) * blockDim.x + threadIdx.x; i < a.n_q_items;
-             i += (int64_t)(gridDim.x - a.kv_ctas) * blockDim.x) {
-            const int u_ = (int)(i % upt);
-            const int64_t t = i / upt;
-            const int group = (int)(t % a.q_groups), n = (int)(t / a.q_groups);
+        const int at_once = blockDim.x / upt, u_ = threadIdx.x % upt;
+        if ((int)threadIdx.x >= at_once * upt) return;
+        for (int64_t i = (int64_t)(blockIdx.x - a.kv_ctas) * at_once + threadIdx.x / upt; i < a.n_q_items;
+             i += (int64_t)(gridDim.x - a.kv_ctas) * at_once) {
+            const int n = (int)((uint32_t)i / (uint32_t)a.q_groups), group = (int)((uint32_t)i - (uint32_t)n * a.q_groups);
             if (n >= a.row_start[a.n_rows]) continue;
             const int r = row_of(a, n), pos = a.row_pos0[r] + n - a.row_start[r];
             const Unit<W> u(u_, a.rot, a.interleaved);
             float c[W], s[W];
             load_angles<W>(a, u, pos, c, s);
             const int end = min(a.H, (group + 1) * per_group);
-#pragma unroll 2
-            for (int h = group * per_group; h < end; ++h) {
-                float v[2 * W];
-                load_unit<T, W>(a, qkv + ((int64_t)n * heads + h) * a.hd, a.bias ? a.bias + (int64_t)h * a.hd : nullptr,
-                                u, true, c, s, v);
-                T* to = q_out + ((int64_t)n * a.H + h) * a.hd;
-                store_w<T, W>(to + u.e0, v);
-                store_w<T, W>(to + u.e1, v + W);
+            constexpr int HEADS = sizeof(T) == 2 ? 4 : 2;      // requested at a time
+            for (int h0 = group * per_group; h0 < end; h0 += HEADS) {
+                Raw<T, W> raw[HEADS];
+#pragma unroll
+                for (int j = 0; j < HEADS; ++j) raw[j].load(qkv + ((int64_t)n * heads + min(h0 + j, end - 1)) * a.hd, u);
+#pragma unroll
+                for (int j = 0; j < HEADS; ++j) {
+                    const int h = h0 + j;
+                    if (h >= end) break;
+                    float v[2 * W];
+                    unit_values<T, W>(a, raw[j], a.bias ? a.bias + (int64_t)h * a.hd : nullptr, u, true, c, s, v);
+                    T* to = q_out + ((int64_t)n * a.H + h) * a.hd;
+                    store_w<T, W>(to + u.e0, v);
+                    store_w<T, W>(to + u.e1, v + W);
+                }
             }
         }
         return;
@@ -143,17 +197,12 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
     const int lanes = a.lanes, in_cta = blockDim.x / lanes;
     const int64_t task = (int64_t)blockIdx.x * in_cta + threadIdx.x / lanes;
     const int lane = threadIdx.x % lanes;
-    const int pg = (int)(task % (2 * a.G)), plane = pg / a.G, g = pg - plane * a.G;
-    const int slot = (int)(task / (2 * a.G));
+    const int slot = (int)(task / (2 * a.G)), pg = (int)(task - (int64_t)slot * 2 * a.G), plane = pg / a.G, g = pg - plane * a.G;
     bool live = task < a.n_tasks;
     int r = slot, at = 0;
     if (live && !a.single) {
-        int lo = 0, hi = a.n_rows - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (a.row_start[mid] / a.block + 2 * mid <= slot) lo = mid; else hi = mid - 1;
-        }
-        r = lo;
+        // row_start[r] / block + 2 r <= slot
+        r = last_row(a, ((int64_t)slot + 1) * a.block, 2 * a.block);
         at = slot - (a.row_start[r] / a.block + 2 * r);
     }
     int t0 = 0, pos0 = 0, n_old = 0, first = 0, count = 0;
@@ -167,38 +216,70 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
         n_old = first - begin;
         live = count > 0;
     }
-    int page = -1, cell = 0, had = 0;
-    if (live) {
-        const int begin = first - n_old;
-        page = a.table[(int64_t)r * a.table_stride + begin / a.page_size];
-        cell = begin % a.page_size;
-        live = page >= 0;                                         // (no page, nothing to store)
-    }
+    // (the page is looked up while the values are on their way)
+    const int begin = first - n_old, cell = begin % a.page_size;
+    const int page = live ? a.table[(int64_t)r * a.table_stride + begin / a.page_size] : -1;
+    const float* bias = a.bias ? a.bias + (int64_t)(a.H + pg) * a.hd : nullptr;
+    const T* src = qkv + ((int64_t)(t0 + first - pos0) * heads + a.H + pg) * a.hd;
+    // every unit of the block's new tokens, `lanes` at a time, AT_ONCE of them requested before the first is worked on:
+    // use(token, unit, values)
+    constexpr int AT_ONCE = sizeof(T) == 2 ? 4 : 2;
+    const int units = live ? count * upt : 0, d_tok = lanes / upt, d_u = lanes - d_tok * upt;
+    auto walk = [&](auto use) {
+        int tok = lane / upt, u_ = lane - tok * upt;
+        for (int i = lane; i < units; i += AT_ONCE * lanes) {
+            Raw<T, W> raw[AT_ONCE];
+            int toks[AT_ONCE], us[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                toks[k] = tok;
+                us[k] = u_;
+                if (i + k * lanes < units) raw[k].load(src + (int64_t)tok * heads * a.hd, Unit<W>(u_, a.rot, a.interleaved));
+                tok += d_tok;
+                u_ += d_u;
+                if (u_ >= upt) { u_ -= upt; ++tok; }
+            }
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                if (i + k * lanes >= units) break;
+                const Unit<W> u(us[k], a.rot, a.interleaved);
+                float c[W], s[W], v[2 * W];
+                if (plane == 0) load_angles<W>(a, u, first + toks[k], c, s);
+                unit_values<T, W>(a, raw[k], bias, u, plane == 0, c, s, v);
+                use(toks[k], u, v);
+            }
+        }
+    };
+    int turn = 0;                                                 // of the two places where warps meet
+    auto over_group = [&](float x) {
+        for (int o = min(lanes, 32) / 2; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+        if (lanes > 32) {                                         // (the CTA is one group)
+            if ((threadIdx.x & 31) == 0) warp_top[turn][threadIdx.x >> 5] = x;
+            __syncthreads();
+            for (int w = 0; w < lanes / 32; ++w) x = fmaxf(x, warp_top[turn][w]);
+            turn ^= 1;
+        }
+        return x;
+    };
+    float top = 0.f;
+    walk([&](int, const Unit<W>&, const float* v) {
+#pragma unroll
+        for (int j = 0; j < 2 * W; ++j) top = fmaxf(top, fabsf(v[j]));                // (a NaN leaves it as it is)
+    });
     const int64_t plane_of = ((int64_t)page * 2 + plane) * a.G + g;
-    uint8_t* scale = a.scales + (live ? plane_of * (a.page_size / a.block) + cell / a.block : 0);
-    if (live && n_old > 0) had = *scale;
-    const int head = a.H + pg;
-    const float* bias = a.bias ? a.bias + (int64_t)head * a.hd : nullptr;
-    constexpr int UNITS = WRITE_UNITS<W>;
-    float v[UNITS][2 * W], top = 0.f;
+    uint8_t* scale = a.scales + (page >= 0 ? plane_of * (a.page_size / a.block) + cell / a.block : 0);
+    const int had = page >= 0 && n_old > 0 ? *scale : 0;          // (read by all before the group meets, written by one after)
+    top = over_group(top);
+    const bool odd = !q8_finite(top);                             // an infinity: it leaves the scale to the others
+    if (__any_sync(0xffffffffu, odd)) {
+        top = 0.f;
+        walk([&](int, const Unit<W>&, const float* v) {
 #pragma unroll
-    for (int k = 0; k < UNITS; ++k) {
-        const int i = lane + k * lanes, tok = i / upt;
-        if (!live || tok >= count) continue;
-        const Unit<W> u(i - tok * upt, a.rot, a.interleaved);
-        float c[W], s[W];
-        if (plane == 0) load_angles<W>(a, u, first + tok, c, s);
-        load_unit<T, W>(a, qkv + ((int64_t)(t0 + first - pos0 + tok) * heads + head) * a.hd, bias, u, plane == 0, c, s, v[k]);
-#pragma unroll
-        for (int j = 0; j < 2 * W; ++j) top = fmaxf(top, q8_finite(v[k][j]) ? fabsf(v[k][j]) : 0.f);
+            for (int j = 0; j < 2 * W; ++j) top = fmaxf(top, q8_finite(v[j]) ? fabsf(v[j]) : 0.f);
+        });
+        top = over_group(top);
     }
-    for (int o = min(lanes, 32) / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lanes > 32) {                                             // (the CTA is one group)
-        if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
-        __syncthreads();
-        for (int w = 0; w < lanes / 32; ++w) top = fmaxf(top, warp_top[w]);
-    }
-    if (!live) return;
+    if (!live || page < 0) return;                                // (no page, nothing to store)
     const int byte = max(q8_scale_byte(top), had);
     const float inv = q8_inverse(byte);
     uint8_t* cells = a.pages + (plane_of * a.page_size + cell) * a.hd;
@@ -216,33 +297,32 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
             *reinterpret_cast<uint4*>(cells + 16 * i) = x;
         }
     }
-    if (lane == 0) *scale = (uint8_t)byte;
-#pragma unroll
-    for (int k = 0; k < UNITS; ++k) {
-        const int i = lane + k * lanes, tok = i / upt;
-        if (tok >= count) continue;
-        const Unit<W> u(i - tok * upt, a.rot, a.interleaved);
+    walk([&](int tok, const Unit<W>& u, const float* v) {
         uint8_t* to = cells + (int64_t)(n_old + tok) * a.hd;
         float x[2 * W];
 #pragma unroll
-        for (int j = 0; j < 2 * W; ++j) x[j] = q8_finite(v[k][j]) ? v[k][j] * inv : __int_as_float(0x7fffffff);
-        if constexpr (W == 8) {
-            uint32_t w[4];
+        for (int j = 0; j < 2 * W; ++j) x[j] = v[j] * inv;
+        if (odd)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = q8_pack4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
-            *reinterpret_cast<uint2*>(to + u.e0) = make_uint2(w[0], w[1]);
-            *reinterpret_cast<uint2*>(to + u.e1) = make_uint2(w[2], w[3]);
+            for (int j = 0; j < 2 * W; ++j) x[j] = q8_finite(x[j]) ? x[j] : __int_as_float(0x7fffffff);
+        if constexpr (W == 4) {
+            *reinterpret_cast<uint32_t*>(to + u.e0) = q8_pack4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<uint32_t*>(to + u.e1) = q8_pack4(x[4], x[5], x[6], x[7]);
         } else {
             const uint32_t two = q8_pack2(x[0], x[1]);
             to[u.e0] = (uint8_t)two;
             to[u.e1] = (uint8_t)(two >> 8);
         }
-    }
+    });
+    if (lane == 0) *scale = (uint8_t)byte;
 }
 
 // Reading back: the values of positions from .. to - 1 of a row, into pages of T through a table of their own.  A page is
-// one run of bytes; a thread takes READ_PIECES pieces of 16.  grid (pieces of a page, pages of a row, rows).
+// one run of bytes; a thread takes READ_PIECES pieces of it, each of which becomes 32 bytes (131,072 tokens of 8 heads of
+// 128 to bfloat16: 131 us, 0.95 of the copy rate; pieces that become 64 bytes took twice as long in 32 bits).  grid
+// (pieces of a page, pages of a row, rows).
 constexpr int READ_THREADS = 256, READ_PIECES = 4;
+template <typename T> constexpr int READ_BYTES = 32 / (int)sizeof(T);
 
 struct ReadArgs {
     const uint8_t* pages; const uint8_t* scales; const int* table; int table_stride;
@@ -260,8 +340,9 @@ template <typename T, bool LISTED>
 __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict__ out, const ReadArgs a) {
     pdl_wait();
     pdl_trigger();
+    constexpr int BYTES = READ_BYTES<T>, WORDS = BYTES / 4;
     const int i = a.first_row + blockIdx.z, r = a.row_list ? a.row_list[i] : i;
-    const int page_size = a.page_size, pieces = 2 * a.G * page_size * a.hd / 16;
+    const int page_size = a.page_size, pieces = 2 * a.G * page_size * a.hd / BYTES;
     constexpr bool listed = LISTED;
     int from, to;
     if (listed) {
@@ -285,20 +366,26 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict_
             out_page = needed ? a.out_table[(int64_t)r * a.out_stride + p] : -1;
         }
         if (!listed && (page < 0 || out_page < 0)) continue;
-        const uint8_t* src = a.pages + (int64_t)page * pieces * 16;
+        const uint8_t* src = a.pages + (int64_t)page * pieces * BYTES;
         const uint8_t* sc = a.scales + (int64_t)page * (2 * a.G * (page_size / a.block));
-        T* dst = out + (int64_t)out_page * pieces * 16;
+        T* dst = out + (int64_t)out_page * pieces * BYTES;
         const int c0 = blockIdx.x * READ_THREADS * READ_PIECES + threadIdx.x;
-        uint4 x[READ_PIECES];
+        uint32_t x[READ_PIECES][WORDS];
         int b[READ_PIECES];
         bool odd = false;
 #pragma unroll
         for (int k = 0; k < READ_PIECES; ++k) {
-            const int c = c0 + k * READ_THREADS, row = c * 16 / a.hd;       // of the page's 2 G page_size rows
+            const int c = c0 + k * READ_THREADS, row = c * BYTES / a.hd;    // of the page's 2 G page_size rows
             const int64_t pos = p * page_size + row % page_size;
             b[k] = -1;
             if (out_page >= 0 && c < pieces && pos >= from && pos < to) {
-                x[k] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+                if constexpr (WORDS == 4) {
+                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(src) + c);
+                    x[k][0] = w.x; x[k][1] = w.y; x[k][2] = w.z; x[k][3] = w.w;
+                } else {
+                    const uint2 w = __ldg(reinterpret_cast<const uint2*>(src) + c);
+                    x[k][0] = w.x; x[k][1] = w.y;
+                }
                 b[k] = sc[row / a.block];
             }
         }
@@ -306,18 +393,18 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict_
         for (int k = 0; k < READ_PIECES; ++k) {
             if (b[k] < 0) continue;
             const float power = q8_power(b[k]);
-            const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-            float v[16];
+            float v[BYTES];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (listed) odd |= ((w[j] & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u) != 0u;
-                const float2 lo = q8_float2(w[j] & 0xffffu), hi = q8_float2(w[j] >> 16);
+            for (int j = 0; j < WORDS; ++j) {
+                const uint32_t w = x[k][j];
+                if (listed) odd |= ((w & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u) != 0u;
+                const float2 lo = q8_float2(w & 0xffffu), hi = q8_float2(w >> 16);
                 v[4 * j] = lo.x * power;
                 v[4 * j + 1] = lo.y * power;
                 v[4 * j + 2] = hi.x * power;
                 v[4 * j + 3] = hi.y * power;
             }
-            store_w<T, 16>(dst + (int64_t)(c0 + k * READ_THREADS) * 16, v);
+            store_w<T, BYTES>(dst + (int64_t)(c0 + k * READ_THREADS) * BYTES, v);
         }
         if (listed) {
             const int any = __syncthreads_or(odd);
@@ -336,7 +423,7 @@ static int launch_write(const void* qkv, void* q_out, const WriteArgs& a, int64_
                                 (const T*)qkv, (T*)q_out, a);
 }
 
-// write = 0: only the queries.  dtype 0: float32, 1: bfloat16.  block divides page_size and block * hd <= 32768.
+// write = 0: only the queries.  dtype 0: float32, 1: bfloat16.  block divides page_size.
 SLLM_EXPORT int sllm_rope_kv_write_q8(const void* qkv, void* q_out, const int* row_start, const int* row_pos0, int n_rows,
                                       int n_tokens, int max_new, const float* cos_t, const float* sin_t, int rot,
                                       int interleaved, const float* bias, void* pages, void* scales, const int* table,
@@ -344,43 +431,41 @@ SLLM_EXPORT int sllm_rope_kv_write_q8(const void* qkv, void* q_out, const int* r
                                       cudaStream_t stream) {
     if (n_rows <= 0 || n_tokens <= 0 || max_new <= 0) return 0;
     if (H <= 0 || G <= 0 || hd <= 0 || hd % 16 || rot < 0 || rot > hd || rot % 2 || page_size <= 0 || block <= 0 ||
-        page_size % block || (int64_t)block * hd > 64 * WRITE_THREADS || (dtype != 0 && dtype != 1))
+        page_size % block || (dtype != 0 && dtype != 1))
         return (int)cudaErrorInvalidValue;
     if (((uintptr_t)pages | (uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)bias | (uintptr_t)cos_t | (uintptr_t)sin_t) & 15)
         return (int)cudaErrorInvalidValue;
-    const bool wide = rot % 16 == 0;     // (the tables' rows are then whole 16-byte words too)
-    const int W = wide ? 8 : 1;
+    const bool wide = rot % 8 == 0;      // (the tables' rows are then whole 16-byte words too)
+    const int W = wide ? 4 : 1;
     WriteArgs a = {row_start, row_pos0, cos_t, sin_t, bias, (uint8_t*)pages, (uint8_t*)scales, table, table_stride, page_size,
                    block, n_rows, n_tokens, H, G, hd, rot, interleaved, max_new == 1};
     const int upt = hd / (2 * W);
-    // the most that a row stores in a block, in threads of `hold` units
-    const int hold = wide ? WRITE_UNITS<8> : WRITE_UNITS<1>;
-    const int units = (max_new < block ? max_new : block) * upt;
-    const int need = (units + hold - 1) / hold;
-    if (need > WRITE_THREADS) return (int)cudaErrorInvalidValue;
-    if (need <= 32) {
-        a.lanes = 1;
-        // (a unit a thread where a warp holds them all: fewer steps in a row)
-        while (a.lanes < need || (a.lanes < 32 && a.lanes < units)) a.lanes *= 2;
-    } else {
-        a.lanes = (need + 31) / 32 * 32;
-    }
-    const int threads = a.lanes > 32 ? a.lanes : 256;
+    // a block's group: a thread for four units of what a row stores in a block, one for each where a warp holds them
+    const int64_t units = (int64_t)(max_new < block ? max_new : block) * upt;
+    a.lanes = 1;
+    while (a.lanes < WRITE_THREADS && (a.lanes < 32 ? a.lanes < units : 4 * (int64_t)a.lanes < units)) a.lanes *= 2;
+    while (a.lanes > 32 && a.lanes < upt) a.lanes *= 2;      // (upt <= 128: a CTA holds a head)
+    const int threads = a.lanes > 32 ? a.lanes : WRITE_THREADS;
     const int64_t slots = a.single ? n_rows : (int64_t)n_tokens / block + 2 * (int64_t)n_rows;
-    a.n_tasks = write ? slots * 2 * G : 0;
     const int in_cta = threads / a.lanes;
+    a.n_tasks = write ? slots * 2 * G : 0;
     const int64_t kv_ctas = (a.n_tasks + in_cta - 1) / in_cta;
+    // (few tokens share a token's heads out further: a thread's heads come one after the other)
     a.q_groups = H < 4 ? H : 4;
-    a.n_q_items = (int64_t)n_tokens * a.q_groups * upt;
-    int64_t q_ctas = (a.n_q_items + threads - 1) / threads;
+    while (a.q_groups < H && (int64_t)n_tokens * a.q_groups * upt < 148 * 256) a.q_groups = a.q_groups * 2 < H ? a.q_groups * 2 : H;
+    a.n_q_items = (int64_t)n_tokens * a.q_groups;
+    if (a.n_q_items > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    const int at_once = threads / upt;
+    int64_t q_ctas = (a.n_q_items + at_once - 1) / at_once;
     const int64_t most = 148 * 16 * 256 / threads;
     if (q_ctas > most) q_ctas = most;
     if (kv_ctas + q_ctas > 0x7fffffff) return (int)cudaErrorInvalidValue;
     a.kv_ctas = (int)kv_ctas;
-    if (dtype == 0) return wide ? launch_write<float, 8>(qkv, q_out, a, kv_ctas + q_ctas, threads, stream)
-                                : launch_write<float, 1>(qkv, q_out, a, kv_ctas + q_ctas, threads, stream);
-    return wide ? launch_write<__nv_bfloat16, 8>(qkv, q_out, a, kv_ctas + q_ctas, threads, stream)
-                : launch_write<__nv_bfloat16, 1>(qkv, q_out, a, kv_ctas + q_ctas, threads, stream);
+    const int64_t ctas = kv_ctas + q_ctas;
+    if (dtype == 0) return wide ? launch_write<float, 4>(qkv, q_out, a, ctas, threads, stream)
+                                : launch_write<float, 1>(qkv, q_out, a, ctas, threads, stream);
+    return wide ? launch_write<__nv_bfloat16, 4>(qkv, q_out, a, ctas, threads, stream)
+                : launch_write<__nv_bfloat16, 1>(qkv, q_out, a, ctas, threads, stream);
 }
 
 static int launch_read(void* out, ReadArgs a, int n_rows, int64_t most, int dtype, cudaStream_t stream) {
@@ -388,7 +473,8 @@ static int launch_read(void* out, ReadArgs a, int n_rows, int64_t most, int dtyp
         (int64_t)a.G * a.page_size * a.hd > (1 << 27) || (((uintptr_t)a.pages | (uintptr_t)out) & 15) ||
         (dtype != 0 && dtype != 1))
         return (int)cudaErrorInvalidValue;
-    const int pieces = 2 * a.G * a.page_size * a.hd / 16, per = READ_THREADS * READ_PIECES;
+    const int pieces = 2 * a.G * a.page_size * a.hd / (dtype == 0 ? READ_BYTES<float> : READ_BYTES<__nv_bfloat16>),
+              per = READ_THREADS * READ_PIECES;
     if (most > 65535) most = 65535;
     for (int r = 0; r < n_rows; r += 65535) {
         a.first_row = r;
@@ -418,7 +504,7 @@ SLLM_EXPORT int sllm_kv_read_q8(const void* pages, const void* scales, const int
 }
 
 SLLM_EXPORT int sllm_kv_read_q8_shares(int page_size, int G, int hd) {
-    return (int)(((int64_t)2 * G * page_size * hd / 16 + READ_THREADS * READ_PIECES - 1) / (READ_THREADS * READ_PIECES));
+    return (int)(((int64_t)2 * G * page_size * hd / READ_BYTES<__nv_bfloat16> + READ_THREADS * READ_PIECES - 1) / (READ_THREADS * READ_PIECES));
 }
 
 // What the queries of the listed rows see (row_list null: rows 0 .. n_list - 1), at most listed_pages pages a row, into

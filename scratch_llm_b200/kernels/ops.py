@@ -914,8 +914,6 @@ def attention_mma_scratch_floats(n_tokens: int, n_heads: int, head_dim: int, n_s
 Q8_DTYPE, Q8_SCALE_DTYPE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 #: the kernels that read and write such a cache take head sizes that are multiples of 16 up to this
 Q8_MAX_HEAD_DIM = 256
-#: a block of the cache has at most this many entries (tokens x head size): what writes it keeps it in registers
-Q8_MAX_BLOCK_ENTRIES = 32768
 
 
 def _device() -> int:
@@ -964,8 +962,6 @@ def _q8_block(n_pages: int, g: int, page_size: int, head_dim: int, scales: tuple
     if head_dim % 16 or not 16 <= head_dim <= Q8_MAX_HEAD_DIM:
         raise KernelError(f"head size {head_dim}: a cache in 8 bits takes multiples of 16 up to {Q8_MAX_HEAD_DIM}")
     block = page_size // scales[3]
-    if block * head_dim > Q8_MAX_BLOCK_ENTRIES:
-        raise KernelError(f"blocks of {block} tokens of {head_dim} entries: at most {Q8_MAX_BLOCK_ENTRIES} entries")
     if g * page_size * head_dim > 1 << 27:
         raise KernelError(f"pages of {page_size} tokens, {g} heads of {head_dim}: at most 2^27 entries a plane")
     if not 1 <= n_pages <= ((1 << 31) - 1) // (2 * g):

@@ -84,7 +84,8 @@ ROWS = [
 @pytest.mark.parametrize("H,G,hd,rot,interleaved,bias,page,block", [
     (4, 2, 128, 128, True, False, 64, 16), (6, 6, 64, 32, False, True, 16, 16), (3, 1, 80, 40, True, True, 32, 32),
     (8, 2, 16, 0, True, False, 16, 1), (2, 2, 256, 256, False, False, 64, 64), (5, 1, 48, 46, False, False, 12, 3),
-    (2, 1, 112, 2, True, False, 128, 128), (4, 4, 96, 96, False, False, 1, 1)])
+    (2, 1, 112, 2, True, False, 128, 128), (4, 4, 96, 96, False, False, 1, 1),
+    (2, 1, 256, 254, True, True, 64, 32), (3, 3, 240, 2, False, False, 256, 256)])
 def test_write(rows, dtype, H, G, hd, rot, interleaved, bias, page, block):
     gen = torch.Generator().manual_seed(hd + len(rows))
     c = Cache(G, hd, page, block, [b + m for b, m in rows], gen).fill(rows, gen)
