@@ -64,7 +64,7 @@ struct Q8Args {
     const uint8_t* pages; const uint8_t* scales; const int* table;
     const int* row_start; const int* row_pos0; const int* row_list;
     float* part; int64_t part_tokens;                    // [tokens, H, n_splits, HD + 2]: sums, maximum, denominator
-    int table_stride, page_size, block, H, G, window, n_splits, wq, q_vec, run, tiled, cluster;
+    int table_stride, page_size, block, H, G, window, n_splits, q_vec, run, tiled, cluster;
     float scale_log2;
     Divisor page_div, block_div;
 };
@@ -195,8 +195,9 @@ __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args
 }
 
 // The queries of a row and kv head are packed: p = token * GS + j is the row's token `token` and query head g GS + j.  A
-// CTA takes 8 NT wq packed queries over a share of the keys; its warps are wq groups of queries by 4 / wq groups of keys,
-// which take turns at the tiles.  A CTA with fewer queries than the launch allows has fewer groups of queries.  Up to
+// CTA takes 8 NT packed queries over a share of the keys; its warps take turns at the tiles.  (Warps that share the
+// queries between them, up to four times as many a CTA, fetch and turn every key as often, and were slower nearly
+// everywhere: 32 rows of up to six drafted tokens 72 us with two groups of 16, 58 so, 51 with eight queries a CTA.)  Up to
 // eight splits can be a cluster, whose CTAs merge their sums through distributed shared memory (one row of 1,000 keys: 10.3
 // us against 12.4 with a merge kernel); in launches that fill the device clusters find less room than CTAs by themselves (24
 // rows of 4,096 keys of 64, three splits: 47 against 37), and the splits' sums meet in attn_q8_merge_kernel.
@@ -211,7 +212,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     float* smem = reinterpret_cast<float*>(tiles);
     __shared__ uint64_t full[WARPS];
     __shared__ float sm_m[WARPS][8 * NT], sm_l[WARPS][8 * NT];
-    __shared__ float all_top[WARPS * 8 * NT], all_total[WARPS * 8 * NT];      // of the CTA, for the cluster
+    __shared__ float all_top[8 * NT], all_total[8 * NT];      // of the CTA, for the cluster
 
     if (threadIdx.x == 0 && a.tiled) asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
     pdl_wait();
@@ -219,27 +220,20 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n8 = lane >> 2, c4 = lane & 3;
     const int r = a.row_list ? a.row_list[blockIdx.z] : blockIdx.z, g = blockIdx.x, GS = a.H / a.G;
     const int split = blockIdx.y % a.n_splits;
-    const int q0 = ((int)(gridDim.y / a.n_splits) - 1 - (int)blockIdx.y / a.n_splits) * 8 * NT * a.wq;
+    const int q0 = ((int)(gridDim.y / a.n_splits) - 1 - (int)blockIdx.y / a.n_splits) * 8 * NT;
     const int t0 = a.row_start[r], n_packed = (a.row_start[r + 1] - t0) * GS;
     if (q0 >= n_packed) return;
-    const int pos0 = a.row_pos0[r], nq = min(n_packed - q0, 8 * NT * a.wq);
+    const int pos0 = a.row_pos0[r], nq = min(n_packed - q0, 8 * NT);
     const int first_pos = pos0 + q0 / GS, last_pos = pos0 + (q0 + nq - 1) / GS;
-    const int wq = min(a.wq, nq <= 8 * NT ? 1 : nq <= 16 * NT ? 2 : 4), wk = WARPS / wq;
     const int* table = a.table + (int64_t)r * a.table_stride;
     const int k_lo = a.window > 0 ? max(0, first_pos - a.window + 1) / KT * KT : 0;
     const int n_tiles = (last_pos - k_lo) / KT + 1;
     const int per_split = (n_tiles + a.n_splits - 1) / a.n_splits;
     const int tile_begin = min(n_tiles, split * per_split), tile_end = min(n_tiles, tile_begin + per_split);
 
-    // ---- this warp's queries: which they are
-    const int w0 = q0 + (warp % wq) * 8 * NT, w_nq = min(8 * NT, q0 + nq - w0);     // (w_nq may be 0 or less)
-    const int w_first = pos0 + w0 / GS, w_last = pos0 + (w0 + max(w_nq, 1) - 1) / GS;
     // ---- tiles: lane i looks up key i (its page, then its two scales); where a page holds whole tiles lane 0 requests
     // them, else lane i the i-th run of `run` keys
     const int blocks = a.page_size / a.block;
-    int tile_stop = tile_end;             // this warp's queries see nothing from here on
-    if (w_nq <= 0) tile_stop = tile_begin;
-    else tile_stop = min(tile_stop, (w_last - k_lo) / KT + 1);
     uint8_t* mine_at = tiles + warp * F::TILE;
     if (lane == 0) {
         mbar_init(&full[warp], 1);
@@ -249,7 +243,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     __syncwarp();
     auto page_of = [&](int tile) {
         const int kpos = k_lo + tile * KT + lane % KT;
-        return tile < tile_stop && kpos <= w_last ? __ldg(table + a.page_div.quotient(kpos)) : -1;
+        return tile < tile_end && kpos <= last_pos ? __ldg(table + a.page_div.quotient(kpos)) : -1;
     };
     // requests a tile and returns the bytes of this lane's key's two scales; -1: no such key
     auto request = [&](int tile, int page) {
@@ -310,10 +304,10 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
             v_at[k][i] = mine_at + KT * HD + place<KT>(2 * c4 + k, n8 * (HD / 8) + 16 * i, a.tiled);
     constexpr int EIGHT = 8 * WIDTH;         // eight rows
 
-    int tile = tile_begin + warp / wq, page = page_of(tile), sc = -1, parity = 0;
+    int tile = tile_begin + warp, page = page_of(tile), sc = -1, parity = 0;
     bool ok = true;
-    if (tile < tile_stop) sc = request(tile, page);
-    page = page_of(tile + wk);
+    if (tile < tile_end) sc = request(tile, page);
+    page = page_of(tile + WARPS);
 
     // ---- its queries, while the first tile is on its way
     uint32_t qf[F::Q_SHARED ? 1 : PARTS][F::Q_SHARED ? 1 : NT][F::Q_SHARED ? 1 : KSTEPS][2];
@@ -322,8 +316,8 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     int qpos[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int i = nt * 8 + n8, p = w0 + i;
-        const bool there = i < w_nq;
+        const int i = nt * 8 + n8, p = q0 + i;
+        const bool there = i < nq;
         const int tok = there ? p / GS : 0, j = there ? p - tok * GS : 0;
         const T* src = q + (int64_t)(t0 + tok) * a.q_stride + (int64_t)(g * GS + j) * HD + c4 * (HD / 4);
         float x[HD / 4], top = 0.f;
@@ -357,7 +351,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         for (int e = 0; e < 2; ++e) {
             fq[nt][e] = __shfl_sync(0xffffffffu, own, (2 * c4 + e) * 4);
             const int pe = nt * 8 + 2 * c4 + e;
-            qpos[nt][e] = pe < w_nq ? pos0 + (w0 + pe) / GS : -1;
+            qpos[nt][e] = pe < nq ? pos0 + (q0 + pe) / GS : -1;
         }
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks) {
@@ -389,7 +383,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         for (int e = 0; e < 2; ++e) { m[nt][e] = M[nt][e] = LOWEST; l[nt][e] = 0.f; }
     }
 
-    for (; tile < tile_stop; tile += wk) {
+    for (; tile < tile_end; tile += WARPS) {
         const int kt = k_lo + tile * KT;
         ok = mbar_wait(&full[warp], parity, 1);
         if (!ok) break;
@@ -430,7 +424,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
             }
         }
         const bool there = sc >= 0;
-        const bool whole = __all_sync(0xffffffffu, there) && kt + KT - 1 <= w_first && (a.window <= 0 || kt > w_last - a.window);
+        const bool whole = __all_sync(0xffffffffu, there) && kt + KT - 1 <= first_pos && (a.window <= 0 || kt > last_pos - a.window);
         uint32_t seen_rows = 0;
         if (!whole) seen_rows = __ballot_sync(0xffffffffu, there);
 
@@ -549,8 +543,8 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
             }
         }
         __syncwarp();                     // (the tile is read)
-        if (tile + wk < tile_stop) sc = request(tile + wk, page);
-        page = page_of(tile + 2 * wk);
+        if (tile + WARPS < tile_end) sc = request(tile + WARPS, page);
+        page = page_of(tile + 2 * WARPS);
         parity ^= 1;
     }
 
@@ -574,7 +568,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         for (int e = 0; e < 2; ++e) {
             const int i = nt * 8 + 2 * c4 + e;
             float top = LOWEST;
-            for (int w = warp % wq; w < WARPS; w += wq) top = fmaxf(top, sm_m[w][i]);
+            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm_m[w][i]);
             const float f = ex2(M[nt][e] - P_SHIFT - top);
             float* to = sums + (warp * 8 * NT + i) * LD + n8 * (HD / 8);
 #pragma unroll
@@ -591,7 +585,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         if (a.n_splits == 1) {
             to_out(i, d, sum, total);
         } else if (a.cluster) {
-            sums[i * LD + d] = sum;                      // (query i's place of the first group of keys)
+            sums[i * LD + d] = sum;                      // (query i's place of the first warp)
             if (d == 0) { all_top[i] = top; all_total[i] = total; }
         } else if (t0 + tok < a.part_tokens) {
             float* part = a.part + (((int64_t)(t0 + tok) * a.H + h) * a.n_splits + split) * (HD + 2);
@@ -601,12 +595,14 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     };
     bool odd = false;
     for (int idx = tid; idx < nq * HD; idx += THREADS) {
-        const int i = idx / HD, d = idx - i * HD, group = i / (8 * NT), j = i - group * 8 * NT;
+        const int i = idx / HD, d = idx - i * HD;
         float top = LOWEST, total = 0.f, sum = 0.f;
-        for (int w = group; w < WARPS; w += wq) top = fmaxf(top, sm_m[w][j]);
-        for (int w = group; w < WARPS; w += wq) {
-            total += sm_l[w][j] * ex2(sm_m[w][j] - top);
-            sum += sums[(w * 8 * NT + j) * LD + d];
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm_m[w][i]);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            total += sm_l[w][i] * ex2(sm_m[w][i] - top);
+            sum += sums[(w * 8 * NT + i) * LD + d];
         }
         odd |= isnan(sum) || isnan(total);
         leave(i, d, sum, top, total);
@@ -650,14 +646,14 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     }
 }
 
-// Joins the splits: a warp per token and head.  grid (tokens of a row x heads / 4, rows).
+// Joins the splits: a CTA per token and head, whose warps share the splits.  grid (tokens of a row x heads, rows).
 template <typename T>
-__global__ void __launch_bounds__(128) attn_q8_merge_kernel(T* __restrict__ out, const Q8Args a) {
+__global__ void __launch_bounds__(THREADS) attn_q8_merge_kernel(T* __restrict__ out, const Q8Args a) {
+    __shared__ float sums[WARPS][HD], totals[WARPS];
     pdl_wait();
     pdl_trigger();
-    const int r = a.row_list ? a.row_list[blockIdx.y] : blockIdx.y, lane = threadIdx.x & 31;
-    const int at = blockIdx.x * 4 + threadIdx.x / 32, tok = at / a.H, h = at - tok * a.H;
-    const int t0 = a.row_start[r];
+    const int r = a.row_list ? a.row_list[blockIdx.y] : blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tok = blockIdx.x / a.H, h = blockIdx.x - tok * a.H, t0 = a.row_start[r];
     if (tok >= a.row_start[r + 1] - t0 || t0 + tok >= a.part_tokens) return;
     const int64_t ld = HD + 2;
     const float* part = a.part + ((int64_t)(t0 + tok) * a.H + h) * a.n_splits * ld;
@@ -667,7 +663,7 @@ __global__ void __launch_bounds__(128) attn_q8_merge_kernel(T* __restrict__ out,
 #pragma unroll
     for (int c = 0; c < DPL; ++c) sum[c] = 0.f;
 #pragma unroll 4
-    for (int k = 0; k < a.n_splits; ++k) {
+    for (int k = warp; k < a.n_splits; k += WARPS) {
         const float f = ex2(part[k * ld + HD] - top);
         total += part[k * ld + HD + 1] * f;
 #pragma unroll
@@ -676,9 +672,18 @@ __global__ void __launch_bounds__(128) attn_q8_merge_kernel(T* __restrict__ out,
     }
 #pragma unroll
     for (int c = 0; c < DPL; ++c)
-        if (lane + 32 * c < HD)
-            out[(int64_t)(t0 + tok) * a.out_stride + (int64_t)h * HD + lane + 32 * c] =
-                from_float<T>(total == 0.f ? 0.f : sum[c] / total);
+        if (lane + 32 * c < HD) sums[warp][lane + 32 * c] = sum[c];
+    if (lane == 0) totals[warp] = total;
+    __syncthreads();
+    total = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) total += totals[w];
+    for (int d = threadIdx.x; d < HD; d += THREADS) {
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) x += sums[w][d];
+        out[(int64_t)(t0 + tok) * a.out_stride + (int64_t)h * HD + d] = from_float<T>(total == 0.f ? 0.f : x / total);
+    }
 }
 
 // After portions were attended to in 16 bits: where their keys or values hold a NaN (a byte of `odd` is set) every query by
@@ -767,7 +772,7 @@ static int launch(const T* q, T* out, Q8Args a, int64_t n_pages, int n_list, int
     cfg.numAttrs = a.cluster ? 2 : 1;
     e = cudaLaunchKernelEx(&cfg, attn_q8_kernel<T, NT>, q, out, map, (const Q8Args)a);
     if (e != cudaSuccess || a.n_splits == 1 || a.cluster) return (int)e;
-    return (int)sllm_launch_pdl(attn_q8_merge_kernel<T>, dim3(((int64_t)max_new * a.H + 3) / 4, n_list), dim3(128), 0, stream,
+    return (int)sllm_launch_pdl(attn_q8_merge_kernel<T>, dim3((unsigned)(max_new * a.H), n_list), dim3(THREADS), 0, stream,
                                 out, a);
 }
 
@@ -787,14 +792,14 @@ template <typename T, int NT> static int slots() {
 
 using namespace sllm;
 
-// CTAs that the device holds at once, of the form for 8 (nt = 1) or 16 (nt = 2) queries a warp; 0: not known.
+// CTAs that the device holds at once, of the form for 8 (nt = 1) or 16 (nt = 2) queries; 0: not known.
 SLLM_EXPORT int sllm_attn_q8_slots(int dtype, int nt) {
-    if (dtype == 0) return nt == 1 ? slots<float, 1>() : slots<float, 2>();
+    if (dtype == 0) return nt == 1 ? slots<float, 1>() : 0;
     return nt == 1 ? slots<__nv_bfloat16, 1>() : slots<__nv_bfloat16, 2>();
 }
 // keys of a warp's tile
 SLLM_EXPORT int sllm_attn_q8_tile(int dtype, int nt) {
-    if (dtype == 0) return nt == 1 ? Form<float, 1>::KT : Form<float, 2>::KT;
+    if (dtype == 0) return Form<float, 1>::KT;
     return nt == 1 ? Form<__nv_bfloat16, 1>::KT : Form<__nv_bfloat16, 2>::KT;
 }
 
@@ -806,29 +811,27 @@ SLLM_EXPORT int sllm_attn_q8_error() {
     return code;
 }
 
-// nt: queries a warp / 8; wq: groups of queries of a CTA (1, 2 or 4).  cluster: up to 8 splits are merged inside the kernel; else
+// nt: queries of a CTA / 8 (2: bfloat16 only).  cluster: up to 8 splits are merged inside the kernel; else
 // part, float [part_tokens, H, n_splits, HD + 2], takes the splits' sums.
 SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages, int64_t n_pages, const void* scales,
                              const int* table, int table_stride, int page_size, int block, const int* row_start, const int* row_pos0,
                              const int* row_list, int n_list, int max_new, void* out, int64_t out_stride, int H, int G,
-                             float scale, int window, int dtype, int nt, int wq, int n_splits, float* part,
+                             float scale, int window, int dtype, int nt, int n_splits, float* part,
                              int64_t part_tokens, int cluster, cudaStream_t stream) {
     if (n_list <= 0 || max_new <= 0) return 0;
     if (H <= 0 || G <= 0 || H % G || page_size <= 0 || block <= 0 || page_size % block || window < 0 || n_list > 65535 ||
-        (dtype != 0 && dtype != 1) || (nt != 1 && nt != 2) || (wq != 1 && wq != 2 && wq != 4) || n_splits < 1 ||
+        (dtype != 0 && dtype != 1) || (nt != 1 && !(nt == 2 && dtype == 1)) || n_splits < 1 ||
         (cluster ? n_splits > MAX_CLUSTER : n_splits > 1 && part == nullptr) || ((uintptr_t)pages & 15))
         return (int)cudaErrorInvalidValue;
-    const int64_t q_tiles = ((int64_t)max_new * (H / G) + 8 * nt * wq - 1) / (8 * nt * wq);
+    const int64_t q_tiles = ((int64_t)max_new * (H / G) + 8 * nt - 1) / (8 * nt);
     if (q_tiles * n_splits > 65535 || (int64_t)max_new * H > (1u << 30)) return (int)cudaErrorInvalidValue;
     const int es = dtype == 0 ? 4 : 2;
     const int q_vec = (uintptr_t)q % (4 * es) == 0 && q_stride % 4 == 0;
     const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
-                      part, part_tokens, table_stride, page_size, block, H, G, window, n_splits, wq, q_vec, 0, 0, cluster && n_splits > 1, scale * LOG2E,
+                      part, part_tokens, table_stride, page_size, block, H, G, window, n_splits, q_vec, 0, 0, cluster && n_splits > 1, scale * LOG2E,
                       divisor(page_size), divisor(block)};
     typedef __nv_bfloat16 bf16;
-    if (dtype == 0)
-        return nt == 1 ? launch<float, 1>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream)
-                       : launch<float, 2>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
+    if (dtype == 0) return launch<float, 1>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
     return nt == 1 ? launch<bf16, 1>((const bf16*)q, (bf16*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream)
                    : launch<bf16, 2>((const bf16*)q, (bf16*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
 }
@@ -841,7 +844,7 @@ SLLM_EXPORT int sllm_attn_q8_odd(const void* q, int64_t q_stride, const void* pa
     if (n_list <= 0 || n_odd <= 0) return 0;
     if (H <= 0 || G <= 0 || H % G || page_size <= 0 || block <= 0 || page_size % block) return (int)cudaErrorInvalidValue;
     const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
-                      nullptr, 0, table_stride, page_size, block, H, G, window, 1, 1, 0, 0, 0, 0, scale * LOG2E,
+                      nullptr, 0, table_stride, page_size, block, H, G, window, 1, 0, 0, 0, 0, scale * LOG2E,
                       divisor(page_size), divisor(block)};
     return (int)sllm_launch_pdl(attn_q8_odd_kernel<__nv_bfloat16>, dim3(148), dim3(128), 0, stream, (const __nv_bfloat16*)q,
                                 (__nv_bfloat16*)out, odd, n_odd, n_list, a);

@@ -147,8 +147,8 @@ __device__ __forceinline__ int row_of(const WriteArgs& a, int n) { return last_r
 // CTAs 0 .. kv_ctas - 1: a group of a.lanes threads takes one block of the cache (what a row stores in it), for one
 // plane and kv head, twice: for its largest value, then, from L1, to store it: blocks of any size, and room for the warps
 // that its chain of look-ups and two reads wants.  8,192 tokens of 32 + 8 + 8 heads of 128, blocks of 16, with the queries:
-// 53 us (29 at the copy rate); 1,581 tokens of 3 x 40 heads, blocks of 64, in 32 bits with biases: 52 (22).  With the block
-// in registers 49 and 60, eight entries at a time instead of four 52 and 55, several heads a group in a row 42 and 68.
+// 48 us (29 at the copy rate); 1,581 tokens of 3 x 40 heads, blocks of 64, in 32 bits with biases: 40 (22); eight rows of
+// one token 3.0.  With the block in registers 49, 60 and 3.0.
 // Row r has the slots from
 // row_start[r] / block + 2 r on, at least as many as it touches blocks: n new tokens touch at most n / block + 2.  The
 // other CTAs turn the queries.
@@ -223,7 +223,7 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
     const T* src = qkv + ((int64_t)(t0 + first - pos0) * heads + a.H + pg) * a.hd;
     // every unit of the block's new tokens, `lanes` at a time, AT_ONCE of them requested before the first is worked on:
     // use(token, unit, values)
-    constexpr int AT_ONCE = sizeof(T) == 2 ? 4 : 2;
+    constexpr int AT_ONCE = 2;
     const int units = live ? count * upt : 0, d_tok = lanes / upt, d_u = lanes - d_tok * upt;
     auto walk = [&](auto use) {
         int tok = lane / upt, u_ = lane - tok * upt;
@@ -440,10 +440,11 @@ SLLM_EXPORT int sllm_rope_kv_write_q8(const void* qkv, void* q_out, const int* r
     WriteArgs a = {row_start, row_pos0, cos_t, sin_t, bias, (uint8_t*)pages, (uint8_t*)scales, table, table_stride, page_size,
                    block, n_rows, n_tokens, H, G, hd, rot, interleaved, max_new == 1};
     const int upt = hd / (2 * W);
-    // a block's group: a thread for four units of what a row stores in a block, one for each where a warp holds them
+    // a block's group: a thread for sixteen units of what a row stores in a block (for four: 53 and 52 us in the two cases
+    // above), one for each where a warp holds them
     const int64_t units = (int64_t)(max_new < block ? max_new : block) * upt;
     a.lanes = 1;
-    while (a.lanes < WRITE_THREADS && (a.lanes < 32 ? a.lanes < units : 4 * (int64_t)a.lanes < units)) a.lanes *= 2;
+    while (a.lanes < WRITE_THREADS && (a.lanes < 32 ? a.lanes < units : 16 * (int64_t)a.lanes < units)) a.lanes *= 2;
     while (a.lanes > 32 && a.lanes < upt) a.lanes *= 2;      // (upt <= 128: a CTA holds a head)
     const int threads = a.lanes > 32 ? a.lanes : WRITE_THREADS;
     const int64_t slots = a.single ? n_rows : (int64_t)n_tokens / block + 2 * (int64_t)n_rows;

@@ -1078,7 +1078,7 @@ def kv_read_q8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Ten
 
 @functools.lru_cache(maxsize=64)
 def _attention_q8_form(device: int, head_dim: int, code: int, nt: int) -> tuple[int, int]:
-    """(CTAs that the device holds at once, keys of a warp's tile) of the form for ``8 * nt`` queries a warp."""
+    """(CTAs that the device holds at once, keys of a warp's tile) of the form for ``8 * nt`` queries a CTA."""
     lib = _load(*attention_q8_library(head_dim))
     slots = int(lib.sllm_attn_q8_slots(c_int(code), c_int(nt)))
     if slots <= 0:
@@ -1088,27 +1088,50 @@ def _attention_q8_form(device: int, head_dim: int, code: int, nt: int) -> tuple[
 
 @functools.lru_cache(maxsize=4096)
 def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_new: int, max_context: int, n_heads: int,
-                       n_kv_heads: int, window: int) -> tuple[int, int, int, bool]:
-    """How a launch is shared out: (queries a warp / 8, groups of queries of a CTA, CTAs along the keys, whether these
-    are a cluster that merges by itself)."""
+                       n_kv_heads: int, window: int) -> tuple[int, int, bool]:
+    """How a launch is shared out: (queries of a CTA / 8, CTAs along the keys, whether these are a cluster that merges by
+    itself).  Sixteen queries a CTA where that leaves no more places empty and the launch has the work: 16 rows of 32
+    packed queries after 4,000 tokens 76 us against 91, 4 rows of 64 after 500 18.2 against 15.3.  A CTA costs about
+    7 us beside its tiles; a tile of its warps 1.45 us where an SM has one CTA (the chain of one warp's work) and 0.9 us
+    a CTA where it has several; a cluster merges in 2.5 us and a little a split, a kernel of its own takes 4 (rows of
+    1,000 to 32,768 keys of 128, 1 to 64 of them)."""
     packed = max_new * (n_heads // n_kv_heads)
-    nt = 1 if packed <= 8 else 2
-    wq = 1 if packed <= 8 * nt else 2 if packed <= 16 * nt else 4
-    slots, tile = _attention_q8_form(device, head_dim, code, nt)
-    base = n_list * n_kv_heads * -(-packed // (8 * nt * wq))
     keys = min(max_context, window + max_new) if window else max_context
-    turns = max(1, -(-keys // (tile * (4 // wq))))        # tiles of a warp without splits
-    best, best_cost = 1, None
+    eights = -(-packed // 8)
+    nt = 2 if code == 1 and eights >= 4 and eights % 2 == 0 and n_list * n_kv_heads * eights * keys >= 250000 else 1
+    slots, tile = _attention_q8_form(device, head_dim, code, nt)
+    sms = _sm_count(device)
+    base = n_list * n_kv_heads * -(-packed // (8 * nt))
+    turns = max(1, -(-keys // (4 * tile)))                # tiles of a warp without splits
+    best, best_cost, best_cluster = 1, None, False
     for n in range(1, min(64, turns) + 1):
-        cost = -(-base * n // slots) * (-(-turns // n) + 2) + (0.1 * n + 1 if n > 1 else 0)
+        ctas = base * n
+        cluster = 1 < n <= 8 and 8 * ctas <= 7 * slots    # (clusters want room: close to a full device they wait for it)
+        cost = max(1.0, ctas / slots) * (7 + -(-turns // n) * nt * max(1.45, 0.9 * min(ctas, slots) / sms))
+        cost += 0 if n == 1 else 2.5 + 0.1 * n if cluster else 4 + 0.1 * n
         if best_cost is None or cost < best_cost:
-            best, best_cost = n, cost
-    return nt, wq, best, best <= 8 and base * best <= _sm_count(device)
+            best, best_cost, best_cluster = n, cost, cluster
+    return nt, best, best_cluster
 
 
-#: from this many packed queries (new tokens x query heads of a kv head) in a row on, bfloat16 portions are read back into
-#: pages of 16 bits and attended to by the tcgen05 kernel
-Q8_TC_MIN_PACKED_QUERIES = 128
+@functools.lru_cache(maxsize=4096)
+def _attention_q8_in_16_bits(device: int, n_list: int, max_new: int, max_context: int, n_heads: int, n_kv_heads: int,
+                             head_dim: int, page_size: int, window: int) -> bool:
+    """Whether bfloat16 rows are read back into pages of 16 bits and attended to by the tcgen05 kernel.  Both ways' times in us
+    from what 1, 4 and 16 rows of 8 to 256 tokens after 500 to 16,000 took, 32 heads of 64 and 128 on 8 kv heads and 40 of
+    128 on 40: the kernel over 8 bits 8 + 3.2e-5 a key and eight queries of a kv head of 128 (2.4e-5 of 64), the other way 14
+    + 0.0105 a key and round of its CTAs + the copy's bytes.  (One row of 64 tokens after 16,000 152 / 177, of 128 285 / 178; 16
+    rows of 16 after 500 35 / 30.)"""
+    if not attention_tc_supports(n_heads, n_kv_heads, head_dim, page_size, window, biased=bool(window)):
+        return False
+    packed = max_new * (n_heads // n_kv_heads)
+    keys = min(max_context, window + max_new) if window else max_context
+    direct = 8 + n_list * n_kv_heads * -(-packed // 8) * keys * (1.64e-5 + 1.25e-7 * head_dim)
+    rounds = max(1.0, n_list * n_kv_heads * -(-packed // 128) / _sm_count(device))
+    other = 14 + keys * 0.0105 * max(1.0, head_dim / 128) * rounds + n_list * keys * n_kv_heads * head_dim * 1e-6
+    return other < direct
+
+
 #: what the portions' keys and values in 16 bits may take at once; rows beyond it follow in launches of their own
 Q8_WORKSPACE_BYTES = 1 << 30
 
@@ -1175,22 +1198,22 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     if n_list <= 0 or max_new <= 0:
         return out
     stream = _stream_of(device)
-    if code == 1 and max_new * (n_heads // n_kv_heads) >= Q8_TC_MIN_PACKED_QUERIES \
-            and attention_tc_supports(n_heads, n_kv_heads, head_dim, page_size, window, biased=bool(window)) \
+    if code == 1 and max_new > 1 and _attention_q8_in_16_bits(device, n_list, max_new, max_context, n_heads, n_kv_heads,
+                                                              head_dim, page_size, window) \
             and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0:
         _attention_q8_portions(q, pages, scales, block_table, page_size, block, row_start, row_pos0, out, row_list, n_list,
                                max_new, max_context, n_heads, n_kv_heads, head_dim, scale, window, stream)
         return out
-    nt, wq, n_splits, cluster = _attention_q8_plan(device, head_dim, code, n_list, max_new, max_context, n_heads, n_kv_heads,
-                                                   window)
+    nt, n_splits, cluster = _attention_q8_plan(device, head_dim, code, n_list, max_new, max_context, n_heads, n_kv_heads,
+                                               window)
     part = None
     if n_splits > 1 and not cluster:
         part = torch.empty(n * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
-    _check(_q8_function("sllm_attn_q8", head_dim, "plplppiiipppiipliifiiiiiplip")(
+    _check(_q8_function("sllm_attn_q8", head_dim, "plplppiiipppiipliifiiiiplip")(
         q.data_ptr(), q.stride(0), pages.data_ptr(), pages.size(0), scales.data_ptr(), block_table.data_ptr(),
         block_table.stride(0), page_size, block, row_start.data_ptr(), row_pos0.data_ptr(),
         0 if row_list is None else row_list.data_ptr(), n_list, max_new, out.data_ptr(), out.stride(0), n_heads, n_kv_heads,
-        scale, window, code, nt, wq, n_splits, 0 if part is None else part.data_ptr(), n, int(cluster), stream),
+        scale, window, code, nt, n_splits, 0 if part is None else part.data_ptr(), n, int(cluster), stream),
         "attention_q8")
     return out
 

@@ -230,10 +230,11 @@ def tolerance(dtype, hd, want, spread, reach, portion=False):
     return 2.0 ** -23 * want.abs() + (2.0 ** -19 + 2 * moved) * spread
 
 
-def is_portion(c, rows, dtype, H):
+def is_portion(c, rows, dtype, H, window=0, context=None):
     from scratch_llm_b200.kernels import ops
-    return dtype == torch.bfloat16 and max(m for _, m in rows) * (H // c.G) >= ops.Q8_TC_MIN_PACKED_QUERIES and \
-        ops.attention_tc_supports(H, c.G, c.hd, c.page, None)
+    new = max(m for _, m in rows)
+    return dtype == torch.bfloat16 and new > 1 and ops._attention_q8_in_16_bits(
+        torch.cuda.current_device(), len(rows), new, context or max(b + m for b, m in rows), H, c.G, c.hd, c.page, window or 0)
 
 
 def check(c, q, rows, dtype, H, window=0, n=None, **kw):
@@ -243,7 +244,7 @@ def check(c, q, rows, dtype, H, window=0, n=None, **kw):
     want, spread, reach = plain.attend(q, c.pages, c.scales, c.table, rows, c.page, H, c.G, c.hd, scale, window)
     n = want.shape[0]
     far = (got[:n].double().cpu() - want).abs()
-    tol = tolerance(dtype, c.hd, want, spread, reach, is_portion(c, rows, dtype, H))
+    tol = tolerance(dtype, c.hd, want, spread, reach, is_portion(c, rows, dtype, H, window, **kw))
     assert not got[:n].isnan().any()
     assert (far <= tol).all(), f"worst {(far / tol.clamp(min=1e-300)).max():.3g} of the tolerance"
     assert (got[n:] == 7).all()
@@ -262,7 +263,13 @@ ATTEND_ROWS = [
 @pytest.mark.parametrize("H,G,hd,page,block,window", [
     (8, 2, 128, 64, 16, 0), (4, 4, 64, 16, 16, 0), (12, 1, 80, 32, 8, 50), (6, 2, 48, 12, 3, 0), (3, 1, 16, 16, 1, 0),
     (4, 2, 256, 64, 64, 33), (20, 1, 96, 128, 128, 0), (7, 1, 112, 5, 5, 1), (34, 1, 32, 16, 4, 0), (2, 2, 192, 1, 1, 0)])
-def test_attention(rows, dtype, H, G, hd, page, block, window):
+@pytest.mark.parametrize("portions", [False, True])
+def test_attention(rows, dtype, H, G, hd, page, block, window, portions, monkeypatch):
+    from scratch_llm_b200.kernels import ops
+    if portions and (dtype == torch.float32 or not ops.attention_tc_supports(H, G, hd, page, window or None, bool(window))
+                     or max(m for _, m in rows) == 1):
+        pytest.skip("only rows of several tokens and shapes of the tcgen05 kernel are read back")
+    monkeypatch.setattr(ops, "_attention_q8_in_16_bits", lambda *a: portions)
     gen = torch.Generator().manual_seed(hd + len(rows))
     n = sum(m for _, m in rows)
     c = Cache(G, hd, page, block, [b + m for b, m in rows], gen).fill([(b + m, 0) for b, m in rows], gen, 0.5)
@@ -306,8 +313,13 @@ def test_attention_listed_rows_and_strides(dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("H,G,hd,rows", [(8, 2, 128, [(40, 6)]), (4, 1, 64, [(3, 70)]), (2, 2, 48, [(64, 3), (9, 2)]),
                                          (8, 2, 128, [(500, 130)])])
-def test_attention_values_that_are_no_numbers(dtype, H, G, hd, rows):
+@pytest.mark.parametrize("portions", [False, True])
+def test_attention_values_that_are_no_numbers(dtype, H, G, hd, rows, portions, monkeypatch):
     """A NaN among the keys or values of a token reaches the queries that see it and no other."""
+    from scratch_llm_b200.kernels import ops
+    if portions and (dtype == torch.float32 or not ops.attention_tc_supports(H, G, hd, 16, None)):
+        pytest.skip("only shapes of the tcgen05 kernel are read back")
+    monkeypatch.setattr(ops, "_attention_q8_in_16_bits", lambda *a: portions)
     gen = torch.Generator().manual_seed(hd)
     c = Cache(G, hd, 16, 4, [b + m for b, m in rows], gen).fill([(b + m, 0) for b, m in rows], gen, 0.5)
     before, m = rows[0]
@@ -322,7 +334,7 @@ def test_attention_values_that_are_no_numbers(dtype, H, G, hd, rows):
     assert torch.equal(got.isnan(), want.isnan())
     assert want.isnan().any() and not want[:2].isnan().any()
     fine = ~want.isnan()
-    tol = tolerance(dtype, hd, want, spread, reach, is_portion(c, rows, dtype, H))
+    tol = tolerance(dtype, hd, want, spread, reach, portions)
     assert ((got - want).abs() <= tol)[fine].all()
 
 
@@ -340,6 +352,7 @@ def test_attention_portions_in_several_launches(window, monkeypatch):
         for r, (b, _) in enumerate(rows):
             c.table[r, :max(0, b - window + 1) // page] = -1
     monkeypatch.setattr(ops, "Q8_WORKSPACE_BYTES", 2 * 4 * G * 640 * hd)
+    monkeypatch.setattr(ops, "_attention_q8_in_16_bits", lambda *a: True)
     dev, s = c.device(), starts(rows)
     want, spread, reach = plain.attend(q, c.pages, c.scales, c.table, rows, page, H, G, hd, hd ** -0.5, window)
     tol = tolerance(torch.bfloat16, hd, want, spread, reach, True)
