@@ -20,12 +20,17 @@ several), zeroed when a request is admitted, so that a slot that is used again s
 Recurrent mixers keep their state there; the Llama architecture has none.  (A request's position and its sampling seed and counter live
 on the host, with the scheduler, and are sent with every step's descriptor.)
 
+Pages may be held in 8 bits (``dtype=torch.float8_e4m3fn``): every group then has, beside its pages, one power of two
+per block of ``scale_block`` tokens (by default the greatest common divisor of the page and 16), plane and kv
+head.
+
 The manager is host-side bookkeeping plus the device tensors; with ``device=None`` it allocates
 no tensor and can be exercised on a machine without a GPU.
 """
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 from typing import Hashable, Sequence
 
@@ -42,6 +47,7 @@ class Group:
     entries: list[int]
     pool: PagePool
     pages: torch.Tensor | None = None  # [n_entries, n_pages, planes, kv_heads, page_size, head_dim]
+    scales: torch.Tensor | None = None  # of pages in 8 bits: [n_entries, n_pages, 2, kv_heads, blocks]
 
 
 @dataclass
@@ -61,13 +67,21 @@ class CacheManager:
                  state_specs: Sequence[StateSpec | None], page_size: int,
                  n_pages: int, max_requests: int, dtype: torch.dtype = torch.float32,
                  device: torch.device | str | None = None,
-                 poison_free_pages: bool = False) -> None:
+                 poison_free_pages: bool = False, scale_block: int | None = None) -> None:
         if page_size < 1:
             raise ValueError(f"page size must be positive, got {page_size}")
         if max_requests < 1:
             raise ValueError("max_requests must be positive")
         self.page_size, self.max_requests = page_size, max_requests
         self.poison_free_pages = poison_free_pages
+        # pages of e4m3 numbers have one scale (a power of two) per block of tokens, plane and kv head
+        self.scale_block: int | None = None
+        if dtype == torch.float8_e4m3fn:
+            self.scale_block = math.gcd(page_size, 16) if scale_block is None else scale_block
+            if self.scale_block < 1 or page_size % self.scale_block:
+                raise ValueError(f"blocks of {self.scale_block} tokens do not divide a page of {page_size}")
+        elif scale_block is not None:
+            raise ValueError("scale_block belongs to pages of float8_e4m3fn")
         self.dtype, self.device = dtype, (torch.device(device) if device is not None else None)
         self.groups: list[Group] = []
         self.entry_group: list[tuple[int, int] | None] = []  # entry -> (group, index in group)
@@ -92,8 +106,14 @@ class CacheManager:
                 group.pages = torch.empty((len(group.entries), n_pages, s.planes, s.n_kv_heads,
                                            page_size, s.head_dim), dtype=dtype,
                                           device=self.device)
+                if self.scale_block is not None:
+                    if s.planes != 2:
+                        raise ValueError("pages in 8 bits hold keys and values")
+                    group.scales = torch.empty(
+                        (len(group.entries), n_pages, 2, s.n_kv_heads, page_size // self.scale_block),
+                        dtype=torch.float8_e8m0fnu, device=self.device)
                 if poison_free_pages:
-                    group.pages.fill_(float("nan"))
+                    self._poison(group, slice(None))
             def make(st: StateSpec) -> torch.Tensor:
                 return torch.zeros((max_requests, *st.shape), dtype=st.dtype, device=self.device)
 
@@ -202,7 +222,15 @@ class CacheManager:
     def _give_back(self, group: Group, pages: list[int], request_id: Hashable) -> None:
         group.pool.free(pages, request_id)
         if self.poison_free_pages and pages and group.pages is not None:
-            group.pages[:, torch.tensor(pages, device=group.pages.device)] = float("nan")
+            self._poison(group, torch.tensor(pages, device=group.pages.device))
+
+    @staticmethod
+    def _poison(group: Group, pages) -> None:
+        if group.scales is None:
+            group.pages[:, pages] = float("nan")
+        else:       # (a NaN's byte of either type)
+            group.pages.view(torch.uint8)[:, pages] = 0x7F
+            group.scales.view(torch.uint8)[:, pages] = 0xFF
 
     # ---------------------------------------------------------------------------- views
 
@@ -222,6 +250,13 @@ class CacheManager:
         g, i = where
         pages = self.groups[g].pages
         return (pages[i] if pages is not None else None), g
+
+    def entry_scales(self, entry: int) -> torch.Tensor | None:
+        """The scales tensor of this entry, where pages are held in 8 bits."""
+        where = self.entry_group[entry]
+        if where is None or self.groups[where[0]].scales is None:
+            return None
+        return self.groups[where[0]].scales[where[1]]
 
     def max_pages_per_request(self, max_position: int) -> int:
         return -(-max_position // self.page_size)

@@ -5,6 +5,7 @@ the reply.
 
     python -m scratch_llm_b200.chat_cli --model DIR [--data-dir DIR] [--max-tokens 256]
         [--temperature 0.0] [--top-p 1.0] [--seed N] [--dtype bfloat16|float32]
+        [--cache-dtype float8_e4m3fn]
         [--random-weights CONFIG.json]
 
 ``--model`` takes the place of the reference's ``--ckpt`` (a model folder instead of a pickle;
@@ -144,6 +145,8 @@ def main(argv=None) -> int:
     ap.add_argument("--top-p", type=float, default=1.0)
     ap.add_argument("--seed", type=int, default=None)
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--cache-dtype", default=None, choices=["float8_e4m3fn"],
+                    help="hold keys and values in 8 bits (default: in --dtype)")
     ap.add_argument("--random-weights", metavar="CONFIG.json", default=None,
                     help="write --model from this configuration with seeded random weights first")
     args = ap.parse_args(argv)
@@ -160,7 +163,7 @@ def main(argv=None) -> int:
 
     tok_path = Path(args.data_dir or args.model) / "tokenizer.json"
     tokenizer = Tokenizer.load(tok_path) if tok_path.is_file() else None
-    llm = LLM(args.model, dtype=args.dtype, verbose=True)
+    llm = LLM(args.model, dtype=args.dtype, verbose=True, cache_dtype=args.cache_dtype)
     repl(llm, tokenizer, args)
     return 0
 

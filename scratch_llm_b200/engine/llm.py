@@ -75,7 +75,8 @@ class LLM:
     number of requests, not the arithmetic, set its speed: 73.5 against 61.5 us at 2,048 tokens);
     ``max_requests`` the number of requests that can be live at once; ``max_batch_tokens`` the
     token budget of one step; ``chunk_size`` the largest prompt portion per request and step
-    (None: the budget alone cuts prompts).
+    (None: the budget alone cuts prompts).  ``cache_dtype``: None holds keys and values in ``dtype``,
+    "float8_e4m3fn" in 8 bits (:class:`~.runner.ModelRunner`; Llama-style and Vobosun's attention).
 
     ``lookahead``: while a decode step runs, the next one is planned, packed and launched with
     its input tokens still on the device (the sampler's output feeds the embedding directly), and
@@ -86,11 +87,12 @@ class LLM:
     def __init__(self, model: str | Path, dtype: str = "bfloat16", max_tokens: int = 65536,
                  page_size: int = 64, max_requests: int = 64, max_batch_tokens: int = 2048,
                  chunk_size: int | None = None, admission: str = "optimistic",
-                 verbose: bool = False, lookahead: bool = True) -> None:
+                 verbose: bool = False, lookahead: bool = True,
+                 cache_dtype: str | None = None) -> None:
         self.model = load_model(model, dtype, verbose=verbose) if isinstance(model, (str, Path)) \
             else model
         self.runner = ModelRunner(self.model, page_size, max(1, -(-max_tokens // page_size)),
-                                  max_requests)
+                                  max_requests, cache_dtype=cache_dtype)
         self.sampler = Sampler(self.runner.device)
         self.max_batch_tokens, self.chunk_size, self.admission = (max_batch_tokens, chunk_size,
                                                                   admission)

@@ -369,7 +369,8 @@ class DecoderModel:
             state, block_state = self._states_of(cache, run.cache)
             view = CacheView(pages=pages,
                              block_table=batch.block_tables[group] if group is not None else None,
-                             page_size=cache.page_size, state=state, block_state=block_state)
+                             page_size=cache.page_size, state=state, block_state=block_state,
+                             scales=cache.entry_scales(run.cache))
             block = self.blocks[run.layer]
             if i == len(s.order) - 1 and self._final_entry is not None and batch.wants_every_token:
                 pending = block.forward(resid, pending, batch, view, run.write,

@@ -72,17 +72,22 @@ class ModelRunner:
     (portions of prompts, alone or beside decoded tokens) are padded to a few sizes
     (engine/batch.py::pad_plan) and captured per padded shape, if every part of the model
     is ``pad_safe``: launched plainly, such a step costs the host more than the device.
-    ``poison_free_pages``: a debugging aid of the cache manager (free pages hold NaN)."""
+    ``poison_free_pages``: a debugging aid of the cache manager (free pages hold NaN).
+    ``cache_dtype``: None holds keys and values in the compute dtype, "float8_e4m3fn" in 8 bits with a power of two per
+    block of tokens, plane and kv head (half or a quarter of the memory, and of what decode reads of it), if every
+    mixer that caches keys takes such pages."""
 
     def __init__(self, model: DecoderModel, page_size: int, n_pages: int, max_requests: int,
-                 cuda_graphs: bool = True, poison_free_pages: bool = False) -> None:
+                 cuda_graphs: bool = True, poison_free_pages: bool = False,
+                 cache_dtype: str | torch.dtype | None = None) -> None:
         if model.ctx is None:
             raise ValueError("load the model's weights before building a runner")
         self.model = model
         self.device = model.ctx.device
         kv, st = model.cache_specs()
+        dtype = self._cache_dtype(model, cache_dtype)
         self.cache = CacheManager(kv, st, page_size, n_pages, max_requests,
-                                  dtype=model.ctx.dtype, device=self.device,
+                                  dtype=dtype, device=self.device,
                                   poison_free_pages=poison_free_pages)
         self._stager = BatchStager(self.device)
         self.vocab_size = model.spec.vocab_size
@@ -112,6 +117,26 @@ class ModelRunner:
         rows = 2 * max_requests + 16
         self._stager.reserve(3 * (PAD_MAX_TOKENS + 64) + 8 * (rows + 4) + 4 * groups +
                              rows * (self._table_width + 4) * groups)
+
+    @staticmethod
+    def _cache_dtype(model: DecoderModel, wanted: str | torch.dtype | None) -> torch.dtype:
+        if wanted is None:
+            return model.ctx.dtype
+        if wanted not in ("float8_e4m3fn", torch.float8_e4m3fn):
+            raise ValueError(f"cache dtype {wanted!r}: a cache is held in the compute dtype (None) or in "
+                             "float8_e4m3fn")
+        mixers = [m for m in {id(b.cache_owner): b.cache_owner for b in model.blocks}.values()
+                  if m is not None and m.kv_spec() is not None]
+        for mixer in mixers:
+            if not mixer.takes_q8_cache:
+                raise ValueError(f"{type(mixer).__name__} does not take a cache held in 8 bits")
+        jobs = [ops.core_job("sllm_kv_q8")] if mixers else []
+        for hd in sorted({m.kv_spec().head_dim for m in mixers}):
+            jobs.append(ops.attention_q8_library(hd))
+            if model.ctx.dtype == torch.bfloat16 and hd % 64 == 0:
+                jobs.append(ops.attention_tc_library(hd))
+        ops.prepare_jobs(jobs, verbose=False)
+        return torch.float8_e4m3fn
 
     # ----------------------------------------------------------------------- requests
 

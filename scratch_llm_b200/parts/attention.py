@@ -57,6 +57,10 @@ class GQAttention(Mixer):
     pad_safe = True   # padding tokens are not stored, rows without tokens leave the kernels at once
     accepts_sink = True   # forward() takes sink=: the output projection may feed the stream itself
 
+    @property
+    def takes_q8_cache(self) -> bool:
+        return self.head_dim <= ops.Q8_MAX_HEAD_DIM
+
     def accepts_normed(self, n_tokens: int) -> bool:
         return self.qkv is not None and self.qkv.takes_normed(n_tokens)
 
@@ -177,6 +181,9 @@ class GQAttention(Mixer):
         if out is None:
             out = (torch.zeros if batch.padded else torch.empty)(
                 (qkv.shape[0], H * hd), dtype=qkv.dtype, device=qkv.device)
+        if cache.scales is not None:
+            self._attend_q8(qkv, out, batch, cache, (cos, sin, interleaved, write))
+            return out
         if (cos is not None and qkv.dtype == torch.bfloat16 and batch.n_multi == 0
                 and batch.n_single > 0 and H // G <= 16
                 and ops.attention_decode_fused_supported(hd)):
@@ -195,6 +202,30 @@ class GQAttention(Mixer):
                                batch.row_start, batch.row_pos0, out, batch.n_rows,
                                batch.max_row, H, G, hd, self.scale, self.window)
         return out
+
+    def _attend_q8(self, qkv, out, batch, cache: CacheView, rope) -> None:
+        """Over pages held in 8 bits: the rotated queries go to a buffer of their own, keys and values are
+        quantised as they are stored, and rows with one new token and rows with several are attended to in a
+        launch each.  What a captured step plans with has to hold for every step that replays it: the
+        single rows' context bucket, and for the others what their block tables can name."""
+        H, G, hd = self.n_heads, self.n_kv_heads, self.head_dim
+        cos, sin, interleaved, write = rope
+        q = (torch.zeros if batch.padded else torch.empty)(
+            (qkv.shape[0], H * hd), dtype=qkv.dtype, device=qkv.device)
+        ops.rope_kv_write_q8(qkv, batch.row_start, batch.row_pos0, batch.n_rows, batch.max_row, cos, sin, q,
+                             cache.pages, cache.scales, cache.block_table, cache.page_size, H, G, hd,
+                             interleaved, write, self.bias)
+        common = (q, cache.pages, cache.scales, cache.block_table, cache.page_size, batch.row_start,
+                  batch.row_pos0, out)
+        if batch.n_multi:
+            context = cache.block_table.shape[1] * cache.page_size if batch.padded else batch.max_context
+            rows = None if batch.n_multi == batch.n_rows else batch.multi_rows
+            ops.attention_q8(*common, rows, batch.n_multi, batch.max_new_multi, context, H, G, hd, self.scale,
+                             self.window)
+        if batch.n_single:
+            rows = None if batch.n_single == batch.n_rows else batch.single_rows
+            ops.attention_q8(*common, rows, batch.n_single, 1, batch.context_bucket, H, G, hd, self.scale,
+                             self.window)
 
     def _n_splits(self, batch) -> int:
         H, G = self.n_heads, self.n_kv_heads

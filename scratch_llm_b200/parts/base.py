@@ -84,6 +84,8 @@ class CacheView:
     """What one run of a layer sees of the cache in this step."""
 
     pages: torch.Tensor | None = None        # [n_pages, planes, n_kv_heads, page_size, head_dim]
+    # of a cache held in 8 bits (pages are then e4m3): e8m0 [n_pages, 2, n_kv_heads, page_size / block]
+    scales: torch.Tensor | None = None
     block_table: torch.Tensor | None = None  # int32 [rows, max_pages]; -1 where no page is held
     page_size: int = 0
     # [n_slots, *StateSpec.shape], or a tuple of such tensors for a mixer with several states
@@ -133,6 +135,9 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
+    #: True if ``forward`` takes pages held in 8 bits (``CacheView.scales`` is then given)
+    takes_q8_cache = False
+
     def kv_spec(self) -> KVSpec | None:
         return None
 
