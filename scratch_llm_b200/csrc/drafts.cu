@@ -23,8 +23,12 @@
 
 namespace sllm {
 
-constexpr int VERIFY_THREADS = 512, VERIFY_WARPS = VERIFY_THREADS / 32, VERIFY_RANKS = 8;
-constexpr int VERIFY_BATCH = 4;         // strips of 128 entries that a warp requests at a time
+constexpr int VERIFY_RANKS = 8;
+// Launches that leave SMs idle take CTAs of 512 threads, each warp requesting 4 strips of 128 entries at a time: 4 rows of
+// 128,256 entries 9.4 us, 13.4 with 256 threads and 3 strips.  Others take the latter, of which an SM holds four: 64 rows
+// 22.8 us, 48 with the former (the bytes: 10 us).
+template <bool FEW> constexpr int VERIFY_THREADS = FEW ? 512 : 256;
+template <bool FEW> constexpr int VERIFY_BATCH = FEW ? 4 : 3;
 
 __device__ __forceinline__ double weight(float p, float q) {
     const double w = (double)p - (double)q;
@@ -62,10 +66,12 @@ struct Weights {
     }
 };
 
-__global__ void __cluster_dims__(VERIFY_RANKS, 1, 1) __launch_bounds__(VERIFY_THREADS)
+template <bool FEW>
+__global__ void __cluster_dims__(VERIFY_RANKS, 1, 1) __launch_bounds__(VERIFY_THREADS<FEW>, FEW ? 1 : 4)
 verify_drafts_kernel(const float* __restrict__ probs, int64_t p_stride, const float* __restrict__ draft_probs,
                      int64_t q_stride, const int* __restrict__ drafts, const int* __restrict__ start,
                      const float* __restrict__ uniforms, int V, int* __restrict__ tokens, int* __restrict__ accepted) {
+    constexpr int VERIFY_WARPS = VERIFY_THREADS<FEW> / 32, BATCH = VERIFY_BATCH<FEW>;
     __shared__ double warp_sum[VERIFY_WARPS], cta_sum[2];
     __shared__ int n_accepted;
     pdl_wait();
@@ -107,12 +113,12 @@ verify_drafts_kernel(const float* __restrict__ probs, int64_t p_stride, const fl
         if (turn) { w.q = nullptr; w.hot = -1; }
         w.vec = (((uintptr_t)w.p | (uintptr_t)w.q) & 15) == 0;
         double mine = 0.0;
-        for (int j0 = begin; j0 < end; j0 += 128 * VERIFY_BATCH) {
-            float4 a[VERIFY_BATCH], b[VERIFY_BATCH];
+        for (int j0 = begin; j0 < end; j0 += 128 * BATCH) {
+            float4 a[BATCH], b[BATCH];
 #pragma unroll
-            for (int t = 0; t < VERIFY_BATCH; ++t) w.load(j0 + 128 * t + 4 * lane, end, a[t], b[t]);
+            for (int t = 0; t < BATCH; ++t) w.load(j0 + 128 * t + 4 * lane, end, a[t], b[t]);
 #pragma unroll
-            for (int t = 0; t < VERIFY_BATCH; ++t) {
+            for (int t = 0; t < BATCH; ++t) {
                 double x[4];
                 w.of(j0 + 128 * t + 4 * lane, a[t], b[t], x);
                 mine += (x[0] + x[1]) + (x[2] + x[3]);
@@ -131,6 +137,7 @@ verify_drafts_kernel(const float* __restrict__ probs, int64_t p_stride, const fl
         double total = 0.0, before = 0.0, sums[VERIFY_RANKS];
 #pragma unroll
         for (int i = 0; i < VERIFY_RANKS; ++i) sums[i] = cluster.map_shared_rank(cta_sum, i)[turn];
+        cluster.sync();                   // (all have read all sums: who has nothing to look for may leave)
 #pragma unroll
         for (int i = 0; i < VERIFY_RANKS; ++i) total += sums[i];
         found = total > 0.0;
@@ -154,47 +161,50 @@ verify_drafts_kernel(const float* __restrict__ probs, int64_t p_stride, const fl
             upto += warp_sum[i];
         }
         if (own_warp != warp) continue;
-        // and its entry, a strip of 128 at a time
+        // and its entry: strips of 128 are requested as above, and looked into where their sum passes the goal
         int token = -1;
+        bool there = false;
         double past = start_at;
-        for (int j0 = begin; j0 < end; j0 += 128) {
-            const int j = j0 + 4 * lane;
-            float4 a, b;
-            double x[4];
-            w.load(j, end, a, b);
-            w.of(j, a, b, x);
-            double scan = (x[0] + x[1]) + (x[2] + x[3]);
-            const double own = scan;
+        for (int j0 = begin; j0 < end && !there; j0 += 128 * BATCH) {
+            float4 a[BATCH], b[BATCH];
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xffffffffu, scan, o);
-                if (lane >= o) scan += up;
-            }
-            // the lane whose entries pass the goal, and which of them; the last one of any weight stands in
-            double at = past + (scan - own);
-            int pick = -1, last = -1;
+            for (int t = 0; t < BATCH; ++t) w.load(j0 + 128 * t + 4 * lane, end, a[t], b[t]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                at += x[i];
-                if (x[i] > 0.0) last = j + i;
-                if (x[i] > 0.0 && pick < 0 && at > goal) pick = j + i;
+            for (int t = 0; t < BATCH; ++t) {
+                if (there) break;
+                const int j = j0 + 128 * t + 4 * lane;
+                double x[4];
+                w.of(j, a[t], b[t], x);
+                double scan = (x[0] + x[1]) + (x[2] + x[3]);
+                const double own = scan;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double up = __shfl_up_sync(0xffffffffu, scan, o);
+                    if (lane >= o) scan += up;
+                }
+                // the lane whose entries pass the goal, and which of them; the last one of any weight stands in
+                double at = past + (scan - own);
+                int pick = -1, last = -1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    at += x[i];
+                    if (x[i] > 0.0) last = j + i;
+                    if (x[i] > 0.0 && pick < 0 && at > goal) pick = j + i;
+                }
+                const uint32_t hits = __ballot_sync(0xffffffffu, pick >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
+                there = hits != 0u;
+                if (there) token = __shfl_sync(0xffffffffu, pick, __ffs(hits) - 1);
+                else if (any) token = __shfl_sync(0xffffffffu, last, 31 - __clz(any));
+                past += __shfl_sync(0xffffffffu, scan, 31);
             }
-            const uint32_t hits = __ballot_sync(0xffffffffu, pick >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
-            if (hits) {
-                token = __shfl_sync(0xffffffffu, pick, __ffs(hits) - 1);
-                break;
-            }
-            if (any) token = __shfl_sync(0xffffffffu, last, 31 - __clz(any));
-            past += __shfl_sync(0xffffffffu, scan, 31);
         }
         if (lane == 0) tokens[p0 + n] = token;
     }
     if (rank == 0) {
-        for (int i = tid; i <= k; i += VERIFY_THREADS)
+        for (int i = tid; i <= k; i += VERIFY_THREADS<FEW>)
             if (i != n || !found) tokens[p0 + i] = i < n ? drafts[d0 + i] : -1;
         if (tid == 0) accepted[r] = n;
     }
-    cluster.sync();                       // (nobody leaves while others read its sum)
 }
 
 }  // namespace sllm
@@ -206,6 +216,10 @@ SLLM_EXPORT int sllm_verify_drafts(const float* probs, int64_t p_stride, const f
                                    int* tokens, int* accepted, cudaStream_t stream) {
     if (n_rows <= 0) return 0;
     if (V <= 0 || n_rows > 0x7fffffff / VERIFY_RANKS) return (int)cudaErrorInvalidValue;
-    return (int)sllm_launch_pdl(verify_drafts_kernel, dim3(n_rows * VERIFY_RANKS), dim3(VERIFY_THREADS), 0, stream, probs, p_stride,
+    const dim3 grid(n_rows * VERIFY_RANKS);
+    if (n_rows * VERIFY_RANKS <= 148)
+        return (int)sllm_launch_pdl(verify_drafts_kernel<true>, grid, dim3(VERIFY_THREADS<true>), 0, stream, probs, p_stride,
+                                    draft_probs, q_stride, drafts, start, uniforms, V, tokens, accepted);
+    return (int)sllm_launch_pdl(verify_drafts_kernel<false>, grid, dim3(VERIFY_THREADS<false>), 0, stream, probs, p_stride,
                                 draft_probs, q_stride, drafts, start, uniforms, V, tokens, accepted);
 }
