@@ -64,16 +64,17 @@ struct Q8Args {
     const uint8_t* pages; const uint8_t* scales; const int* table;
     const int* row_start; const int* row_pos0; const int* row_list;
     float* part; int64_t part_tokens;                    // [tokens, H, n_splits, HD + 2]: sums, maximum, denominator
-    int table_stride, page_size, block, H, G, window, n_splits, q_vec, run, tiled, cluster;
+    int table_stride, table_width, page_size, block, H, G, window, n_splits, per_split, q_vec, run, tiled, cluster;
     float scale_log2;
     Divisor page_div, block_div;
 };
 
+constexpr int KT = HD <= 128 ? 32 : 16;                  // keys of a tile
 constexpr bool WIDE = HD % 128 == 0;                     // a tile is columns of 128 bytes, each [KT][128]
 constexpr bool CAN_TILE = WIDE || HD == 64;
 constexpr int WIDTH = WIDE ? 128 : HD;
 // where byte b of a key (or value) lies in a tile of KT rows
-template <int KT> __device__ __forceinline__ int place(int row, int b, bool swizzled) {
+__device__ __forceinline__ int place(int row, int b, bool swizzled) {
     if constexpr (WIDE) return (b / 128) * KT * 128 + row * 128 + ((b % 128 / 16 ^ (swizzled ? row & 7 : 0)) << 4) + b % 16;
     else if constexpr (HD == 64) return row * 64 + ((b / 16 ^ (swizzled ? row >> 1 & 3 : 0)) << 4) + b % 16;
     else return row * HD + b;
@@ -81,14 +82,13 @@ template <int KT> __device__ __forceinline__ int place(int row, int b, bool swiz
 
 template <typename T, int NT> struct Form {
     static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;           // halves that an operand of T is split into
-    static constexpr int KT = HD <= 128 && NT * PARTS <= 2 ? 32 : 16;   // keys of a tile
     static constexpr int Q_REGS = NT * PARTS * KSTEPS * 2;
     static constexpr bool Q_SHARED = Q_REGS > 32;
     static constexpr int LD = HD + 4;
     static constexpr int TILE = 2 * KT * HD;                      // bytes of a tile: keys, then values
     static constexpr int TILES = WARPS * TILE;
     static constexpr int MERGE = (int)sizeof(float) * WARPS * 8 * NT * LD;
-    static constexpr int Q_BYTES = Q_SHARED ? (int)sizeof(uint32_t) * WARPS * 32 * Q_REGS : 0;
+    static constexpr int Q_BYTES = Q_SHARED ? (int)sizeof(uint32_t) * 32 * Q_REGS : 0;
     // the tiles (at the end the meeting of the warps takes their place), then the queries
     static constexpr int Q_AT = ((TILES > MERGE ? TILES : MERGE) + 1023) / 1024 * 1024;
     static constexpr size_t smem() { return 1024 + Q_AT + Q_BYTES; }
@@ -197,16 +197,19 @@ __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args
 // The queries of a row and kv head are packed: p = token * GS + j is the row's token `token` and query head g GS + j.  A
 // CTA takes 8 NT packed queries over a share of the keys; its warps take turns at the tiles.  (Warps that share the
 // queries between them, up to four times as many a CTA, fetch and turn every key as often, and were slower nearly
-// everywhere: 32 rows of up to six drafted tokens 72 us with two groups of 16, 58 so, 51 with eight queries a CTA.)  Up to
+// everywhere: 32 rows of up to six drafted tokens 72 us with two groups of 16, 58 so, 51 with eight queries a CTA; 24
+// queries a CTA are a few per cent better for uniform rows with just as many, and 15 to 20 worse for ragged ones.)  Up to
 // eight splits can be a cluster, whose CTAs merge their sums through distributed shared memory (one row of 1,000 keys: 10.3
 // us against 12.4 with a merge kernel); in launches that fill the device clusters find less room than CTAs by themselves (24
-// rows of 4,096 keys of 64, three splits: 47 against 37), and the splits' sums meet in attn_q8_merge_kernel.
+// rows of 4,096 keys of 64, three splits: 47 against 37), and the splits' sums meet in attn_q8_merge_kernel.  A share is
+// as long for all rows as the longest row needs, so that short rows have fewer: 16 rows of up to 16,000 keys and 24
+// packed queries 260 us unsplit, 129 in shares of a sixth.
 // grid (kv heads, splits x tiles of queries, rows), the tiles with the most keys first.
 template <typename T, int NT>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 2)
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3)
 attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_constant__ CUtensorMap map, const Q8Args a) {
     using F = Form<T, NT>;
-    constexpr int PARTS = F::PARTS, KT = F::KT, KG = KT / 16, LD = F::LD;
+    constexpr int PARTS = F::PARTS, KG = KT / 16, LD = F::LD;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* tiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     float* smem = reinterpret_cast<float*>(tiles);
@@ -221,15 +224,28 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     const int r = a.row_list ? a.row_list[blockIdx.z] : blockIdx.z, g = blockIdx.x, GS = a.H / a.G;
     const int split = blockIdx.y % a.n_splits;
     const int q0 = ((int)(gridDim.y / a.n_splits) - 1 - (int)blockIdx.y / a.n_splits) * 8 * NT;
-    const int t0 = a.row_start[r], n_packed = (a.row_start[r + 1] - t0) * GS;
-    if (q0 >= n_packed) return;
-    const int pos0 = a.row_pos0[r], nq = min(n_packed - q0, 8 * NT);
-    const int first_pos = pos0 + q0 / GS, last_pos = pos0 + (q0 + nq - 1) / GS;
     const int* table = a.table + (int64_t)r * a.table_stride;
+    // (asked for at once: the row, and the page of this lane's first key if that lies where the call says)
+    const int t0 = __ldg(a.row_start + r), t1 = __ldg(a.row_start + r + 1), pos0 = __ldg(a.row_pos0 + r);
+    const int guess = __ldg(table + min(a.page_div.quotient((split * a.per_split + warp) * KT + lane % KT), a.table_width - 1));
+    const int n_packed = (t1 - t0) * GS;
+    if (q0 >= n_packed) return;
+    const int nq = min(n_packed - q0, 8 * NT);
+    const int first_pos = pos0 + q0 / GS, last_pos = pos0 + (q0 + nq - 1) / GS;
     const int k_lo = a.window > 0 ? max(0, first_pos - a.window + 1) / KT * KT : 0;
     const int n_tiles = (last_pos - k_lo) / KT + 1;
-    const int per_split = (n_tiles + a.n_splits - 1) / a.n_splits;
+    // shares of one size for all rows: a short row has fewer of them, not smaller ones
+    const int per_split = max(a.per_split, (n_tiles + a.n_splits - 1) / a.n_splits);
     const int tile_begin = min(n_tiles, split * per_split), tile_end = min(n_tiles, tile_begin + per_split);
+
+    if (tile_begin >= tile_end && a.n_splits > 1 && !a.cluster) {      // no share: nothing is read or merged
+        for (int i = tid; i < nq; i += THREADS) {
+            const int p = q0 + i, tok = p / GS, h = g * GS + p - tok * GS;
+            if (t0 + tok < a.part_tokens)
+                a.part[(((int64_t)(t0 + tok) * a.H + h) * a.n_splits + split) * (HD + 2) + HD + 1] = 0.f;
+        }
+        return;
+    }
 
     // ---- tiles: lane i looks up key i (its page, then its two scales); where a page holds whole tiles lane 0 requests
     // them, else lane i the i-th run of `run` keys
@@ -296,22 +312,24 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     const uint8_t* k_at[(HD / 4 + 15) / 16];
     const uint8_t* v_at[2][(HD / 8 + 15) / 16];
 #pragma unroll
-    for (int i = 0; i < (HD / 4 + 15) / 16; ++i) k_at[i] = mine_at + place<KT>(n8, c4 * (HD / 4) + 16 * i, a.tiled);
+    for (int i = 0; i < (HD / 4 + 15) / 16; ++i) k_at[i] = mine_at + place(n8, c4 * (HD / 4) + 16 * i, a.tiled);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int i = 0; i < (HD / 8 + 15) / 16; ++i)
-            v_at[k][i] = mine_at + KT * HD + place<KT>(2 * c4 + k, n8 * (HD / 8) + 16 * i, a.tiled);
+            v_at[k][i] = mine_at + KT * HD + place(2 * c4 + k, n8 * (HD / 8) + 16 * i, a.tiled);
     constexpr int EIGHT = 8 * WIDTH;         // eight rows
 
-    int tile = tile_begin + warp, page = page_of(tile), sc = -1, parity = 0;
+    int tile = tile_begin + warp, sc = -1, parity = 0;
+    int page = a.window > 0 || per_split != a.per_split ? page_of(tile)
+               : tile < tile_end && tile * KT + lane % KT <= last_pos ? guess : -1;
     bool ok = true;
     if (tile < tile_end) sc = request(tile, page);
     page = page_of(tile + WARPS);
 
     // ---- its queries, while the first tile is on its way
     uint32_t qf[F::Q_SHARED ? 1 : PARTS][F::Q_SHARED ? 1 : NT][F::Q_SHARED ? 1 : KSTEPS][2];
-    uint2* q_sh = reinterpret_cast<uint2*>(tiles + F::Q_AT) + warp * (F::Q_REGS / 2) * 32 + lane;   // [part][nt][ks][lane]
+    uint2* q_sh = reinterpret_cast<uint2*>(tiles + F::Q_AT) + lane;   // [part][nt][ks][lane]
     float fq[NT][2];                      // scale * log2 e / the query's power of two, of queries 2 c4 and 2 c4 + 1
     int qpos[NT][2];
 #pragma unroll
@@ -363,14 +381,18 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
                 r1 = halves_rest(y2, y3, h1);
             }
             if constexpr (F::Q_SHARED) {
-                q_sh[(nt * KSTEPS + ks) * 32] = make_uint2(h0, h1);
-                if constexpr (PARTS == 2) q_sh[((NT + nt) * KSTEPS + ks) * 32] = make_uint2(r0, r1);
+                if (nt % WARPS == warp) {
+                    q_sh[(nt * KSTEPS + ks) * 32] = make_uint2(h0, h1);
+                    if constexpr (PARTS == 2) q_sh[((NT + nt) * KSTEPS + ks) * 32] = make_uint2(r0, r1);
+                }
             } else {
                 qf[0][nt][ks][0] = h0; qf[0][nt][ks][1] = h1;
                 if constexpr (PARTS == 2) { qf[1][nt][ks][0] = r0; qf[1][nt][ks][1] = r1; }
             }
         }
     }
+
+    if constexpr (F::Q_SHARED) __syncthreads();
 
     float o[KSTEPS][NT][4], m[NT][2], M[NT][2], l[NT][2];
 #pragma unroll
@@ -658,14 +680,18 @@ __global__ void __launch_bounds__(THREADS) attn_q8_merge_kernel(T* __restrict__ 
     const int64_t ld = HD + 2;
     const float* part = a.part + ((int64_t)(t0 + tok) * a.H + h) * a.n_splits * ld;
     float top = LOWEST, total = 0.f, sum[DPL];
-    for (int k = lane; k < a.n_splits; k += 32) top = fmaxf(top, part[k * ld + HD]);
+    // (a total of zero: a share without a key)
+    for (int k = lane; k < a.n_splits; k += 32)
+        if (part[k * ld + HD + 1] != 0.f) top = fmaxf(top, part[k * ld + HD]);
     top = warp_max(top);
 #pragma unroll
     for (int c = 0; c < DPL; ++c) sum[c] = 0.f;
 #pragma unroll 4
     for (int k = warp; k < a.n_splits; k += WARPS) {
+        const float mine = part[k * ld + HD + 1];
+        if (mine == 0.f) continue;
         const float f = ex2(part[k * ld + HD] - top);
-        total += part[k * ld + HD + 1] * f;
+        total += mine * f;
 #pragma unroll
         for (int c = 0; c < DPL; ++c)
             if (lane + 32 * c < HD) sum[c] += part[k * ld + lane + 32 * c] * f;
@@ -736,7 +762,6 @@ static EncodeFn encode_fn() {
 
 template <typename T, int NT>
 static int launch(const T* q, T* out, Q8Args a, int64_t n_pages, int n_list, int max_new, int q_tiles, cudaStream_t stream) {
-    constexpr int KT = Form<T, NT>::KT;
     const size_t smem = Form<T, NT>::smem();
     // runs of keys that lie in a page and start a tile's share of it
     a.run = KT;
@@ -798,10 +823,7 @@ SLLM_EXPORT int sllm_attn_q8_slots(int dtype, int nt) {
     return nt == 1 ? slots<__nv_bfloat16, 1>() : slots<__nv_bfloat16, 2>();
 }
 // keys of a warp's tile
-SLLM_EXPORT int sllm_attn_q8_tile(int dtype, int nt) {
-    if (dtype == 0) return Form<float, 1>::KT;
-    return nt == 1 ? Form<__nv_bfloat16, 1>::KT : Form<__nv_bfloat16, 2>::KT;
-}
+SLLM_EXPORT int sllm_attn_q8_tile() { return KT; }
 
 // The code of a wait that was given up since the last call, 0 if none was (synchronises the device).
 SLLM_EXPORT int sllm_attn_q8_error() {
@@ -814,21 +836,25 @@ SLLM_EXPORT int sllm_attn_q8_error() {
 // nt: queries of a CTA / 8 (2: bfloat16 only).  cluster: up to 8 splits are merged inside the kernel; else
 // part, float [part_tokens, H, n_splits, HD + 2], takes the splits' sums.
 SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages, int64_t n_pages, const void* scales,
-                             const int* table, int table_stride, int page_size, int block, const int* row_start, const int* row_pos0,
-                             const int* row_list, int n_list, int max_new, void* out, int64_t out_stride, int H, int G,
+                             const int* table, int table_stride, int table_width, int page_size, int block,
+                             const int* row_start, const int* row_pos0, const int* row_list, int n_list, int max_new,
+                             int max_context, void* out, int64_t out_stride, int H, int G,
                              float scale, int window, int dtype, int nt, int n_splits, float* part,
                              int64_t part_tokens, int cluster, cudaStream_t stream) {
     if (n_list <= 0 || max_new <= 0) return 0;
     if (H <= 0 || G <= 0 || H % G || page_size <= 0 || block <= 0 || page_size % block || window < 0 || n_list > 65535 ||
-        (dtype != 0 && dtype != 1) || (nt != 1 && !(nt == 2 && dtype == 1)) || n_splits < 1 ||
+        table_width <= 0 || (dtype != 0 && dtype != 1) || (nt != 1 && !(nt == 2 && dtype == 1)) || n_splits < 1 ||
         (cluster ? n_splits > MAX_CLUSTER : n_splits > 1 && part == nullptr) || ((uintptr_t)pages & 15))
         return (int)cudaErrorInvalidValue;
     const int64_t q_tiles = ((int64_t)max_new * (H / G) + 8 * nt - 1) / (8 * nt);
     if (q_tiles * n_splits > 65535 || (int64_t)max_new * H > (1u << 30)) return (int)cudaErrorInvalidValue;
     const int es = dtype == 0 ? 4 : 2;
+    const int64_t keys = window > 0 && (int64_t)window + max_new < max_context ? (int64_t)window + max_new : max_context;
+    const int64_t share = ((keys + KT - 1) / KT + n_splits - 1) / n_splits;          // a row's at most
     const int q_vec = (uintptr_t)q % (4 * es) == 0 && q_stride % 4 == 0;
     const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
-                      part, part_tokens, table_stride, page_size, block, H, G, window, n_splits, q_vec, 0, 0, cluster && n_splits > 1, scale * LOG2E,
+                      part, part_tokens, table_stride, table_width, page_size, block, H, G, window, n_splits,
+                      (int)(share < 1 ? 1 : share), q_vec, 0, 0, cluster && n_splits > 1, scale * LOG2E,
                       divisor(page_size), divisor(block)};
     typedef __nv_bfloat16 bf16;
     if (dtype == 0) return launch<float, 1>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
@@ -844,7 +870,7 @@ SLLM_EXPORT int sllm_attn_q8_odd(const void* q, int64_t q_stride, const void* pa
     if (n_list <= 0 || n_odd <= 0) return 0;
     if (H <= 0 || G <= 0 || H % G || page_size <= 0 || block <= 0 || page_size % block) return (int)cudaErrorInvalidValue;
     const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
-                      nullptr, 0, table_stride, page_size, block, H, G, window, 1, 0, 0, 0, 0, scale * LOG2E,
+                      nullptr, 0, table_stride, 0, page_size, block, H, G, window, 1, 0, 0, 0, 0, 0, scale * LOG2E,
                       divisor(page_size), divisor(block)};
     return (int)sllm_launch_pdl(attn_q8_odd_kernel<__nv_bfloat16>, dim3(148), dim3(128), 0, stream, (const __nv_bfloat16*)q,
                                 (__nv_bfloat16*)out, odd, n_odd, n_list, a);

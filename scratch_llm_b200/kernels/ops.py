@@ -1078,37 +1078,42 @@ def kv_read_q8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Ten
 
 @functools.lru_cache(maxsize=64)
 def _attention_q8_form(device: int, head_dim: int, code: int, nt: int) -> tuple[int, int]:
-    """(CTAs that the device holds at once, keys of a warp's tile) of the form for ``8 * nt`` queries a CTA."""
+    """(CTAs that the device holds at once of the form for ``8 * nt`` queries a CTA, keys of a warp's tile)."""
     lib = _load(*attention_q8_library(head_dim))
     slots = int(lib.sllm_attn_q8_slots(c_int(code), c_int(nt)))
     if slots <= 0:
         raise KernelError("the occupancy of the 8-bit attention kernel could not be read")
-    return slots, int(lib.sllm_attn_q8_tile(c_int(code), c_int(nt)))
+    return slots, int(lib.sllm_attn_q8_tile())
 
 
 @functools.lru_cache(maxsize=4096)
 def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_new: int, max_context: int, n_heads: int,
                        n_kv_heads: int, window: int) -> tuple[int, int, bool]:
     """How a launch is shared out: (queries of a CTA / 8, CTAs along the keys, whether these are a cluster that merges by
-    itself).  Sixteen queries a CTA where that leaves no more places empty and the launch has the work: 16 rows of 32
-    packed queries after 4,000 tokens 76 us against 91, 4 rows of 64 after 500 18.2 against 15.3.  A CTA costs about
-    7 us beside its tiles; a tile of its warps 1.45 us where an SM has one CTA (the chain of one warp's work) and 0.9 us
-    a CTA where it has several; a cluster merges in 2.5 us and a little a split, a kernel of its own takes 4 (rows of
-    1,000 to 32,768 keys of 128, 1 to 64 of them)."""
+    itself).  Sixteen queries a CTA where that leaves no places empty and there is work to fill the device: 16 ragged rows
+    of 32 packed queries after up to 4,000 tokens 65 us against 74, 4 rows after 300 14.8 against 10.4.  The number of CTAs
+    along the keys is the one with the least cost in turns of a warp (a tile): a CTA costs 1.5 turns beside its
+    own, launches of more CTAs than fit take between the whole and the fractional number of rounds, a cluster merges in
+    1.8 turns and more where the device is nearly full of clusters, a kernel of its own in 4.9.  The
+    numbers are those with which 215 launches (1 to 64 rows of 300 to 16,000 keys, even and ragged, 32 heads of 64 and 128
+    on 8 kv heads and 40 on 40, one to eight tokens) came out 3 % above the best of all choices on average."""
     packed = max_new * (n_heads // n_kv_heads)
     keys = min(max_context, window + max_new) if window else max_context
     eights = -(-packed // 8)
-    nt = 2 if code == 1 and eights >= 4 and eights % 2 == 0 and n_list * n_kv_heads * eights * keys >= 250000 else 1
+    nt = 2 if code == 1 and eights % 2 == 0 and n_list * n_kv_heads * eights * keys >= 400000 else 1
     slots, tile = _attention_q8_form(device, head_dim, code, nt)
-    sms = _sm_count(device)
-    base = n_list * n_kv_heads * -(-packed // (8 * nt))
+    tiles = -(-eights // nt)
+    if tiles > 65535 or n_list > 65535:
+        raise KernelError(f"{n_list} rows of {packed} queries a kv head: at most 65,535 rows and {65535 * 8 * nt} queries")
     turns = max(1, -(-keys // (4 * tile)))                # tiles of a warp without splits
     best, best_cost, best_cluster = 1, None, False
-    for n in range(1, min(64, turns) + 1):
-        ctas = base * n
-        cluster = 1 < n <= 8 and 8 * ctas <= 7 * slots    # (clusters want room: close to a full device they wait for it)
-        cost = max(1.0, ctas / slots) * (7 + -(-turns // n) * nt * max(1.45, 0.9 * min(ctas, slots) / sms))
-        cost += 0 if n == 1 else 2.5 + 0.1 * n if cluster else 4 + 0.1 * n
+    for n in range(1, min(64, turns, 65535 // tiles) + 1):
+        ctas = n_list * n_kv_heads * tiles * n
+        full = ctas / slots
+        cluster = 1 < n <= 8 and full <= 0.9
+        cost = (1.0 if full <= 1 else 0.55 * full + 0.45 * -(-ctas // slots)) * (1.5 + -(-turns // n))
+        if n > 1:
+            cost += 1.8 + 5.6 * max(0.0, full - 0.4) if cluster else 4.9
         if best_cost is None or cost < best_cost:
             best, best_cost, best_cluster = n, cost, cluster
     return nt, best, best_cluster
@@ -1209,11 +1214,11 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     part = None
     if n_splits > 1 and not cluster:
         part = torch.empty(n * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
-    _check(_q8_function("sllm_attn_q8", head_dim, "plplppiiipppiipliifiiiiplip")(
+    _check(_q8_function("sllm_attn_q8", head_dim, "plplppiiiipppiiipliifiiiiplip")(
         q.data_ptr(), q.stride(0), pages.data_ptr(), pages.size(0), scales.data_ptr(), block_table.data_ptr(),
-        block_table.stride(0), page_size, block, row_start.data_ptr(), row_pos0.data_ptr(),
-        0 if row_list is None else row_list.data_ptr(), n_list, max_new, out.data_ptr(), out.stride(0), n_heads, n_kv_heads,
-        scale, window, code, nt, n_splits, 0 if part is None else part.data_ptr(), n, int(cluster), stream),
+        block_table.stride(0), block_table.size(1), page_size, block, row_start.data_ptr(), row_pos0.data_ptr(),
+        0 if row_list is None else row_list.data_ptr(), n_list, max_new, max_context, out.data_ptr(), out.stride(0), n_heads,
+        n_kv_heads, scale, window, code, nt, n_splits, 0 if part is None else part.data_ptr(), n, int(cluster), stream),
         "attention_q8")
     return out
 

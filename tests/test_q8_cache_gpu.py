@@ -288,6 +288,27 @@ def test_attention_long_rows(dtype, H, G, hd, window, rows):
     check(c, q, rows, dtype, H, window, context=4096)       # (a bound above what the rows have)
 
 
+@pytest.mark.parametrize("context", [None, 4096])
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("plan", [(1, 3, False), (1, 8, True), (1, 13, False), (1, 64, False), (2, 5, False), (2, 2, True)])
+def test_attention_shares_of_ragged_rows(plan, window, context, monkeypatch):
+    """However the keys are shared out: rows of fewer keys than shares, of none before their token, and a workspace that
+    holds NaN beforehand."""
+    from scratch_llm_b200.kernels import ops
+    monkeypatch.setattr(ops, "_attention_q8_in_16_bits", lambda *a: False)
+    monkeypatch.setattr(ops, "_attention_q8_plan", lambda *a: plan)
+    H, G, hd = 8, 2, 64
+    rows = [(1100, 4), (0, 1), (30, 2), (257, 4), (0, 0), (127, 1), (640, 3)]
+    gen = torch.Generator().manual_seed(17)
+    c = Cache(G, hd, 16, 16, [b + m for b, m in rows], gen).fill([(b + m, 0) for b, m in rows], gen, 0.5)
+    n = sum(m for _, m in rows)
+    q = (1.5 * torch.randn(n, H * hd, generator=gen)).to(torch.bfloat16)
+    for _ in range(2):
+        gone = torch.full((n * H * plan[1] * (hd + 2),), float("nan"), device=DEV)
+        del gone
+        check(c, q, rows, torch.bfloat16, H, window, context=context)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_attention_listed_rows_and_strides(dtype):
     """Only the listed rows, in any order, the same bits as all of them; queries and outputs as column slices."""
