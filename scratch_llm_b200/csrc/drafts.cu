@@ -15,8 +15,8 @@
 //
 // A row needs its drafts' own entries (one warp, a draft a lane) and then one pass over the distribution that decides: a
 // cluster of eight CTAs per row, every warp with a run of the vocabulary of its own.  Sums of runs go through shared
-// memory, sums of CTAs through distributed shared memory; the warp whose run holds the goal walks it once more (a
-// few KB that the SM has just read).  One CTA per row, every pass by itself, took 155 us for 4 rows of 128,256 entries.
+// memory, sums of CTAs through distributed shared memory; the run that holds the goal is gone through once more by
+// all warps of its CTA (a few KB that the SM has just read), and the share that holds it by one.  One CTA per row, every pass by itself, took 155 us for 4 rows of 128,256 entries.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -24,11 +24,9 @@
 namespace sllm {
 
 constexpr int VERIFY_RANKS = 8;
-// Launches that leave SMs idle take CTAs of 512 threads, each warp requesting 4 strips of 128 entries at a time: 4 rows of
-// 128,256 entries 9.4 us, 13.4 with 256 threads and 3 strips.  Others take the latter, of which an SM holds four: 64 rows
-// 22.8 us, 48 with the former (the bytes: 10 us).
-template <bool FEW> constexpr int VERIFY_THREADS = FEW ? 512 : 256;
-template <bool FEW> constexpr int VERIFY_BATCH = FEW ? 4 : 3;
+// Four CTAs an SM, each warp requesting three strips of 128 entries at a time.  CTAs of 512 threads with four strips took 8.7 us
+// instead of 9.0 for 4 rows of 128,256 entries and four drafts, but 13.1 instead of 10.3 for 16 and 35 instead of 18 for 64.
+constexpr int VERIFY_THREADS = 256, VERIFY_WARPS = VERIFY_THREADS / 32, VERIFY_BATCH = 3;
 
 __device__ __forceinline__ double weight(float p, float q) {
     const double w = (double)p - (double)q;
@@ -66,13 +64,43 @@ struct Weights {
     }
 };
 
-template <bool FEW>
-__global__ void __cluster_dims__(VERIFY_RANKS, 1, 1) __launch_bounds__(VERIFY_THREADS<FEW>, FEW ? 1 : 4)
+// the weights from `begin` to `end`, by a warp
+__device__ __forceinline__ double sum_of(const Weights& w, int begin, int end) {
+    const int lane = threadIdx.x & 31;
+    double sum = 0.0;
+    for (int j0 = begin; j0 < end; j0 += 128 * VERIFY_BATCH) {
+        float4 a[VERIFY_BATCH], b[VERIFY_BATCH];
+#pragma unroll
+        for (int t = 0; t < VERIFY_BATCH; ++t) w.load(j0 + 128 * t + 4 * lane, end, a[t], b[t]);
+#pragma unroll
+        for (int t = 0; t < VERIFY_BATCH; ++t) {
+            double x[4];
+            w.of(j0 + 128 * t + 4 * lane, a[t], b[t], x);
+            sum += (x[0] + x[1]) + (x[2] + x[3]);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+// Of sums of parts in order, of which the first starts at `at`: the first part whose end lies past the goal, or the last one
+// with any weight (-1: none has any).  `at` becomes the start of that part.
+template <int N> __device__ __forceinline__ int part_of(const double* sums, double goal, double& at) {
+    int own = -1;
+    double upto = at, start = at, after = at;
+    for (int i = 0; i < N; ++i) {
+        if ((own < 0 || after <= goal) && sums[i] > 0.0) { own = i; start = upto; after = upto + sums[i]; }
+        upto += sums[i];
+    }
+    at = start;
+    return own;
+}
+
+__global__ void __cluster_dims__(VERIFY_RANKS, 1, 1) __launch_bounds__(VERIFY_THREADS, 4)
 verify_drafts_kernel(const float* __restrict__ probs, int64_t p_stride, const float* __restrict__ draft_probs,
                      int64_t q_stride, const int* __restrict__ drafts, const int* __restrict__ start,
                      const float* __restrict__ uniforms, int V, int* __restrict__ tokens, int* __restrict__ accepted) {
-    constexpr int VERIFY_WARPS = VERIFY_THREADS<FEW> / 32, BATCH = VERIFY_BATCH<FEW>;
-    __shared__ double warp_sum[VERIFY_WARPS], cta_sum[2];
+    __shared__ double warp_sum[VERIFY_WARPS], share_sum[VERIFY_WARPS], cta_sum[2];
     __shared__ int n_accepted;
     pdl_wait();
     pdl_trigger();
@@ -112,20 +140,7 @@ verify_drafts_kernel(const float* __restrict__ probs, int64_t p_stride, const fl
     for (int turn = 0; turn < 2 && !found; ++turn) {          // the weights, or p itself (the same turn in all CTAs)
         if (turn) { w.q = nullptr; w.hot = -1; }
         w.vec = (((uintptr_t)w.p | (uintptr_t)w.q) & 15) == 0;
-        double mine = 0.0;
-        for (int j0 = begin; j0 < end; j0 += 128 * BATCH) {
-            float4 a[BATCH], b[BATCH];
-#pragma unroll
-            for (int t = 0; t < BATCH; ++t) w.load(j0 + 128 * t + 4 * lane, end, a[t], b[t]);
-#pragma unroll
-            for (int t = 0; t < BATCH; ++t) {
-                double x[4];
-                w.of(j0 + 128 * t + 4 * lane, a[t], b[t], x);
-                mine += (x[0] + x[1]) + (x[2] + x[3]);
-            }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        const double mine = sum_of(w, begin, end);
         if (lane == 0) warp_sum[warp] = mine;
         __syncthreads();
         if (tid == 0) {
@@ -134,7 +149,7 @@ verify_drafts_kernel(const float* __restrict__ probs, int64_t p_stride, const fl
             cta_sum[turn] = sum;
         }
         cluster.sync();
-        double total = 0.0, before = 0.0, sums[VERIFY_RANKS];
+        double total = 0.0, sums[VERIFY_RANKS];
 #pragma unroll
         for (int i = 0; i < VERIFY_RANKS; ++i) sums[i] = cluster.map_shared_rank(cta_sum, i)[turn];
         cluster.sync();                   // (all have read all sums: who has nothing to look for may leave)
@@ -142,35 +157,28 @@ verify_drafts_kernel(const float* __restrict__ probs, int64_t p_stride, const fl
         for (int i = 0; i < VERIFY_RANKS; ++i) total += sums[i];
         found = total > 0.0;
         if (!found) continue;
-        // the first CTA whose end lies past the goal, or the last one with any weight
+        // whose CTA, whose warp's run, and, the run shared out in strips of 128, which warp's share of it holds the goal
         const double goal = u * total;
-        int owner = -1;
-        double upto = 0.0, after = 0.0;
-#pragma unroll
-        for (int i = 0; i < VERIFY_RANKS; ++i) {
-            if ((owner < 0 || after <= goal) && sums[i] > 0.0) { owner = i; before = upto; after = upto + sums[i]; }
-            upto += sums[i];
-        }
-        if (owner != rank) continue;
-        // likewise its warp
-        int own_warp = -1;
-        double start_at = 0.0;
-        upto = before;
-        for (int i = 0; i < VERIFY_WARPS; ++i) {
-            if ((own_warp < 0 || after <= goal) && warp_sum[i] > 0.0) { own_warp = i; start_at = upto; after = upto + warp_sum[i]; }
-            upto += warp_sum[i];
-        }
-        if (own_warp != warp) continue;
-        // and its entry: strips of 128 are requested as above, and looked into where their sum passes the goal
+        double past = 0.0;
+        if (part_of<VERIFY_RANKS>(sums, goal, past) != rank) continue;
+        const int own_warp = part_of<VERIFY_WARPS>(warp_sum, goal, past);
+        const int64_t own0 = (int64_t)(rank * VERIFY_WARPS + own_warp) * run;
+        const int own_end = (int)min((int64_t)V, own0 + run), strips = (own_end - (int)own0 + 127) / 128;
+        const int share = (strips + VERIFY_WARPS - 1) / VERIFY_WARPS * 128;
+        const int from = min(own_end, (int)own0 + warp * share), to = min(own_end, from + share);
+        const double shared = sum_of(w, from, to);
+        if (lane == 0) share_sum[warp] = shared;
+        __syncthreads();
+        if (part_of<VERIFY_WARPS>(share_sum, goal, past) != warp) continue;
+        // and its entry
         int token = -1;
         bool there = false;
-        double past = start_at;
-        for (int j0 = begin; j0 < end && !there; j0 += 128 * BATCH) {
-            float4 a[BATCH], b[BATCH];
+        for (int j0 = from; j0 < to && !there; j0 += 128 * VERIFY_BATCH) {
+            float4 a[VERIFY_BATCH], b[VERIFY_BATCH];
 #pragma unroll
-            for (int t = 0; t < BATCH; ++t) w.load(j0 + 128 * t + 4 * lane, end, a[t], b[t]);
+            for (int t = 0; t < VERIFY_BATCH; ++t) w.load(j0 + 128 * t + 4 * lane, to, a[t], b[t]);
 #pragma unroll
-            for (int t = 0; t < BATCH; ++t) {
+            for (int t = 0; t < VERIFY_BATCH; ++t) {
                 if (there) break;
                 const int j = j0 + 128 * t + 4 * lane;
                 double x[4];
@@ -201,7 +209,7 @@ verify_drafts_kernel(const float* __restrict__ probs, int64_t p_stride, const fl
         if (lane == 0) tokens[p0 + n] = token;
     }
     if (rank == 0) {
-        for (int i = tid; i <= k; i += VERIFY_THREADS<FEW>)
+        for (int i = tid; i <= k; i += VERIFY_THREADS)
             if (i != n || !found) tokens[p0 + i] = i < n ? drafts[d0 + i] : -1;
         if (tid == 0) accepted[r] = n;
     }
@@ -215,11 +223,7 @@ SLLM_EXPORT int sllm_verify_drafts(const float* probs, int64_t p_stride, const f
                                    const int* drafts, const int* start, const float* uniforms, int n_rows, int V,
                                    int* tokens, int* accepted, cudaStream_t stream) {
     if (n_rows <= 0) return 0;
-    if (V <= 0 || n_rows > 0x7fffffff / VERIFY_RANKS) return (int)cudaErrorInvalidValue;
-    const dim3 grid(n_rows * VERIFY_RANKS);
-    if (n_rows * VERIFY_RANKS <= 148)
-        return (int)sllm_launch_pdl(verify_drafts_kernel<true>, grid, dim3(VERIFY_THREADS<true>), 0, stream, probs, p_stride,
-                                    draft_probs, q_stride, drafts, start, uniforms, V, tokens, accepted);
-    return (int)sllm_launch_pdl(verify_drafts_kernel<false>, grid, dim3(VERIFY_THREADS<false>), 0, stream, probs, p_stride,
+    if (V <= 0 || V > 1 << 30 || n_rows > 0x7fffffff / VERIFY_RANKS) return (int)cudaErrorInvalidValue;
+    return (int)sllm_launch_pdl(verify_drafts_kernel, dim3(n_rows * VERIFY_RANKS), dim3(VERIFY_THREADS), 0, stream, probs, p_stride,
                                 draft_probs, q_stride, drafts, start, uniforms, V, tokens, accepted);
 }

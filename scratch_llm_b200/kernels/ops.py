@@ -1245,8 +1245,8 @@ def verify_drafts(probs: torch.Tensor, drafts: torch.Tensor, draft_start: torch.
     if not _is_rows(accepted, device, 0):
         _refuse(accepted, "accepted", torch.int32, device, "a vector")
     v = probs.size(-1)
-    if v < 1 or not _is_matrix(probs, torch.float32, device, k + n, v):
-        _refuse(probs, "probs", torch.float32, device, f"[{k + n}, V] with contiguous rows")
+    if not 1 <= v <= 1 << 30 or not _is_matrix(probs, torch.float32, device, k + n, v):
+        _refuse(probs, "probs", torch.float32, device, f"[{k + n}, V] with contiguous rows, V from 1 to 2^30")
     if not (_is_rows(draft_start, device, 0) and draft_start.numel() == n + 1):
         _refuse(draft_start, "draft_start", torch.int32, device, f"{n + 1} entries for {n} rows")
     if not (_is(uniforms, torch.float32, device) and uniforms.numel() == k + n):
