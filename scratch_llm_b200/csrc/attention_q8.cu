@@ -64,7 +64,7 @@ struct Q8Args {
     const uint8_t* pages; const uint8_t* scales; const int* table;
     const int* row_start; const int* row_pos0; const int* row_list;
     float* part; int64_t part_tokens;                    // [tokens, H, n_splits, HD + 2]: sums, maximum, denominator
-    int table_stride, table_width, page_size, block, H, G, window, n_splits, per_split, q_vec, run, tiled, cluster;
+    int table_stride, table_width, page_size, block, H, G, window, n_splits, per_split, one_length, q_vec, run, tiled, cluster;
     float scale_log2;
     Divisor page_div, block_div;
 };
@@ -201,9 +201,9 @@ __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args
 // queries a CTA are a few per cent better for uniform rows with just as many, and 15 to 20 worse for ragged ones.)  Up to
 // eight splits can be a cluster, whose CTAs merge their sums through distributed shared memory (one row of 1,000 keys: 10.3
 // us against 12.4 with a merge kernel); in launches that fill the device clusters find less room than CTAs by themselves (24
-// rows of 4,096 keys of 64, three splits: 47 against 37), and the splits' sums meet in attn_q8_merge_kernel.  A share is
-// as long for all rows as the longest row needs, so that short rows have fewer: 16 rows of up to 16,000 keys and 24
-// packed queries 260 us unsplit, 129 in shares of a sixth.
+// rows of 4,096 keys of 64, three splits: 47 against 37), and the splits' sums meet in attn_q8_merge_kernel.  Where the
+// CTAs do not all fit, a share is as long for all rows as the longest row needs, so that short rows have fewer: 16 rows of up
+// to 16,000 keys and 24 packed queries 260 us unsplit, 129 in shares of a sixth; else each row is cut evenly.
 // grid (kv heads, splits x tiles of queries, rows), the tiles with the most keys first.
 template <typename T, int NT>
 __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3)
@@ -225,17 +225,17 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     const int split = blockIdx.y % a.n_splits;
     const int q0 = ((int)(gridDim.y / a.n_splits) - 1 - (int)blockIdx.y / a.n_splits) * 8 * NT;
     const int* table = a.table + (int64_t)r * a.table_stride;
-    // (asked for at once: the row, and the page of this lane's first key if that lies where the call says)
+    // (asked for at once: the row, and the page of this lane's first key if the row is as long as the call says)
     const int t0 = __ldg(a.row_start + r), t1 = __ldg(a.row_start + r + 1), pos0 = __ldg(a.row_pos0 + r);
-    const int guess = __ldg(table + min(a.page_div.quotient((split * a.per_split + warp) * KT + lane % KT), a.table_width - 1));
+    const int guess_at = min(a.page_div.quotient((split * a.per_split + warp) * KT + lane % KT), a.table_width - 1);
+    const int guess = __ldg(table + guess_at);
     const int n_packed = (t1 - t0) * GS;
     if (q0 >= n_packed) return;
     const int nq = min(n_packed - q0, 8 * NT);
     const int first_pos = pos0 + q0 / GS, last_pos = pos0 + (q0 + nq - 1) / GS;
     const int k_lo = a.window > 0 ? max(0, first_pos - a.window + 1) / KT * KT : 0;
     const int n_tiles = (last_pos - k_lo) / KT + 1;
-    // shares of one size for all rows: a short row has fewer of them, not smaller ones
-    const int per_split = max(a.per_split, (n_tiles + a.n_splits - 1) / a.n_splits);
+    const int per_split = max(a.one_length ? a.per_split : 1, (n_tiles + a.n_splits - 1) / a.n_splits);
     const int tile_begin = min(n_tiles, split * per_split), tile_end = min(n_tiles, tile_begin + per_split);
 
     if (tile_begin >= tile_end && a.n_splits > 1 && !a.cluster) {      // no share: nothing is read or merged
@@ -259,7 +259,9 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     __syncwarp();
     auto page_of = [&](int tile) {
         const int kpos = k_lo + tile * KT + lane % KT;
-        return tile < tile_end && kpos <= last_pos ? __ldg(table + a.page_div.quotient(kpos)) : -1;
+        if (tile >= tile_end || kpos > last_pos) return -1;
+        const int at = a.page_div.quotient(kpos);
+        return at == guess_at ? guess : __ldg(table + at);
     };
     // requests a tile and returns the bytes of this lane's key's two scales; -1: no such key
     auto request = [&](int tile, int page) {
@@ -320,9 +322,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
             v_at[k][i] = mine_at + KT * HD + place(2 * c4 + k, n8 * (HD / 8) + 16 * i, a.tiled);
     constexpr int EIGHT = 8 * WIDTH;         // eight rows
 
-    int tile = tile_begin + warp, sc = -1, parity = 0;
-    int page = a.window > 0 || per_split != a.per_split ? page_of(tile)
-               : tile < tile_end && tile * KT + lane % KT <= last_pos ? guess : -1;
+    int tile = tile_begin + warp, page = page_of(tile), sc = -1, parity = 0;
     bool ok = true;
     if (tile < tile_end) sc = request(tile, page);
     page = page_of(tile + WARPS);
@@ -833,18 +833,18 @@ SLLM_EXPORT int sllm_attn_q8_error() {
     return code;
 }
 
-// nt: queries of a CTA / 8 (2: bfloat16 only).  cluster: up to 8 splits are merged inside the kernel; else
-// part, float [part_tokens, H, n_splits, HD + 2], takes the splits' sums.
+// nt: queries of a CTA / 8 (2: bfloat16 only).  merge 1: up to 8 splits are a cluster; else part, float [part_tokens, H,
+// n_splits, HD + 2], takes the splits' sums, of shares of one length (0) or of rows cut evenly (2).
 SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages, int64_t n_pages, const void* scales,
                              const int* table, int table_stride, int table_width, int page_size, int block,
                              const int* row_start, const int* row_pos0, const int* row_list, int n_list, int max_new,
                              int max_context, void* out, int64_t out_stride, int H, int G,
                              float scale, int window, int dtype, int nt, int n_splits, float* part,
-                             int64_t part_tokens, int cluster, cudaStream_t stream) {
+                             int64_t part_tokens, int merge, cudaStream_t stream) {
     if (n_list <= 0 || max_new <= 0) return 0;
     if (H <= 0 || G <= 0 || H % G || page_size <= 0 || block <= 0 || page_size % block || window < 0 || n_list > 65535 ||
         table_width <= 0 || (dtype != 0 && dtype != 1) || (nt != 1 && !(nt == 2 && dtype == 1)) || n_splits < 1 ||
-        (cluster ? n_splits > MAX_CLUSTER : n_splits > 1 && part == nullptr) || ((uintptr_t)pages & 15))
+        (merge == 1 ? n_splits > MAX_CLUSTER : n_splits > 1 && part == nullptr) || ((uintptr_t)pages & 15))
         return (int)cudaErrorInvalidValue;
     const int64_t q_tiles = ((int64_t)max_new * (H / G) + 8 * nt - 1) / (8 * nt);
     if (q_tiles * n_splits > 65535 || (int64_t)max_new * H > (1u << 30)) return (int)cudaErrorInvalidValue;
@@ -854,7 +854,7 @@ SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages,
     const int q_vec = (uintptr_t)q % (4 * es) == 0 && q_stride % 4 == 0;
     const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
                       part, part_tokens, table_stride, table_width, page_size, block, H, G, window, n_splits,
-                      (int)(share < 1 ? 1 : share), q_vec, 0, 0, cluster && n_splits > 1, scale * LOG2E,
+                      (int)(share < 1 ? 1 : share), merge == 0, q_vec, 0, 0, merge == 1 && n_splits > 1, scale * LOG2E,
                       divisor(page_size), divisor(block)};
     typedef __nv_bfloat16 bf16;
     if (dtype == 0) return launch<float, 1>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
@@ -870,7 +870,7 @@ SLLM_EXPORT int sllm_attn_q8_odd(const void* q, int64_t q_stride, const void* pa
     if (n_list <= 0 || n_odd <= 0) return 0;
     if (H <= 0 || G <= 0 || H % G || page_size <= 0 || block <= 0 || page_size % block) return (int)cudaErrorInvalidValue;
     const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
-                      nullptr, 0, table_stride, 0, page_size, block, H, G, window, 1, 0, 0, 0, 0, 0, scale * LOG2E,
+                      nullptr, 0, table_stride, 0, page_size, block, H, G, window, 1, 0, 0, 0, 0, 0, 0, scale * LOG2E,
                       divisor(page_size), divisor(block)};
     return (int)sllm_launch_pdl(attn_q8_odd_kernel<__nv_bfloat16>, dim3(148), dim3(128), 0, stream, (const __nv_bfloat16*)q,
                                 (__nv_bfloat16*)out, odd, n_odd, n_list, a);

@@ -1088,9 +1088,9 @@ def _attention_q8_form(device: int, head_dim: int, code: int, nt: int) -> tuple[
 
 @functools.lru_cache(maxsize=4096)
 def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_new: int, max_context: int, n_heads: int,
-                       n_kv_heads: int, window: int) -> tuple[int, int, bool]:
-    """How a launch is shared out: (queries of a CTA / 8, CTAs along the keys, whether these are a cluster that merges by
-    itself).  Sixteen queries a CTA where that leaves no places empty and there is work to fill the device: 16 ragged rows
+                       n_kv_heads: int, window: int) -> tuple[int, int, int]:
+    """How a launch is shared out: (queries of a CTA / 8, CTAs along the keys, 1 where these are a cluster that merges by
+    itself, else 2 where all CTAs fit and 0 where they do not).  Sixteen queries a CTA where that leaves no places empty and there is work to fill the device: 16 ragged rows
     of 32 packed queries after up to 4,000 tokens 65 us against 74, 4 rows after 300 14.8 against 10.4.  The number of CTAs
     along the keys is the one with the least cost in turns of a warp (a tile): a CTA costs 1.5 turns beside its
     own, launches of more CTAs than fit take between the whole and the fractional number of rounds, a cluster merges in
@@ -1106,7 +1106,7 @@ def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_n
     if tiles > 65535 or n_list > 65535:
         raise KernelError(f"{n_list} rows of {packed} queries a kv head: at most 65,535 rows and {65535 * 8 * nt} queries")
     turns = max(1, -(-keys // (4 * tile)))                # tiles of a warp without splits
-    best, best_cost, best_cluster = 1, None, False
+    best, best_cost, best_merge = 1, None, 0
     for n in range(1, min(64, turns, 65535 // tiles) + 1):
         ctas = n_list * n_kv_heads * tiles * n
         full = ctas / slots
@@ -1115,8 +1115,8 @@ def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_n
         if n > 1:
             cost += 1.8 + 5.6 * max(0.0, full - 0.4) if cluster else 4.9
         if best_cost is None or cost < best_cost:
-            best, best_cost, best_cluster = n, cost, cluster
-    return nt, best, best_cluster
+            best, best_cost, best_merge = n, cost, 1 if cluster else 0 if full > 1 else 2
+    return nt, best, best_merge
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1209,16 +1209,16 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
         _attention_q8_portions(q, pages, scales, block_table, page_size, block, row_start, row_pos0, out, row_list, n_list,
                                max_new, max_context, n_heads, n_kv_heads, head_dim, scale, window, stream)
         return out
-    nt, n_splits, cluster = _attention_q8_plan(device, head_dim, code, n_list, max_new, max_context, n_heads, n_kv_heads,
-                                               window)
+    nt, n_splits, merge = _attention_q8_plan(device, head_dim, code, n_list, max_new, max_context, n_heads, n_kv_heads,
+                                             window)
     part = None
-    if n_splits > 1 and not cluster:
+    if n_splits > 1 and merge != 1:
         part = torch.empty(n * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
     _check(_q8_function("sllm_attn_q8", head_dim, "plplppiiiipppiiipliifiiiiplip")(
         q.data_ptr(), q.stride(0), pages.data_ptr(), pages.size(0), scales.data_ptr(), block_table.data_ptr(),
         block_table.stride(0), block_table.size(1), page_size, block, row_start.data_ptr(), row_pos0.data_ptr(),
         0 if row_list is None else row_list.data_ptr(), n_list, max_new, max_context, out.data_ptr(), out.stride(0), n_heads,
-        n_kv_heads, scale, window, code, nt, n_splits, 0 if part is None else part.data_ptr(), n, int(cluster), stream),
+        n_kv_heads, scale, window, code, nt, n_splits, 0 if part is None else part.data_ptr(), n, int(merge), stream),
         "attention_q8")
     return out
 

@@ -290,7 +290,7 @@ def test_attention_long_rows(dtype, H, G, hd, window, rows):
 
 @pytest.mark.parametrize("context", [None, 4096])
 @pytest.mark.parametrize("window", [0, 300])
-@pytest.mark.parametrize("plan", [(1, 3, False), (1, 8, True), (1, 13, False), (1, 64, False), (2, 5, False), (2, 2, True)])
+@pytest.mark.parametrize("plan", [(1, 3, 0), (1, 8, 1), (1, 13, 2), (1, 13, 0), (1, 64, 0), (2, 5, 0), (2, 5, 2), (2, 2, 1)])
 def test_attention_shares_of_ragged_rows(plan, window, context, monkeypatch):
     """However the keys are shared out: rows of fewer keys than shares, of none before their token, and a workspace that
     holds NaN beforehand."""
