@@ -1036,7 +1036,8 @@ def rope_kv_write_q8(qkv: torch.Tensor, row_start: torch.Tensor, row_pos0: torch
     q_at, out_at = qkv.data_ptr(), q_out.data_ptr()
     if (q_at | out_at | cos_at | sin_at | bias_at) % 16:
         raise KernelError("qkv, q_out, cos, sin and bias must start on 16-byte boundaries")
-    if q_at == out_at and n > 0:
+    size = qkv.element_size() * n
+    if q_at < out_at + size * n_heads * head_dim and out_at < q_at + size * width:
         raise KernelError("q_out must be memory of its own: qkv stays as it is")
     _check(_q8_function("sllm_rope_kv_write_q8", 0, "ppppiiippiippppiiiiiiiip")(
         q_at, out_at, row_start.data_ptr(), row_pos0.data_ptr(), n_rows, n, max_new, cos_at, sin_at, rot, int(interleaved),
@@ -1202,6 +1203,8 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
         raise KernelError(f"window must not be negative, got {window}")
     if n_list <= 0 or max_new <= 0:
         return out
+    if q.data_ptr() == out.data_ptr():
+        raise KernelError("out must be memory of its own: queries are read while outputs are written")
     stream = _stream_of(device)
     if code == 1 and max_new > 1 and _attention_q8_in_16_bits(device, n_list, max_new, max_context, n_heads, n_kv_heads,
                                                               head_dim, page_size, window) \

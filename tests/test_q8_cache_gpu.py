@@ -504,3 +504,49 @@ def test_write_read_attend_over_a_sequence():
         want, spread, reach = plain.attend(want_q, c.pages, c.scales, c.table, [(at, n)], page, H, G, hd, hd ** -0.5)
         assert ((got - want).abs() <= tolerance(torch.bfloat16, hd, want, spread, reach)).all()
         at += keep
+
+
+@pytest.mark.parametrize("hd,page", [(128, 64), (64, 64), (48, 12)])
+def test_pages_past_32_bits(hd, page, monkeypatch):
+    """Pages that lie more than 2^32 bytes into a cache: written, read and attended to as the first ones are."""
+    from scratch_llm_b200.kernels import ops
+    H, G, tokens = 8, 2, 150
+    n = (1 << 32) // (2 * G * page * hd) + 40
+    pages = torch.empty((n, 2, G, page, hd), dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    scales = torch.empty((n, 2, G, 2), dtype=torch.uint8, device=DEV).view(torch.float8_e8m0fnu)
+    gen = torch.Generator().manual_seed(hd)
+    qkv = torch.randn(tokens, (H + 2 * G) * hd, generator=gen).bfloat16().to(DEV)
+    need = -(-tokens // page)
+    start, pos0, upto = i32([0, tokens]), i32([0]), i32([tokens])
+    back_table = i32([list(range(need))])
+    results = []
+    for first in (0, n - need):
+        table = i32([list(range(first, first + need))])
+        q_out = torch.empty((tokens, H * hd), dtype=torch.bfloat16, device=DEV)
+        ops.rope_kv_write_q8(qkv, start, pos0, 1, tokens, None, None, q_out, pages, scales, table, page, H, G, hd, True)
+        back = torch.zeros((need, 2, G, page, hd), dtype=torch.bfloat16, device=DEV)
+        ops.kv_read_q8(pages, scales, table, page, pos0, upto, back, back_table, 1, tokens)
+        got = [q_out, back]
+        for portions in (False, True):
+            if portions and not ops.attention_tc_supports(H, G, hd, page, None, False):
+                continue
+            monkeypatch.setattr(ops, "_attention_q8_in_16_bits", lambda *a: portions)
+            out = torch.empty_like(q_out)
+            got.append(ops.attention_q8(q_out, pages, scales, table, page, start, pos0, out, None, 1, tokens, tokens, H, G, hd, 0.1))
+        results.append(got)
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and a.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_of_a_row_that_is_listed_twice(dtype):
+    H, G, hd = 8, 2, 64
+    rows = [(700, 1), (900, 3), (20, 2)]
+    gen = torch.Generator().manual_seed(21)
+    c = Cache(G, hd, 16, 16, [b + m for b, m in rows], gen).fill([(b + m, 0) for b, m in rows], gen, 0.5)
+    q = torch.randn(sum(m for _, m in rows), H * hd, generator=gen).to(dtype).to(DEV)
+    dev = c.device()
+    once = attend_on_device(c, q, rows, dev, H, 0.1, row_list=[1, 0], context=1024)
+    twice = attend_on_device(c, q, rows, dev, H, 0.1, row_list=[1, 0, 1, 1], context=1024)
+    torch.testing.assert_close(twice[:4], once[:4], rtol=2.0 ** -7, atol=2.0 ** -9)
+    assert (twice[4:] == 7).all()

@@ -28,7 +28,16 @@ def fake(monkeypatch):
 
     monkeypatch.setattr(ops, "_q8_function", lambda *a: reach)
     monkeypatch.setattr(ops, "_attention_q8_plan", lambda *a: (1, 1, False))
-    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda self: 4096 * (1 + id(self) % 97))
+    seen = []       # (kept alive, so that no address comes twice)
+
+    def data_ptr(self):
+        at = next((i for i, t in enumerate(seen) if t is self), None)
+        if at is None:
+            at = len(seen)
+            seen.append(self)
+        return (1 + at) << 20
+
+    monkeypatch.setattr(torch.Tensor, "data_ptr", data_ptr)
     with FakeTensorMode():
         yield lambda *shape, dtype=F32, device="cuda": torch.empty(shape, dtype=dtype, device=device)
 
@@ -100,6 +109,10 @@ def test_write_refuses_shared_and_unaligned_memory(fake, monkeypatch):
     monkeypatch.setattr(torch.Tensor, "data_ptr", lambda self: 4096)
     with pytest.raises(KernelError, match="memory of its own"):
         ops.rope_kv_write_q8(**write_args(fake))
+    for far in (5 * 8 * 64 * 2 - 16, -(5 * 4 * 64 * 2 - 16)):          # (q_out starts inside qkv, or ends there)
+        monkeypatch.setattr(torch.Tensor, "data_ptr", lambda self: 1 << 20 if self.shape[-1] == 8 * 64 else (1 << 20) + far)
+        with pytest.raises(KernelError, match="memory of its own"):
+            ops.rope_kv_write_q8(**write_args(fake))
     pages = write_args(fake)["pages"]
     monkeypatch.setattr(torch.Tensor, "data_ptr", lambda self: 4096 if self.dtype == E4M3 else 4100 + id(self) % 9 * 16)
     with pytest.raises(KernelError, match="16-byte boundaries"):
@@ -146,6 +159,21 @@ def test_attention_refuses(fake):
         with pytest.raises(KernelError, match=says):
             ops.attention_q8(**{**base, **change})
     assert ops.attention_q8(**{**base, "n_list": 0}) is base["out"]
+    with pytest.raises(KernelError, match="memory of its own"):
+        ops.attention_q8(**{**base, "out": base["q"]})
+
+
+def test_attention_says_what_a_launch_holds(monkeypatch):
+    monkeypatch.setattr(ops, "_attention_q8_form", lambda *a: (592, 32))
+    plan = ops._attention_q8_plan.__wrapped__
+    for rows, new in ((65536, 1), (1, 200000)):
+        with pytest.raises(KernelError, match="at most 65,535 rows"):
+            plan(0, 64, 0, rows, new, 300000, 32, 8, 0)
+    for args in ((0, 64, 0, 1, 1, 1, 8, 8, 0), (0, 128, 1, 65535, 1, 1, 8, 8, 0), (0, 64, 0, 1, 100000, 200000, 32, 8, 100),
+                 (0, 128, 1, 3, 4, 1 << 20, 32, 8, 0)):
+        nt, n, merge = plan(*args)
+        packed = args[4] * (args[6] // args[7])
+        assert nt in (1, 2) and 1 <= n <= 64 and merge in (0, 1, 2) and (merge != 1 or n <= 8) and -(-packed // (8 * nt)) * n <= 65535
 
 
 def test_verify_refuses(fake):
