@@ -926,7 +926,7 @@ def _stream_of(device: int) -> int:
 
 
 # The operators below are called for every layer of every step: what a call checks is one expression per tensor, and only
-# a tensor that fails it is asked what is wrong (_refuse).
+# a tensor that fails it is asked what is wrong (_refuse).  (shape and stride() as a whole: size(i) costs as much as both.)
 
 def _is(t: torch.Tensor, dtype: torch.dtype, device: int) -> bool:
     return t.dtype is dtype and t.get_device() == device and t.is_contiguous()
@@ -936,14 +936,19 @@ def _is_rows(t: torch.Tensor, device: int, n: int) -> bool:
     return t.dtype is torch.int32 and t.get_device() == device and t.is_contiguous() and t.dim() == 1 and t.numel() >= n
 
 
+def _is_shaped(t: torch.Tensor, dtype: torch.dtype, device: int, shape: tuple) -> bool:
+    return t.dtype is dtype and t.get_device() == device and t.is_contiguous() and t.shape == shape
+
+
 def _is_table(t: torch.Tensor, device: int, n_rows: int) -> bool:
-    return t.dtype is torch.int32 and t.get_device() == device and t.dim() == 2 and t.size(0) >= n_rows \
-        and (t.size(1) <= 1 or t.stride(1) == 1)
+    shape = t.shape
+    return t.dtype is torch.int32 and t.get_device() == device and len(shape) == 2 and shape[0] >= n_rows \
+        and (shape[1] <= 1 or t.stride()[1] == 1)
 
 
 def _is_matrix(t: torch.Tensor, dtype: torch.dtype, device: int, rows: int, columns: int) -> bool:
-    return t.dtype is dtype and t.get_device() == device and t.dim() == 2 and t.size(0) == rows and t.size(1) == columns \
-        and (columns <= 1 or t.stride(1) == 1)
+    return t.dtype is dtype and t.get_device() == device and t.shape == (rows, columns) \
+        and (columns <= 1 or t.stride()[1] == 1)
 
 
 def _refuse(t: torch.Tensor, name: str, dtype: torch.dtype | None, device: int, wanted: str) -> None:
@@ -973,12 +978,11 @@ def _q8_cache(pages: torch.Tensor, scales: torch.Tensor, n_kv_heads: int, page_s
               device: int) -> int:
     """Checks a cache in 8 bits and returns the tokens of its blocks."""
     shape = pages.shape
-    if not (_is(pages, Q8_DTYPE, device) and len(shape) == 5 and shape[1] == 2 and shape[2] == n_kv_heads
-            and shape[3] == page_size and shape[4] == head_dim):
+    if not (_is(pages, Q8_DTYPE, device) and len(shape) == 5 and shape[1:] == (2, n_kv_heads, page_size, head_dim)):
         _refuse(pages, "pages", Q8_DTYPE, device, f"contiguous [n_pages, 2, {n_kv_heads}, {page_size}, {head_dim}]")
     if not _is(scales, Q8_SCALE_DTYPE, device):
         _refuse(scales, "scales", Q8_SCALE_DTYPE, device, "contiguous [n_pages, 2, kv heads, blocks of a page]")
-    block = _q8_block(shape[0], n_kv_heads, page_size, head_dim, tuple(scales.shape))
+    block = _q8_block(shape[0], n_kv_heads, page_size, head_dim, scales.shape)
     if pages.data_ptr() % 16:
         raise KernelError("pages must start on a 16-byte boundary")
     return block
@@ -1010,10 +1014,11 @@ def rope_kv_write_q8(qkv: torch.Tensor, row_start: torch.Tensor, row_pos0: torch
     device, dtype = _device(), qkv.dtype
     code = _code(dtype)
     block = _q8_cache(pages, scales, n_kv_heads, page_size, head_dim, device)
-    n, width = qkv.size(0), (n_heads + 2 * n_kv_heads) * head_dim
-    if not (_is(qkv, dtype, device) and qkv.dim() == 2 and qkv.size(1) == width):
+    shape, width = qkv.shape, (n_heads + 2 * n_kv_heads) * head_dim
+    n = shape[0] if shape else 0
+    if not (_is(qkv, dtype, device) and shape == (n, width)):
         _refuse(qkv, "qkv", None, device, f"contiguous [tokens, {width}]")
-    if not (_is(q_out, dtype, device) and q_out.dim() == 2 and q_out.size(0) == n and q_out.size(1) == n_heads * head_dim):
+    if not _is_shaped(q_out, dtype, device, (n, n_heads * head_dim)):
         _refuse(q_out, "q_out", dtype, device, f"contiguous [{n}, {n_heads * head_dim}]")
     if not _is_rows(row_start, device, n_rows + 1):
         _refuse(row_start, "row_start", torch.int32, device, f"{n_rows + 1} entries")
@@ -1023,10 +1028,11 @@ def rope_kv_write_q8(qkv: torch.Tensor, row_start: torch.Tensor, row_pos0: torch
         _refuse(block_table, "block_table", torch.int32, device, f"{n_rows} contiguous rows")
     rot, cos_at, sin_at, bias_at = 0, 0, 0, 0
     if cos is not None:
-        rot = 2 * cos.size(-1)
-        if not (_is(cos, torch.float32, device) and cos.dim() == 2 and 2 <= rot <= head_dim):
+        shape = cos.shape
+        rot = 2 * shape[-1] if shape else 0
+        if not (_is(cos, torch.float32, device) and len(shape) == 2 and 2 <= rot <= head_dim):
             _refuse(cos, "cos", torch.float32, device, f"contiguous [positions, 1 to {head_dim // 2}]")
-        if sin is None or not (_is(sin, torch.float32, device) and sin.shape == cos.shape):
+        if sin is None or not _is_shaped(sin, torch.float32, device, shape):
             _refuse(cos if sin is None else sin, "sin", torch.float32, device, "a table like cos")
         cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
     if bias is not None:
@@ -1041,7 +1047,7 @@ def rope_kv_write_q8(qkv: torch.Tensor, row_start: torch.Tensor, row_pos0: torch
         raise KernelError("q_out must be memory of its own: qkv stays as it is")
     _check(_q8_function("sllm_rope_kv_write_q8", 0, "ppppiiippiippppiiiiiiiip")(
         q_at, out_at, row_start.data_ptr(), row_pos0.data_ptr(), n_rows, n, max_new, cos_at, sin_at, rot, int(interleaved),
-        bias_at, pages.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), page_size, block,
+        bias_at, pages.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride()[0], page_size, block,
         n_heads, n_kv_heads, head_dim, int(write), code, _stream_of(device)), "rope_kv_write_q8")
 
 
@@ -1071,8 +1077,8 @@ def kv_read_q8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Ten
     if at % 16:
         raise KernelError("out must start on a 16-byte boundary")
     _check(_q8_function("sllm_kv_read_q8", 0, "pppippppiiiiiiiip")(
-        pages.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), row_from.data_ptr(),
-        row_to.data_ptr(), at, out_table.data_ptr(), out_table.stride(0), n_rows, max_tokens, page_size, block, g, hd, code,
+        pages.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride()[0], row_from.data_ptr(),
+        row_to.data_ptr(), at, out_table.data_ptr(), out_table.stride()[0], n_rows, max_tokens, page_size, block, g, hd, code,
         _stream_of(device)), "kv_read_q8")
     return out
 
@@ -1180,8 +1186,8 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     bits (:func:`rope_kv_write_q8`), for single tokens, drafted tokens and portions of prompts alike.  ``q`` [N, H * hd] may be
     a column slice; bfloat16 or float32, and ``out`` likewise.  No row brings more than ``max_new`` tokens, and no query
     stands at a position of ``max_context`` or more."""
-    device, dtype, n, width = _device(), q.dtype, q.size(0), n_heads * head_dim
-    code = _code(dtype)
+    device, dtype, shape, width = _device(), q.dtype, q.shape, n_heads * head_dim
+    code, n = _code(dtype), shape[0] if shape else 0
     block = _q8_cache(pages, scales, n_kv_heads, page_size, head_dim, device)
     if not _is_matrix(q, dtype, device, n, width):
         _refuse(q, "q", None, device, f"[tokens, {width}] with contiguous rows")
@@ -1203,12 +1209,13 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
         raise KernelError(f"window must not be negative, got {window}")
     if n_list <= 0 or max_new <= 0:
         return out
-    if q.data_ptr() == out.data_ptr():
+    q_at, out_at, q_stride, out_stride = q.data_ptr(), out.data_ptr(), q.stride()[0], out.stride()[0]
+    if q_at == out_at:
         raise KernelError("out must be memory of its own: queries are read while outputs are written")
     stream = _stream_of(device)
     if code == 1 and max_new > 1 and _attention_q8_in_16_bits(device, n_list, max_new, max_context, n_heads, n_kv_heads,
                                                               head_dim, page_size, window) \
-            and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0:
+            and (q_stride | out_stride) % 8 == 0 and (q_at | out_at) % 16 == 0:
         _attention_q8_portions(q, pages, scales, block_table, page_size, block, row_start, row_pos0, out, row_list, n_list,
                                max_new, max_context, n_heads, n_kv_heads, head_dim, scale, window, stream)
         return out
@@ -1218,9 +1225,9 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     if n_splits > 1 and merge != 1:
         part = torch.empty(n * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
     _check(_q8_function("sllm_attn_q8", head_dim, "plplppiiiipppiiipliifiiiiplip")(
-        q.data_ptr(), q.stride(0), pages.data_ptr(), pages.size(0), scales.data_ptr(), block_table.data_ptr(),
-        block_table.stride(0), block_table.size(1), page_size, block, row_start.data_ptr(), row_pos0.data_ptr(),
-        0 if row_list is None else row_list.data_ptr(), n_list, max_new, max_context, out.data_ptr(), out.stride(0), n_heads,
+        q_at, q_stride, pages.data_ptr(), pages.shape[0], scales.data_ptr(), block_table.data_ptr(),
+        block_table.stride()[0], block_table.shape[1], page_size, block, row_start.data_ptr(), row_pos0.data_ptr(),
+        0 if row_list is None else row_list.data_ptr(), n_list, max_new, max_context, out_at, out_stride, n_heads,
         n_kv_heads, scale, window, code, nt, n_splits, 0 if part is None else part.data_ptr(), n, int(merge), stream),
         "attention_q8")
     return out
@@ -1247,7 +1254,8 @@ def verify_drafts(probs: torch.Tensor, drafts: torch.Tensor, draft_start: torch.
         _refuse(drafts, "drafts", torch.int32, device, "a vector")
     if not _is_rows(accepted, device, 0):
         _refuse(accepted, "accepted", torch.int32, device, "a vector")
-    v = probs.size(-1)
+    shape = probs.shape
+    v = shape[-1] if shape else 0
     if not 1 <= v <= 1 << 30 or not _is_matrix(probs, torch.float32, device, k + n, v):
         _refuse(probs, "probs", torch.float32, device, f"[{k + n}, V] with contiguous rows, V from 1 to 2^30")
     if not (_is_rows(draft_start, device, 0) and draft_start.numel() == n + 1):
@@ -1263,8 +1271,8 @@ def verify_drafts(probs: torch.Tensor, drafts: torch.Tensor, draft_start: torch.
     if n == 0:
         return
     _check(_q8_function("sllm_verify_drafts", 0, "plplpppiippp")(
-        probs.data_ptr(), probs.stride(0), 0 if draft_probs is None else draft_probs.data_ptr(),
-        0 if draft_probs is None else draft_probs.stride(0), drafts.data_ptr(), draft_start.data_ptr(), uniforms.data_ptr(), n,
+        probs.data_ptr(), probs.stride()[0], 0 if draft_probs is None else draft_probs.data_ptr(),
+        0 if draft_probs is None else draft_probs.stride()[0], drafts.data_ptr(), draft_start.data_ptr(), uniforms.data_ptr(), n,
         v, tokens.data_ptr(), accepted.data_ptr(), _stream_of(device)), "verify_drafts")
 
 
