@@ -20,7 +20,7 @@
 // by movmatrix.  Every warp fetches tiles of its own into shared memory by TMA (one request per plane and tile where a
 // page holds whole tiles, else one per run of keys), so that no warp waits for another before the end.  One tile a warp
 // is on its way or worked on, four warps a scheduler cover the wait: 64 rows of 4,096 keys, 32 heads of 128 on 8 kv heads,
-// take 99 us (5.4 TB/s); two tiles in turn for three warps a scheduler took 121 us, the keys of the next tile requested as
+// take 97 us (5.5 TB/s); two tiles in turn for three warps a scheduler took 121 us, the keys of the next tile requested as
 // soon as this one's are read 111, loads straight into registers 210: what counts is instructions and the warps that are
 // there to issue them.  128-byte (heads of 64: 64-byte) swizzle: no two lanes of a read meet in a bank.  Other
 // heads, and pages of no whole eights of tokens, come by untiled bulk copies, as they lie.
@@ -259,9 +259,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     __syncwarp();
     auto page_of = [&](int tile) {
         const int kpos = k_lo + tile * KT + lane % KT;
-        if (tile >= tile_end || kpos > last_pos) return -1;
-        const int at = a.page_div.quotient(kpos);
-        return at == guess_at ? guess : __ldg(table + at);
+        return tile < tile_end && kpos <= last_pos ? __ldg(table + a.page_div.quotient(kpos)) : -1;
     };
     // requests a tile and returns the bytes of this lane's key's two scales; -1: no such key
     auto request = [&](int tile, int page) {
@@ -322,7 +320,9 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
             v_at[k][i] = mine_at + KT * HD + place(2 * c4 + k, n8 * (HD / 8) + 16 * i, a.tiled);
     constexpr int EIGHT = 8 * WIDTH;         // eight rows
 
-    int tile = tile_begin + warp, page = page_of(tile), sc = -1, parity = 0;
+    int tile = tile_begin + warp, page = guess, sc = -1, parity = 0;
+    const int first_key = k_lo + tile * KT + lane % KT;
+    if (tile >= tile_end || first_key > last_pos || a.page_div.quotient(first_key) != guess_at) page = page_of(tile);
     bool ok = true;
     if (tile < tile_end) sc = request(tile, page);
     page = page_of(tile + WARPS);
@@ -451,15 +451,15 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         if (!whole) seen_rows = __ballot_sync(0xffffffffu, there);
 
         // ---- scaled scores, their maxima
+        const float own_k = __int_as_float((sc & 0xff) << 23), own_v = (float)(sc >> 8 & 0xff) - 127.f;
         float ev[KG][2];                  // the values' exponents of this lane's keys
 #pragma unroll
         for (int i = 0; i < KG; ++i)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int key = 16 * i + 8 * k + n8;
-                const int both = __shfl_sync(0xffffffffu, sc, key);
-                const float fk = __int_as_float((both & 0xff) << 23);
-                ev[i][k] = (float)(both >> 8 & 0xff) - 127.f;
+                const float fk = __shfl_sync(0xffffffffu, own_k, key);
+                ev[i][k] = __shfl_sync(0xffffffffu, own_v, key);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
