@@ -48,17 +48,6 @@ constexpr float STALE = 8.f;                             // how far a maximum ma
 constexpr int MAX_CLUSTER = 8;                           // CTAs of a cluster, on every device of the kind
 constexpr float P_SHIFT = 6.f;                           // probabilities become halves times 2^6: 2^14 at most
 
-// n / d for 0 <= n < 2^31: 2 n * ceil(2^(31 + s) / d) / 2^(32 + s), 2^s >= d
-struct Divisor {
-    uint32_t magic; int shift, d;
-    __device__ __forceinline__ int quotient(int n) const { return (int)(__umulhi(2u * (uint32_t)n, magic) >> shift); }
-};
-static Divisor divisor(int d) {
-    int s = 0;
-    while ((1ll << s) < d) ++s;
-    return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s, d};
-}
-
 struct Q8Args {
     int64_t q_stride, out_stride;
     const uint8_t* pages; const uint8_t* scales; const int* table;

@@ -22,8 +22,10 @@ struct WriteArgs {
     uint8_t* pages; uint8_t* scales; const int* table;
     int table_stride, page_size, block, n_rows, n_tokens, H, G, hd, rot, interleaved, single;
     int lanes;              // threads of a block of the cache: a power of two up to 32, or whole warps
-    int kv_ctas, q_groups;
-    int64_t n_tasks, n_q_items;
+    int kv_ctas, q_groups, q_per_group, q_at_once, lane_tokens, page_blocks;
+    Divisor by_lanes, by_upt, by_planes, by_g, by_block, by_page, by_q_groups;     // (a division costs twenty instructions)
+    int n_tasks;
+    int64_t n_q_items;
 };
 
 constexpr int WRITE_THREADS = 256;
@@ -162,12 +164,12 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
     if ((int)blockIdx.x >= a.kv_ctas) {
         // ---- queries: a thread takes a unit of a token and walks a share of the token's heads with it (an item: a token's
         // share of heads)
-        const int per_group = (a.H + a.q_groups - 1) / a.q_groups;
-        const int at_once = blockDim.x / upt, u_ = threadIdx.x % upt;
-        if ((int)threadIdx.x >= at_once * upt) return;
-        for (int64_t i = (int64_t)(blockIdx.x - a.kv_ctas) * at_once + threadIdx.x / upt; i < a.n_q_items;
+        const int per_group = a.q_per_group, at_once = a.q_at_once;
+        const int mine = a.by_upt.quotient(threadIdx.x), u_ = threadIdx.x - mine * upt;
+        if (mine >= at_once) return;
+        for (int64_t i = (int64_t)(blockIdx.x - a.kv_ctas) * at_once + mine; i < a.n_q_items;
              i += (int64_t)(gridDim.x - a.kv_ctas) * at_once) {
-            const int n = (int)((uint32_t)i / (uint32_t)a.q_groups), group = (int)((uint32_t)i - (uint32_t)n * a.q_groups);
+            const int n = a.by_q_groups.quotient((int)i), group = (int)i - n * a.q_groups;
             if (n >= a.row_start[a.n_rows]) continue;
             const int r = row_of(a, n), pos = a.row_pos0[r] + n - a.row_start[r];
             const Unit<W> u(u_, a.rot, a.interleaved);
@@ -194,39 +196,39 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
         return;
     }
     // ---- keys and values
-    const int lanes = a.lanes, in_cta = blockDim.x / lanes;
-    const int64_t task = (int64_t)blockIdx.x * in_cta + threadIdx.x / lanes;
-    const int lane = threadIdx.x % lanes;
-    const int slot = (int)(task / (2 * a.G)), pg = (int)(task - (int64_t)slot * 2 * a.G), plane = pg / a.G, g = pg - plane * a.G;
-    bool live = task < a.n_tasks;
+    const int lanes = a.lanes, in_cta = a.by_lanes.quotient(blockDim.x), group = a.by_lanes.quotient(threadIdx.x);
+    const int64_t at_task = (int64_t)blockIdx.x * in_cta + group;
+    bool live = at_task < a.n_tasks;
+    const int task = live ? (int)at_task : 0, lane = threadIdx.x - group * lanes;
+    const int slot = a.by_planes.quotient(task), pg = task - slot * 2 * a.G, plane = a.by_g.quotient(pg), g = pg - plane * a.G;
     int r = slot, at = 0;
     if (live && !a.single) {
         // row_start[r] / block + 2 r <= slot
         r = last_row(a, ((int64_t)slot + 1) * a.block, 2 * a.block);
-        at = slot - (a.row_start[r] / a.block + 2 * r);
+        at = slot - (a.by_block.quotient(a.row_start[r]) + 2 * r);
     }
     int t0 = 0, pos0 = 0, n_old = 0, first = 0, count = 0;
     if (live) {
         t0 = a.row_start[r];
         const int n_new = a.row_start[r + 1] - t0;
         pos0 = a.row_pos0[r];
-        const int begin = (pos0 / a.block + at) * a.block;       // the block's first position
+        const int begin = (a.by_block.quotient(pos0) + at) * a.block;       // the block's first position
         first = max(pos0, begin);
         count = min(pos0 + n_new, begin + a.block) - first;
         n_old = first - begin;
         live = count > 0;
     }
     // (the page is looked up while the values are on their way)
-    const int begin = first - n_old, cell = begin % a.page_size;
-    const int page = live ? a.table[(int64_t)r * a.table_stride + begin / a.page_size] : -1;
+    const int begin = first - n_old, at_page = a.by_page.quotient(begin), cell = begin - at_page * a.page_size;
+    const int page = live ? a.table[(int64_t)r * a.table_stride + at_page] : -1;
     const float* bias = a.bias ? a.bias + (int64_t)(a.H + pg) * a.hd : nullptr;
     const T* src = qkv + ((int64_t)(t0 + first - pos0) * heads + a.H + pg) * a.hd;
     // every unit of the block's new tokens, `lanes` at a time, AT_ONCE of them requested before the first is worked on:
     // use(token, unit, values)
     constexpr int AT_ONCE = 2;
-    const int units = live ? count * upt : 0, d_tok = lanes / upt, d_u = lanes - d_tok * upt;
+    const int units = live ? count * upt : 0, d_tok = a.lane_tokens, d_u = lanes - d_tok * upt;
     auto walk = [&](auto use) {
-        int tok = lane / upt, u_ = lane - tok * upt;
+        int tok = a.by_upt.quotient(lane), u_ = lane - tok * upt;
         for (int i = lane; i < units; i += AT_ONCE * lanes) {
             Raw<T, W> raw[AT_ONCE];
             int toks[AT_ONCE], us[AT_ONCE];
@@ -267,7 +269,7 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
         for (int j = 0; j < 2 * W; ++j) top = fmaxf(top, fabsf(v[j]));                // (a NaN leaves it as it is)
     });
     const int64_t plane_of = ((int64_t)page * 2 + plane) * a.G + g;
-    uint8_t* scale = a.scales + (page >= 0 ? plane_of * (a.page_size / a.block) + cell / a.block : 0);
+    uint8_t* scale = a.scales + (page >= 0 ? plane_of * a.page_blocks + a.by_block.quotient(cell) : 0);
     const int had = page >= 0 && n_old > 0 ? *scale : 0;          // (read by all before the group meets, written by one after)
     top = over_group(top);
     const bool odd = !q8_finite(top);                             // an infinity: it leaves the scale to the others
@@ -317,10 +319,27 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
     if (lane == 0) *scale = (uint8_t)byte;
 }
 
+// 32 bytes of T in one store: a whole sector
+__device__ __forceinline__ void store_32_bytes(float* to, const float* v) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                 "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+}
+__device__ __forceinline__ void store_32_bytes(__nv_bfloat16* to, const float* v) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
 // Reading back: the values of positions from .. to - 1 of a row, into pages of T through a table of their own.  A page is
-// one run of bytes; a thread takes READ_PIECES pieces of it, each of which becomes 32 bytes (131,072 tokens of 8 heads of
-// 128 to bfloat16: 131 us, 0.95 of the copy rate; pieces that become 64 bytes took twice as long in 32 bits).  grid
-// (pieces of a page, pages of a row, rows).
+// one run of bytes; a thread takes READ_PIECES pieces of it, each of which becomes 32 bytes and leaves in one store:
+// 131,072 tokens of 8 heads of 128 to bfloat16 123 us (the bytes at the copy rate: 125), nine rows of up to 1,777 tokens of
+// heads of 64 to 32 bits 8.2.  Two stores of 16 bytes, so that a warp's store fills halves of sectors, took 148 and 13.6,
+// pieces that become 16 bytes 143 and 10.3.  grid (pieces of a page, pages of a row, rows).
 constexpr int READ_THREADS = 256, READ_PIECES = 4;
 template <typename T> constexpr int READ_BYTES = 32 / (int)sizeof(T);
 
@@ -334,6 +353,7 @@ struct ReadArgs {
     const int* row_from; const int* row_to;
     const int* row_start; const int* row_pos0; const int* row_list; int window, listed_pages;
     int* out_table; int out_stride; uint8_t* odd;
+    Divisor by_hd, by_page, by_block; int page_blocks;
 };
 
 template <typename T, bool LISTED>
@@ -349,14 +369,15 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict_
         const int n_new = a.row_start[r + 1] - a.row_start[r], pos0 = a.row_pos0[r];
         to = n_new > 0 ? pos0 + n_new : 0;
         // (whole pages: what the first one holds in front of the window meets a probability of zero)
-        from = a.window > 0 ? max(0, pos0 - a.window + 1) / page_size * page_size : 0;
+        from = a.window > 0 ? a.by_page.quotient(max(0, pos0 - a.window + 1)) * page_size : 0;
     } else {
         from = max(a.row_from[r], 0);
         to = a.row_to[r];
     }
-    const int64_t p_end = listed ? a.listed_pages : ((int64_t)to + page_size - 1) / page_size;
-    for (int64_t p = (listed ? 0 : from / page_size) + (int64_t)blockIdx.y; p < p_end; p += gridDim.y) {
-        const bool needed = p >= from / page_size && p * page_size < to;
+    const int first_page = a.by_page.quotient(from);
+    const int64_t p_end = listed ? a.listed_pages : to > 0 ? a.by_page.quotient(to - 1) + 1 : 0;
+    for (int64_t p = (listed ? 0 : first_page) + (int64_t)blockIdx.y; p < p_end; p += gridDim.y) {
+        const bool needed = p >= first_page && p * page_size < to;
         const int page = needed ? a.table[(int64_t)r * a.table_stride + p] : -1;
         int out_page;
         if (listed) {
@@ -367,7 +388,7 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict_
         }
         if (!listed && (page < 0 || out_page < 0)) continue;
         const uint8_t* src = a.pages + (int64_t)page * pieces * BYTES;
-        const uint8_t* sc = a.scales + (int64_t)page * (2 * a.G * (page_size / a.block));
+        const uint8_t* sc = a.scales + (int64_t)page * (2 * a.G * a.page_blocks);
         T* dst = out + (int64_t)out_page * pieces * BYTES;
         const int c0 = blockIdx.x * READ_THREADS * READ_PIECES + threadIdx.x;
         uint32_t x[READ_PIECES][WORDS];
@@ -375,8 +396,8 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict_
         bool odd = false;
 #pragma unroll
         for (int k = 0; k < READ_PIECES; ++k) {
-            const int c = c0 + k * READ_THREADS, row = c * BYTES / a.hd;    // of the page's 2 G page_size rows
-            const int64_t pos = p * page_size + row % page_size;
+            const int c = c0 + k * READ_THREADS, row = a.by_hd.quotient(c * BYTES);    // of the page's 2 G page_size rows
+            const int64_t pos = p * page_size + row - a.by_page.quotient(row) * page_size;
             b[k] = -1;
             if (out_page >= 0 && c < pieces && pos >= from && pos < to) {
                 if constexpr (WORDS == 4) {
@@ -386,7 +407,7 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict_
                     const uint2 w = __ldg(reinterpret_cast<const uint2*>(src) + c);
                     x[k][0] = w.x; x[k][1] = w.y;
                 }
-                b[k] = sc[row / a.block];
+                b[k] = sc[a.by_block.quotient(row)];
             }
         }
 #pragma unroll
@@ -404,7 +425,7 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict_
                 v[4 * j + 2] = hi.x * power;
                 v[4 * j + 3] = hi.y * power;
             }
-            store_w<T, BYTES>(dst + (int64_t)(c0 + k * READ_THREADS) * BYTES, v);
+            store_32_bytes(dst + (int64_t)(c0 + k * READ_THREADS) * BYTES, v);
         }
         if (listed) {
             const int any = __syncthreads_or(odd);
@@ -449,8 +470,9 @@ SLLM_EXPORT int sllm_rope_kv_write_q8(const void* qkv, void* q_out, const int* r
     const int threads = a.lanes > 32 ? a.lanes : WRITE_THREADS;
     const int64_t slots = a.single ? n_rows : (int64_t)n_tokens / block + 2 * (int64_t)n_rows;
     const int in_cta = threads / a.lanes;
-    a.n_tasks = write ? slots * 2 * G : 0;
-    const int64_t kv_ctas = (a.n_tasks + in_cta - 1) / in_cta;
+    if (slots * 2 * G > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    a.n_tasks = write ? (int)(slots * 2 * G) : 0;
+    const int64_t kv_ctas = ((int64_t)a.n_tasks + in_cta - 1) / in_cta;
     // (few tokens share a token's heads out further: a thread's heads come one after the other)
     a.q_groups = H < 4 ? H : 4;
     while (a.q_groups < H && (int64_t)n_tokens * a.q_groups * upt < 148 * 256) a.q_groups = a.q_groups * 2 < H ? a.q_groups * 2 : H;
@@ -462,6 +484,17 @@ SLLM_EXPORT int sllm_rope_kv_write_q8(const void* qkv, void* q_out, const int* r
     if (q_ctas > most) q_ctas = most;
     if (kv_ctas + q_ctas > 0x7fffffff) return (int)cudaErrorInvalidValue;
     a.kv_ctas = (int)kv_ctas;
+    a.q_per_group = (H + a.q_groups - 1) / a.q_groups;
+    a.q_at_once = at_once;
+    a.lane_tokens = a.lanes / upt;
+    a.page_blocks = page_size / block;
+    a.by_lanes = divisor(a.lanes);
+    a.by_upt = divisor(upt);
+    a.by_planes = divisor(2 * G);
+    a.by_g = divisor(G);
+    a.by_block = divisor(block);
+    a.by_page = divisor(page_size);
+    a.by_q_groups = divisor(a.q_groups);
     const int64_t ctas = kv_ctas + q_ctas;
     if (dtype == 0) return wide ? launch_write<float, 4>(qkv, q_out, a, ctas, threads, stream)
                                 : launch_write<float, 1>(qkv, q_out, a, ctas, threads, stream);
@@ -471,12 +504,16 @@ SLLM_EXPORT int sllm_rope_kv_write_q8(const void* qkv, void* q_out, const int* r
 
 static int launch_read(void* out, ReadArgs a, int n_rows, int64_t most, int dtype, cudaStream_t stream) {
     if (a.G <= 0 || a.hd <= 0 || a.hd % 16 || a.page_size <= 0 || a.block <= 0 || a.page_size % a.block ||
-        (int64_t)a.G * a.page_size * a.hd > (1 << 27) || (((uintptr_t)a.pages | (uintptr_t)out) & 15) ||
+        (int64_t)a.G * a.page_size * a.hd > (1 << 27) || ((uintptr_t)a.pages & 15) || ((uintptr_t)out & 31) ||
         (dtype != 0 && dtype != 1))
         return (int)cudaErrorInvalidValue;
     const int pieces = 2 * a.G * a.page_size * a.hd / (dtype == 0 ? READ_BYTES<float> : READ_BYTES<__nv_bfloat16>),
               per = READ_THREADS * READ_PIECES;
     if (most > 65535) most = 65535;
+    a.by_hd = divisor(a.hd);
+    a.by_page = divisor(a.page_size);
+    a.by_block = divisor(a.block);
+    a.page_blocks = a.page_size / a.block;
     for (int r = 0; r < n_rows; r += 65535) {
         a.first_row = r;
         const dim3 grid((pieces + per - 1) / per, (unsigned)most, n_rows - r < 65535 ? n_rows - r : 65535);

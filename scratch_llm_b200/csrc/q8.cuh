@@ -17,6 +17,17 @@
 
 namespace sllm {
 
+// n / d for 0 <= n < 2^31: 2 n * ceil(2^(31 + s) / d) / 2^(32 + s), 2^s >= d
+struct Divisor {
+    uint32_t magic; int shift, d;
+    __device__ __forceinline__ int quotient(int n) const { return (int)(__umulhi(2u * (uint32_t)n, magic) >> shift); }
+};
+static Divisor divisor(int d) {
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s, d};
+}
+
 // 448 = 1.75 * 2^8: with amax = m * 2^(E - 127), 1 <= m < 2, b = E - 8, one more where m > 1.75.
 __device__ __forceinline__ int q8_scale_byte(float amax) {
     const int bits = __float_as_int(amax);

@@ -1074,8 +1074,8 @@ def kv_read_q8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Ten
     if not _is_table(out_table, device, n_rows):
         _refuse(out_table, "out_table", torch.int32, device, f"{n_rows} contiguous rows")
     at = out.data_ptr()
-    if at % 16:
-        raise KernelError("out must start on a 16-byte boundary")
+    if at % 32:
+        raise KernelError("out must start on a 32-byte boundary")
     _check(_q8_function("sllm_kv_read_q8", 0, "pppippppiiiiiiiip")(
         pages.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride()[0], row_from.data_ptr(),
         row_to.data_ptr(), at, out_table.data_ptr(), out_table.stride()[0], n_rows, max_tokens, page_size, block, g, hd, code,

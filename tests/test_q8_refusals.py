@@ -122,7 +122,7 @@ def test_write_refuses_shared_and_unaligned_memory(fake, monkeypatch):
         ops.rope_kv_write_q8(**write_args(fake, pages=pages))
 
 
-def test_read_refuses(fake):
+def test_read_refuses(fake, monkeypatch):
     pages, scales = cache(fake)
     rows, table = fake(2, dtype=I32), fake(2, 4, dtype=I32)
     call = lambda out, **k: ops.kv_read_q8(pages, scales, k.get("table", table), 16, k.get("a", rows), k.get("z", rows), out,  # noqa: E731
@@ -142,6 +142,9 @@ def test_read_refuses(fake):
         call(good, z=fake(2))
     with pytest.raises(KernelError, match="out_table"):
         call(good, out_table=fake(1, 4, dtype=I32))
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda self: 4096 if self.dtype == E4M3 else 4096 + 16)
+    with pytest.raises(KernelError, match="32-byte"):
+        call(good)
 
 
 def test_attention_refuses(fake):
