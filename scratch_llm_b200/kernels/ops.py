@@ -1097,13 +1097,14 @@ def _attention_q8_form(device: int, head_dim: int, code: int, nt: int) -> tuple[
 def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_new: int, max_context: int, n_heads: int,
                        n_kv_heads: int, window: int) -> tuple[int, int, int]:
     """How a launch is shared out: (queries of a CTA / 8, CTAs along the keys, 1 where these are a cluster that merges by
-    itself, else 2 where all CTAs fit and 0 where they do not).  Sixteen queries a CTA where that leaves no places empty and there is work to fill the device: 16 ragged rows
-    of 32 packed queries after up to 4,000 tokens 65 us against 74, 4 rows after 300 14.8 against 10.4.  The number of CTAs
-    along the keys is the one with the least cost in turns of a warp (a tile): a CTA costs 1.5 turns beside its
-    own, launches of more CTAs than fit take between the whole and the fractional number of rounds, a cluster merges in
-    1.8 turns and more where the device is nearly full of clusters, a kernel of its own in 4.9.  The
-    numbers are those with which 215 launches (1 to 64 rows of 300 to 16,000 keys, even and ragged, 32 heads of 64 and 128
-    on 8 kv heads and 40 on 40, one to eight tokens) came out 3 % above the best of all choices on average."""
+    itself, else 2 where all CTAs fit and 0 where they do not).  Sixteen queries a CTA where that leaves no places empty and
+    there is work to fill the device: 16 ragged rows of 32 packed queries after up to 4,000 tokens 65 us against 74, 4 rows
+    after 300 14.8 against 10.4.  The number of CTAs along the keys is the one with the least cost in turns of a warp (a
+    tile): a CTA costs 1.5 turns beside its own, launches of more CTAs than fit take between the whole and the
+    fractional number of rounds, a cluster merges in 1.8 turns and more where the device is nearly full of clusters, a
+    kernel of its own in 4.9.  The numbers are those with which 215 launches (1 to 64 rows of 300 to 16,000 keys, even and
+    ragged, 32 heads of 64 and 128 on 8 kv heads and 40 on 40, one to eight tokens) came out 3 % above the best of all
+    choices on average."""
     packed = max_new * (n_heads // n_kv_heads)
     keys = min(max_context, window + max_new) if window else max_context
     eights = -(-packed // 8)
@@ -1130,17 +1131,17 @@ def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_n
 def _attention_q8_in_16_bits(device: int, n_list: int, max_new: int, max_context: int, n_heads: int, n_kv_heads: int,
                              head_dim: int, page_size: int, window: int) -> bool:
     """Whether bfloat16 rows are read back into pages of 16 bits and attended to by the tcgen05 kernel.  Both ways' times in us
-    from what 1, 4 and 16 rows of 8 to 256 tokens after 500 to 16,000 took, 32 heads of 64 and 128 on 8 kv heads and 40 of
-    128 on 40: the kernel over 8 bits 8 + 3.2e-5 a key and eight queries of a kv head of 128 (2.4e-5 of 64), the other way 14
-    + 0.0105 a key and round of its CTAs + the copy's bytes.  (One row of 64 tokens after 16,000 152 / 177, of 128 285 / 178; 16
-    rows of 16 after 500 35 / 30.)"""
+    from what 1, 4 and 16 rows of 4 to 256 tokens after none to 16,000 took, 32 heads of 64 and 128 on 8 kv heads and 40 of
+    128 on 40 (284 launches, 1 % above the better way on average): the kernel over 8 bits 11.5 + 2.9e-5 a key and eight
+    queries of a kv head of 128 (1.8e-5 of 64), the other way 11.7 + 0.0084 a key and round of its CTAs + the copy's bytes.
+    (One row of 64 tokens after 16,000 139 / 172, of 128 250 / 173; 16 rows of 16 after 500 39 / 27.)"""
     if not attention_tc_supports(n_heads, n_kv_heads, head_dim, page_size, window, biased=bool(window)):
         return False
     packed = max_new * (n_heads // n_kv_heads)
     keys = min(max_context, window + max_new) if window else max_context
-    direct = 8 + n_list * n_kv_heads * -(-packed // 8) * keys * (1.64e-5 + 1.25e-7 * head_dim)
+    direct = 11.5 + n_list * n_kv_heads * -(-packed // 8) * keys * (7.5e-6 + 1.68e-7 * head_dim)
     rounds = max(1.0, n_list * n_kv_heads * -(-packed // 128) / _sm_count(device))
-    other = 14 + keys * 0.0105 * max(1.0, head_dim / 128) * rounds + n_list * keys * n_kv_heads * head_dim * 1e-6
+    other = 11.7 + keys * 0.0084 * max(1.0, head_dim / 128) * rounds + n_list * keys * n_kv_heads * head_dim * 1.58e-6
     return other < direct
 
 
