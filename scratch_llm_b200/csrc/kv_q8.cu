@@ -101,18 +101,18 @@ template <typename T, int W> struct Raw {
 };
 
 // A unit's values with the bias, turned.
-template <typename T, int W>
+template <typename T, int W, bool BIAS>
 __device__ __forceinline__ void unit_values(const WriteArgs& a, const Raw<T, W>& raw, const float* bias, const Unit<W>& u,
-                                            bool turns, const float* c, const float* s, float* v) {
+                                            const float* c, const float* s, float* v) {
     raw.values(v);
-    if (bias != nullptr) {
+    if constexpr (BIAS) {
         float b[2 * W];
         load_w<float, W>(bias + u.e0, b);
         load_w<float, W>(bias + u.e1, b + W);
 #pragma unroll
         for (int i = 0; i < 2 * W; ++i) v[i] = __fadd_rn(v[i], b[i]);
     }
-    if (turns && u.pair0 >= 0) {
+    if (u.pair0 >= 0) {
         auto turn = [&](float& x0, float& x1, int i) {
             const float y0 = __fsub_rn(__fmul_rn(x0, c[i]), __fmul_rn(x1, s[i]));
             x1 = __fadd_rn(__fmul_rn(x0, s[i]), __fmul_rn(x1, c[i]));
@@ -149,13 +149,13 @@ __device__ __forceinline__ int row_of(const WriteArgs& a, int n) { return last_r
 // CTAs 0 .. kv_ctas - 1: a group of a.lanes threads takes one block of the cache (what a row stores in it), for one
 // plane and kv head, twice: for its largest value, then, from L1, to store it: blocks of any size, and room for the warps
 // that its chain of look-ups and two reads wants.  8,192 tokens of 32 + 8 + 8 heads of 128, blocks of 16, with the queries:
-// 46 us (29 at the copy rate); 1,581 tokens of 3 x 40 heads, blocks of 64, in 32 bits with biases: 38 (22); eight rows of
-// one token 2.7.  With the block in registers 49, 60 and 3.0; with a CTA a block and a thread's unit in several heads 45, 36
+// 42 us (29 at the copy rate, 46 where every unit asks for a bias); 1,581 tokens of 3 x 40 heads, blocks of 64, in 32 bits with biases: 38 (22); eight rows of
+// one token 2.5.  With the block in registers 49, 60 and 3.0; with a CTA a block and a thread's unit in several heads 45, 36
 // and 2.9, but up to 60 % more where rows fill parts of blocks.  The queries stream (26 us alone); the blocks' CTAs are
 // bound by instruction issue, so that the two parts' times add up in whichever order their CTAs start.
 // Row r has the slots from row_start[r] / block + 2 r on, at least as many as it touches blocks: n new tokens touch at
 // most n / block + 2.  The other CTAs turn the queries.
-template <typename T, int W>
+template <typename T, int W, bool BIAS>
 __global__ void __launch_bounds__(WRITE_THREADS, 4)
 rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const WriteArgs a) {
     __shared__ float warp_top[2][WRITE_THREADS / 32];
@@ -187,7 +187,7 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
                     const int h = h0 + j;
                     if (h >= end) break;
                     float v[2 * W];
-                    unit_values<T, W>(a, raw[j], a.bias ? a.bias + (int64_t)h * a.hd : nullptr, u, true, c, s, v);
+                    unit_values<T, W, BIAS>(a, raw[j], BIAS ? a.bias + (int64_t)h * a.hd : nullptr, u, c, s, v);
                     T* to = q_out + ((int64_t)n * a.H + h) * a.hd;
                     store_w<T, W>(to + u.e0, v);
                     store_w<T, W>(to + u.e1, v + W);
@@ -222,11 +222,12 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
     // (the page is looked up while the values are on their way)
     const int begin = first - n_old, at_page = a.by_page.quotient(begin), cell = begin - at_page * a.page_size;
     const int page = live ? a.table[(int64_t)r * a.table_stride + at_page] : -1;
-    const float* bias = a.bias ? a.bias + (int64_t)(a.H + pg) * a.hd : nullptr;
+    const float* bias = BIAS ? a.bias + (int64_t)(a.H + pg) * a.hd : nullptr;
     const T* src = qkv + ((int64_t)(t0 + first - pos0) * heads + a.H + pg) * a.hd;
     // every unit of the block's new tokens, `lanes` at a time, AT_ONCE of them requested before the first is worked on:
     // use(token, unit, values)
     constexpr int AT_ONCE = 2;
+    const int rot = plane == 0 ? a.rot : 0;
     const int units = live ? count * upt : 0, d_tok = a.lane_tokens, d_u = lanes - d_tok * upt;
     auto walk = [&](auto use) {
         int tok = a.by_upt.quotient(lane), u_ = lane - tok * upt;
@@ -237,7 +238,7 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
             for (int k = 0; k < AT_ONCE; ++k) {
                 toks[k] = tok;
                 us[k] = u_;
-                if (i + k * lanes < units) raw[k].load(src + (int64_t)tok * heads * a.hd, Unit<W>(u_, a.rot, a.interleaved));
+                if (i + k * lanes < units) raw[k].load(src + (int64_t)tok * heads * a.hd, Unit<W>(u_, rot, a.interleaved));
                 tok += d_tok;
                 u_ += d_u;
                 if (u_ >= upt) { u_ -= upt; ++tok; }
@@ -245,10 +246,10 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
 #pragma unroll
             for (int k = 0; k < AT_ONCE; ++k) {
                 if (i + k * lanes >= units) break;
-                const Unit<W> u(us[k], a.rot, a.interleaved);
+                const Unit<W> u(us[k], rot, a.interleaved);
                 float c[W], s[W], v[2 * W];
-                if (plane == 0) load_angles<W>(a, u, first + toks[k], c, s);
-                unit_values<T, W>(a, raw[k], bias, u, plane == 0, c, s, v);
+                load_angles<W>(a, u, first + toks[k], c, s);
+                unit_values<T, W, BIAS>(a, raw[k], bias, u, c, s, v);
                 use(toks[k], u, v);
             }
         }
@@ -441,8 +442,8 @@ using namespace sllm;
 
 template <typename T, int W>
 static int launch_write(const void* qkv, void* q_out, const WriteArgs& a, int64_t ctas, int threads, cudaStream_t stream) {
-    return (int)sllm_launch_pdl(rope_kv_write_q8_kernel<T, W>, dim3((unsigned)ctas), dim3(threads), 0, stream,
-                                (const T*)qkv, (T*)q_out, a);
+    return (int)sllm_launch_pdl(a.bias ? rope_kv_write_q8_kernel<T, W, true> : rope_kv_write_q8_kernel<T, W, false>,
+                                dim3((unsigned)ctas), dim3(threads), 0, stream, (const T*)qkv, (T*)q_out, a);
 }
 
 // write = 0: only the queries.  dtype 0: float32, 1: bfloat16.  block divides page_size.
