@@ -148,11 +148,12 @@ __device__ __forceinline__ int row_of(const WriteArgs& a, int n) { return last_r
 
 // CTAs 0 .. kv_ctas - 1: a group of a.lanes threads takes one block of the cache (what a row stores in it), for one
 // plane and kv head, twice: for its largest value, then, from L1, to store it: blocks of any size, and room for the warps
-// that its chain of look-ups and two reads wants.  8,192 tokens of 32 + 8 + 8 heads of 128, blocks of 16, with the queries:
-// 42 us (29 at the copy rate, 46 where every unit asks for a bias); 1,581 tokens of 3 x 40 heads, blocks of 64, in 32 bits with biases: 38 (22); eight rows of
-// one token 2.5.  With the block in registers 49, 60 and 3.0; with a CTA a block and a thread's unit in several heads 45, 36
-// and 2.9, but up to 60 % more where rows fill parts of blocks.  The queries stream (26 us alone); the blocks' CTAs are
-// bound by instruction issue, so that the two parts' times add up in whichever order their CTAs start.
+// that its chain of look-ups and two reads wants.  8,192 tokens of 32 + 8 + 8 heads of 128, blocks of 16, with the
+// queries: 42 us (29 at the copy rate; 46 where every unit asks for a bias); 1,581 tokens of 3 x 40 heads, blocks of 64,
+// in 32 bits with biases: 38 (22); eight rows of one token 2.5.  With the block in registers 49, 60 and 3.0; with a CTA a
+// block and a thread's unit in several heads 45, 36 and 2.9, but up to 60 % more where rows fill parts of blocks.  The
+// queries stream (26 us alone); the blocks' CTAs are bound by instruction issue, so that the two parts' times add up in
+// whichever order their CTAs start.
 // Row r has the slots from row_start[r] / block + 2 r on, at least as many as it touches blocks: n new tokens touch at
 // most n / block + 2.  The other CTAs turn the queries.
 template <typename T, int W, bool BIAS>
