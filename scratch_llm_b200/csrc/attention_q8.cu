@@ -413,7 +413,10 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     for (; tile < tile_end; tile += WARPS) {
         const int kt = k_lo + tile * KT;
         ok = mbar_wait(&full[warp], parity, 1);
-        if (!ok) break;
+        if (!ok) {                        // (given up on: once more as long for the copies under way)
+            mbar_wait(&full[warp], parity, 1);
+            break;
+        }
         // ---- scores, transposed: rows are keys, columns queries
         float s[KG][NT][4];
 #pragma unroll

@@ -5,7 +5,7 @@
 // stored.  The 8-bit form of rope_cache.cu, with its conventions: qkv [n_tokens, (H + 2G) * hd], q heads,
 // then k heads, then v heads; `bias` (may be null) added first; only the first `rot` entries of a head
 // turn, in pairs (2j, 2j + 1) or (j, j + rot / 2).  Row r brings the tokens row_start[r] .. row_start[r + 1] - 1, at
-// the positions from row_pos0[r] on; tokens behind the last row are left alone.
+// the positions from row_pos0[r] on; tokens before the first row and behind the last are left alone.
 //   pages  [n_pages, 2, G, page_size, hd]             e4m3
 //   scales [n_pages, 2, G, page_size / block]         e8m0
 // A block's scale comes from the values that this step stores in it and, where the row has stored earlier
@@ -172,7 +172,7 @@ rope_kv_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, const 
         for (int64_t i = (int64_t)(blockIdx.x - a.kv_ctas) * at_once + mine; i < a.n_q_items;
              i += (int64_t)(gridDim.x - a.kv_ctas) * at_once) {
             const int n = a.by_q_groups.quotient((int)i), group = (int)i - n * a.q_groups;
-            if (n >= a.row_start[a.n_rows]) continue;
+            if (n < a.row_start[0] || n >= a.row_start[a.n_rows]) continue;      // (of no row)
             const int r = row_of(a, n), pos = a.row_pos0[r] + n - a.row_start[r];
             const Unit<W> u(u_, a.rot, a.interleaved);
             float c[W], s[W];

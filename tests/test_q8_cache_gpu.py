@@ -169,6 +169,27 @@ def test_write_queries_only():
     assert torch.equal(dev[0].view(torch.uint8).cpu(), c.pages) and torch.equal(dev[1].view(torch.uint8).cpu(), c.scales)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_write_tokens_of_no_row(dtype):
+    """Tokens before the first row and behind the last: as if they were not there, and their places are left alone."""
+    from scratch_llm_b200.kernels import ops
+    H, G, hd, page = 4, 2, 64, 16
+    rows, n, front = [(20, 2), (0, 19), (5, 0), (31, 1)], 22, 37
+    gen = torch.Generator().manual_seed(9)
+    c = Cache(G, hd, page, 8, [b + m for b, m in rows], gen).fill(rows, gen)
+    cos, sin = (t.to(DEV) for t in tables(hd, hd, 64))
+    qkv = torch.randn(front + n + 9, (H + 2 * G) * hd, generator=gen).to(dtype).to(DEV)
+    start, pos0, got = i32(starts(rows)), i32([b for b, _ in rows]), []
+    for x, at in ((qkv[front:front + n].contiguous(), start), (qkv, start + front)):
+        dev = c.device()
+        q_out = torch.full((x.shape[0], H * hd), 7.0, dtype=dtype, device=DEV)
+        ops.rope_kv_write_q8(x, at, pos0, len(rows), 19, cos, sin, q_out, *dev, page, H, G, hd, True)
+        got.append((q_out, dev[0].view(torch.uint8), dev[1].view(torch.uint8)))
+    assert torch.equal(got[1][0][front:front + n], got[0][0]) and (got[0][0] != 7).any()
+    assert (got[1][0][:front] == 7).all() and (got[1][0][front + n:] == 7).all()
+    assert torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][2], got[1][2])
+
+
 def test_write_many_rows():
     """More rows than a warp has lanes, of mixed lengths, empty ones among them; a table wider than the rows need."""
     H, G, hd, page, block = 2, 1, 32, 16, 8
