@@ -824,7 +824,7 @@ using namespace sllm;
 
 // CTAs that the device holds at once, of the form for 8 (nt = 1) or 16 (nt = 2) queries; 0: not known.
 SLLM_EXPORT int sllm_attn_q8_slots(int dtype, int nt) {
-    if (dtype == 0) return nt == 1 ? slots<float, 1>() : 0;
+    if (dtype == 0) return nt == 1 ? slots<float, 1>() : slots<float, 2>();
     return nt == 1 ? slots<__nv_bfloat16, 1>() : slots<__nv_bfloat16, 2>();
 }
 // keys of a warp's tile
@@ -838,7 +838,7 @@ SLLM_EXPORT int sllm_attn_q8_error() {
     return code;
 }
 
-// nt: queries of a CTA / 8 (2: bfloat16 only).  merge 1: up to 8 splits are a cluster; else part, float [part_tokens, H,
+// nt: queries of a CTA / 8, 1 or 2.  merge 1: up to 8 splits are a cluster; else part, float [part_tokens, H,
 // n_splits, HD + 2], takes the splits' sums, of shares of one length (0) or of rows cut evenly (2).
 SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages, int64_t n_pages, const void* scales,
                              const int* table, int table_stride, int table_width, int page_size, int block,
@@ -848,7 +848,7 @@ SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages,
                              int64_t part_tokens, int merge, cudaStream_t stream) {
     if (n_list <= 0 || max_new <= 0) return 0;
     if (H <= 0 || G <= 0 || H % G || page_size <= 0 || block <= 0 || page_size % block || window < 0 || n_list > 65535 ||
-        table_width <= 0 || (dtype != 0 && dtype != 1) || (nt != 1 && !(nt == 2 && dtype == 1)) || n_splits < 1 ||
+        table_width <= 0 || (dtype != 0 && dtype != 1) || (nt != 1 && nt != 2) || n_splits < 1 ||
         (merge == 1 ? n_splits > MAX_CLUSTER : n_splits > 1 && part == nullptr) || ((uintptr_t)pages & 15))
         return (int)cudaErrorInvalidValue;
     const int64_t q_tiles = ((int64_t)max_new * (H / G) + 8 * nt - 1) / (8 * nt);
@@ -862,7 +862,9 @@ SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages,
                       (int)(share < 1 ? 1 : share), merge == 0, q_vec, 0, 0, merge == 1 && n_splits > 1, scale * LOG2E,
                       divisor(page_size), divisor(block)};
     typedef __nv_bfloat16 bf16;
-    if (dtype == 0) return launch<float, 1>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
+    if (dtype == 0)
+        return nt == 1 ? launch<float, 1>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream)
+                       : launch<float, 2>((const float*)q, (float*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
     return nt == 1 ? launch<bf16, 1>((const bf16*)q, (bf16*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream)
                    : launch<bf16, 2>((const bf16*)q, (bf16*)out, a, n_pages, n_list, max_new, (int)q_tiles, stream);
 }

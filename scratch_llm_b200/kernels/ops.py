@@ -1097,9 +1097,9 @@ def _attention_q8_form(device: int, head_dim: int, code: int, nt: int) -> tuple[
 def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_new: int, max_context: int, n_heads: int,
                        n_kv_heads: int, window: int) -> tuple[int, int, int]:
     """How a launch is shared out: (queries of a CTA / 8, CTAs along the keys, 1 where these are a cluster that merges by
-    itself, else 2 where all CTAs fit and 0 where they do not).  Sixteen queries a CTA where that leaves no places empty and
-    there is work to fill the device: 16 ragged rows of 32 packed queries after up to 4,000 tokens 65 us against 74, 4 rows
-    after 300 14.8 against 10.4.  The number of CTAs along the keys is the one with the least cost in turns of a warp (a
+    itself, else 2 where all CTAs fit and 0 where they do not).  Sixteen queries a CTA where that leaves few places empty and
+    there is work to fill the device: 16 ragged rows of 32 packed queries after up to 4,000 tokens 65 us against 74, 300
+    tokens of 32 bits after 3,000 168 against 189; 4 rows of 32 after 300 14.8 against 10.4.  The number of CTAs along the keys is the one with the least cost in turns of a warp (a
     tile): a CTA costs 1.5 turns beside its own, launches of more CTAs than fit take between the whole and the
     fractional number of rounds, a cluster merges in 1.8 turns and more where the device is nearly full of clusters, a
     kernel of its own in 4.9.  The numbers are those with which 215 launches (1 to 64 rows of 300 to 16,000 keys, even and
@@ -1108,7 +1108,7 @@ def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_n
     packed = max_new * (n_heads // n_kv_heads)
     keys = min(max_context, window + max_new) if window else max_context
     eights = -(-packed // 8)
-    nt = 2 if code == 1 and eights % 2 == 0 and n_list * n_kv_heads * eights * keys >= 400000 else 1
+    nt = 2 if (eights % 2 == 0 or eights >= 8) and n_list * n_kv_heads * eights * keys >= 400000 else 1
     slots, tile = _attention_q8_form(device, head_dim, code, nt)
     tiles = -(-eights // nt)
     if tiles > 65535 or n_list > 65535:

@@ -309,10 +309,11 @@ def test_attention_long_rows(dtype, H, G, hd, window, rows):
     check(c, q, rows, dtype, H, window, context=4096)       # (a bound above what the rows have)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("context", [None, 4096])
 @pytest.mark.parametrize("window", [0, 300])
 @pytest.mark.parametrize("plan", [(1, 3, 0), (1, 8, 1), (1, 13, 2), (1, 13, 0), (1, 64, 0), (2, 5, 0), (2, 5, 2), (2, 2, 1)])
-def test_attention_shares_of_ragged_rows(plan, window, context, monkeypatch):
+def test_attention_shares_of_ragged_rows(plan, window, context, dtype, monkeypatch):
     """However the keys are shared out: rows of fewer keys than shares, of none before their token, and a workspace that
     holds NaN beforehand."""
     from scratch_llm_b200.kernels import ops
@@ -323,11 +324,11 @@ def test_attention_shares_of_ragged_rows(plan, window, context, monkeypatch):
     gen = torch.Generator().manual_seed(17)
     c = Cache(G, hd, 16, 16, [b + m for b, m in rows], gen).fill([(b + m, 0) for b, m in rows], gen, 0.5)
     n = sum(m for _, m in rows)
-    q = (1.5 * torch.randn(n, H * hd, generator=gen)).to(torch.bfloat16)
+    q = (1.5 * torch.randn(n, H * hd, generator=gen)).to(dtype)
     for _ in range(2):
         gone = torch.full((n * H * plan[1] * (hd + 2),), float("nan"), device=DEV)
         del gone
-        check(c, q, rows, torch.bfloat16, H, window, context=context)
+        check(c, q, rows, dtype, H, window, context=context)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -169,7 +169,7 @@ def test_attention_refuses(fake):
 def test_attention_says_what_a_launch_holds(monkeypatch):
     monkeypatch.setattr(ops, "_attention_q8_form", lambda *a: (592, 32))
     plan = ops._attention_q8_plan.__wrapped__
-    for rows, new in ((65536, 1), (1, 200000)):
+    for rows, new in ((65536, 1), (1, 300000)):
         with pytest.raises(KernelError, match="at most 65,535 rows"):
             plan(0, 64, 0, rows, new, 300000, 32, 8, 0)
     for args in ((0, 64, 0, 1, 1, 1, 8, 8, 0), (0, 128, 1, 65535, 1, 1, 8, 8, 0), (0, 64, 0, 1, 100000, 200000, 32, 8, 100),
