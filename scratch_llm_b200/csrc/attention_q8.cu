@@ -513,6 +513,9 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                         Top = fmaxf(Top, __shfl_xor_sync(0xffffffffu, Top, x));
                     }
+                    // (whole numbers: their differences are exact, and so are the powers of two that bring sums together)
+                    top = ceilf(top);
+                    Top = ceilf(Top);
                     l[nt][e] *= ex2(m[nt][e] - top);
                     const float keep = ex2(M[nt][e] - Top);
                     m[nt][e] = top;
