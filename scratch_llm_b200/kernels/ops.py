@@ -1186,7 +1186,8 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     """Causal attention of the listed rows (all ``n_list`` of them in order for ``row_list`` None) over a cache held in 8
     bits (:func:`rope_kv_write_q8`), for single tokens, drafted tokens and portions of prompts alike.  ``q`` [N, H * hd] may be
     a column slice; bfloat16 or float32, and ``out`` likewise.  No row brings more than ``max_new`` tokens, and no query
-    stands at a position of ``max_context`` or more."""
+    stands at a position of ``max_context`` or more.  A listed row may be empty or listed twice, but ``row_start``,
+    ``row_pos0`` and ``block_table`` have to hold it."""
     device, dtype, shape, width = _device(), q.dtype, q.shape, n_heads * head_dim
     code, n = _code(dtype), shape[0] if shape else 0
     block = _q8_cache(pages, scales, n_kv_heads, page_size, head_dim, device)
