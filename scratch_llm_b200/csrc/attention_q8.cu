@@ -456,7 +456,8 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         const bool there = sc >= 0;
         const bool whole = __all_sync(0xffffffffu, there) && kt + KT - 1 <= first_pos && (a.window <= 0 || kt > last_pos - a.window);
         uint32_t seen_rows = 0;
-        if (!whole) seen_rows = __ballot_sync(0xffffffffu, there);
+        // (in front of the first query's window lies nothing that any query here sees)
+        if (!whole) seen_rows = __ballot_sync(0xffffffffu, there && (a.window <= 0 || kt + lane % KT > first_pos - a.window));
 
         // ---- scaled scores, their maxima
         const float own_k = __int_as_float((sc & 0xff) << 23), own_v = (float)(sc >> 8 & 0xff) - 127.f;
@@ -555,7 +556,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
                 take<HD / 8>(v_at[k & 1], (2 * i + (k >> 1)) * EIGHT, vr[k]);
                 if (!whole && !(seen_rows >> (16 * i + 2 * c4 + (k & 1) + 8 * (k >> 1)) & 1u))
 #pragma unroll
-                    for (int w = 0; w < VREGS; ++w) vr[k][w] = 0u;         // (a place without a key may hold a NaN)
+                    for (int w = 0; w < VREGS; ++w) vr[k][w] = 0u;         // (a place without a key that is seen may hold a NaN)
             }
 #pragma unroll
             for (int j = 0; j < KSTEPS; ++j) {
@@ -637,7 +638,8 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         odd |= isnan(sum) || isnan(total);
         leave(i, d, sum, top, total);
     }
-    // a NaN, and not all queries see the same keys: each of them by itself
+    // a NaN, and not all queries see the same keys (queries of one token do, and what they do not see is zeros above): each of
+    // them by itself
     if (__syncthreads_or(odd) && first_pos != last_pos) {
         for (int i = warp; i < nq; i += WARPS) {
             const int p = q0 + i, tok = p / GS, pos = pos0 + tok;
