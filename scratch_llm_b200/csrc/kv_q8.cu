@@ -351,8 +351,8 @@ struct ReadArgs {
     int page_size, block, G, hd, first_row;
     // positions [row_from[r], row_to[r]) of row r through out_table, or, where row_start is given: everything that the
     // queries of the listed rows see, page p of the i-th of them to page i * listed_pages + p, which the kernel writes
-    // into out_table[r] itself (-1 where a page is not needed); odd[i * listed_pages + p, blockIdx.x] is set to whether
-    // the CTA met a NaN
+    // into out_table[r] itself (-1 where a page is not needed); a NaN becomes zero there, and odd[i * listed_pages + p,
+    // blockIdx.x] is set to whether the CTA met one
     const int* row_from; const int* row_to;
     const int* row_start; const int* row_pos0; const int* row_list; int window, listed_pages;
     int* out_table; int out_stride; uint8_t* odd;
@@ -420,8 +420,12 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict_
             float v[BYTES];
 #pragma unroll
             for (int j = 0; j < WORDS; ++j) {
-                const uint32_t w = x[k][j];
-                if (listed) odd |= ((w & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u) != 0u;
+                uint32_t w = x[k][j];
+                if (listed) {
+                    const uint32_t nan = (w & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u;      // (the top bits of such bytes)
+                    odd |= nan != 0u;
+                    if (nan) w &= ~((nan >> 7) * 255u);
+                }
                 const float2 lo = q8_float2(w & 0xffffu), hi = q8_float2(w >> 16);
                 v[4 * j] = lo.x * power;
                 v[4 * j + 1] = lo.y * power;
@@ -550,7 +554,7 @@ SLLM_EXPORT int sllm_kv_read_q8_shares(int page_size, int G, int hd) {
 
 // What the queries of the listed rows see (row_list null: rows 0 .. n_list - 1), at most listed_pages pages a row, into
 // out [n_list * listed_pages, 2, G, page_size, hd]; row r's part of out_table names the pages.  odd: a byte for each page and
-// sllm_kv_read_q8_shares() of it, not 0 where a NaN was met.  bfloat16 only.
+// sllm_kv_read_q8_shares() of it, not 0 where a NaN was met, for which zero is read.  bfloat16 only.
 SLLM_EXPORT int sllm_kv_read_q8_listed(const void* pages, const void* scales, const int* table, int table_stride,
                                        const int* row_start, const int* row_pos0, const int* row_list, int n_list,
                                        int window, int listed_pages, void* out, int* out_table, int out_stride, uint8_t* odd,

@@ -1173,10 +1173,9 @@ def _attention_q8_portions(q, pages, scales, block_table, page_size, block, row_
             n_kv_heads, head_dim, stream), "kv_read_q8")
         attention_tc(q, plain, plain_table, page_size, starts, pos0, out, listed, n, max_new, n_heads, n_kv_heads, head_dim,
                      scale, window or None)
-        _check(_q8_function("sllm_attn_q8_odd", head_dim, "plpppiiipppipliifiplp")(
-            q.data_ptr(), q.stride(0), pages.data_ptr(), scales.data_ptr(), table.data_ptr(), table.stride(0), page_size, block,
-            starts.data_ptr(), pos0.data_ptr(), listed_at, n, out.data_ptr(), out.stride(0), n_heads, n_kv_heads, scale,
-            window, odd.data_ptr(), odd.numel(), stream), "attention_q8")
+        _check(_q8_function("sllm_attn_q8_odd", head_dim, "ppiipppipliiipiip")(
+            pages.data_ptr(), table.data_ptr(), table.stride(0), page_size, starts.data_ptr(), pos0.data_ptr(), listed_at, n,
+            out.data_ptr(), out.stride(0), n_heads, n_kv_heads, window, odd.data_ptr(), width, shares, stream), "attention_q8")
 
 
 def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, page_size: int,

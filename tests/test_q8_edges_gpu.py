@@ -31,3 +31,40 @@ def test_no_numbers_in_front_of_a_window(dtype, H, G, hd, page, window, rows, mo
         want, spread, reach = plain.attend(q, c.pages, c.scales, c.table, rows, page, H, G, hd, hd ** -0.5, window)
         assert not want.isnan().any() and not got.isnan().any()
         assert ((got - want).abs() <= tolerance(dtype, hd, want, spread, reach)).all()
+
+
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("planes", [(1,), (0, 1)])
+def test_portions_beside_a_row_with_no_numbers(window, planes, monkeypatch):
+    """Portions by way of 16 bits: a NaN in one row leaves the other rows' bits as they are, and of its own row those of the
+    queries far in front of it and of the other kv heads; what sees it, or stands beside it in a tile, is right."""
+    from scratch_llm_b200.kernels import ops
+    monkeypatch.setattr(ops, "_attention_q8_in_16_bits", lambda *a: True)
+    H, G, hd, page = 8, 2, 64, 16
+    rows = [(300, 200), (20, 300), (0, 33), (250, 150)]
+    gen = torch.Generator().manual_seed(31)
+    c = Cache(G, hd, page, 8, [b + m for b, m in rows], gen).fill([(b + m, 0) for b, m in rows], gen, 0.5)
+    q = torch.randn(sum(m for _, m in rows), H * hd, generator=gen).bfloat16()
+    clean = attend_on_device(c, q.to(DEV), rows, c.device(), H, hd ** -0.5, window)
+    bad = [(1, 250, 5), (3, 3, 9), (3, 280, 63)]                  # row, position, entry
+    for r, pos, d in bad:
+        for plane in planes:
+            c.pages[int(c.table[r, pos // page]), plane, 1, pos % page, d] = 0xFF
+    dev = c.device()
+    for row_list in (None, [3, 0, 1]):
+        got = attend_on_device(c, q.to(DEV), rows, dev, H, hd ** -0.5, window, row_list=row_list)
+        s = starts(rows)
+        for r in (0, 2):
+            if row_list is None or r in row_list:
+                assert torch.equal(got[s[r]:s[r + 1]], clean[s[r]:s[r + 1]])
+        same = lambda a, z: torch.equal(got[a:z].view(-1, H, hd)[:, :4], clean[a:z].view(-1, H, hd)[:, :4])  # noqa: E731
+        assert same(s[1], s[2]) and same(s[3], s[4])
+        assert torch.equal(got[s[1]:s[1] + 100], clean[s[1]:s[1] + 100])
+        for r in (1, 3):
+            part = slice(s[r], s[r + 1])
+            only = [(0, 0) if i != r else row for i, row in enumerate(rows)]
+            want, spread, reach = plain.attend(q[part], c.pages, c.scales, c.table, only, page, H, G, hd, hd ** -0.5, window)
+            mine = got[part].double().cpu()
+            assert torch.equal(mine.isnan(), want.isnan()) and want.isnan().any() and not want.isnan().all()
+            tol = tolerance(torch.bfloat16, hd, want, spread, reach, True)
+            assert ((mine - want).abs() <= tol)[~want.isnan()].all()
