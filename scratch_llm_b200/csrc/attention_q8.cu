@@ -639,9 +639,13 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         leave(i, d, sum, top, total);
     }
     // a NaN, and not all queries see the same keys (queries of one token do, and what they do not see is zeros above): each of
-    // them by itself
+    // them by itself, but for those whose denominator is one: they see a key with a NaN
     if (__syncthreads_or(odd) && first_pos != last_pos) {
         for (int i = warp; i < nq; i += WARPS) {
+            bool sees = false;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) sees |= isnan(sm_l[w][i]);
+            if (sees) continue;
             const int p = q0 + i, tok = p / GS, pos = pos0 + tok;
             const int lo = max(k_lo + tile_begin * KT, a.window > 0 ? pos - a.window + 1 : 0);
             const int hi = min(k_lo + tile_end * KT - 1, pos);
