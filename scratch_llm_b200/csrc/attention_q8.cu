@@ -8,10 +8,13 @@
 // cores' f16 form with the cache's numbers as they are (by bit operations, seven for four numbers, 64 rows of 4,096
 // keys took 141 us instead of 124).  The blocks' powers of two join the scores (2^ek) and the probabilities (2^ev) in 32
 // bits.  A query is brought into f16's range by a power of two of its own (largest entry
-// in [2^14, 2^15)): bfloat16 entries keep all their bits down to 2^-38 of the largest, 32-bit ones are split into two
-// halves (22 bits).  A probability is multiplied by its key's 2^ev before it becomes a half, against a running
-// maximum of its own, M = max(s + ev): what counts towards the output keeps 11 bits (22 in the 32-bit form) down
-// to 2^-20 of the largest, whatever the blocks' scales.
+// in [2^14, 2^15)): bfloat16 entries keep all their bits down to 2^-31 of the largest (a half's steps end at 2^-24), 32-bit
+// ones are split into two halves (22 bits down to 2^-16 of the largest, then steps of 2^-38 of it).  A probability is
+// multiplied by its key's 2^ev before it becomes a half, against a running maximum of its own, M = max(s + ev) rounded up: what
+// counts towards the output keeps 11 bits down to 2^-19 of the largest, whatever the blocks' scales.  In the 32-bit form
+// the rest beside the half becomes one too, 2^11 times as large, and is brought back in 32 bits: 22 bits down to 2^-18, 20 at
+// 2^-20 (unscaled it ran into the halves' steps: next to a key with most of the probability and values of zero 4.1e-5 off
+// sum p |v|, now below 1.1e-5).
 //
 // Layout.  The products are taken transposed, keys and then the values' entries as the 16 rows of mma.m16n8k16, queries as
 // its 8 columns: a decoded token's group of up to 8 query heads fills the instruction, and an output is spread over
@@ -47,6 +50,7 @@ constexpr float LOWEST = -1e30f;                         // below every score; f
 constexpr float STALE = 8.f;                             // how far a maximum may lag behind the scores (base 2)
 constexpr int MAX_CLUSTER = 8;                           // CTAs of a cluster, on every device of the kind
 constexpr float P_SHIFT = 6.f;                           // probabilities become halves times 2^6: 2^14 at most
+constexpr float REST = 2048.f;                           // what is left of a probability beside its half, times this
 
 struct Q8Args {
     int64_t q_stride, out_stride;
@@ -104,8 +108,10 @@ template <int PARTS, typename B> __device__ __forceinline__ void mma_parts(float
         mma_f16(d, a, b(0, 0), b(0, 1));
     } else {
         float x[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_f16(x, a, b(1, 0), b(1, 1));
 #pragma unroll
-        for (int part = PARTS - 1; part >= 0; --part) mma_f16(x, a, b(part, 0), b(part, 1));
+        for (int i = 0; i < 4; ++i) x[i] *= 1.f / REST;
+        mma_f16(x, a, b(0, 0), b(0, 1));
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[i] += x[i];
     }
@@ -120,9 +126,9 @@ __device__ __forceinline__ uint32_t halves(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 // what is left of (a, b) beside their halves
-__device__ __forceinline__ uint32_t halves_rest(float a, float b, uint32_t h) {
+__device__ __forceinline__ uint32_t halves_rest(float a, float b, uint32_t h, float times = 1.f) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    return halves(a - f.x, b - f.y);
+    return halves((a - f.x) * times, (b - f.y) * times);
 }
 
 // bytes 0 and 1 of a word, and bytes 2 and 3, as pairs of halves
@@ -545,7 +551,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
                     }
                     const uint32_t h = halves(y[0], y[1]);
                     p[0][i][nt][k] = transposed(h);
-                    if constexpr (PARTS == 2) p[1][i][nt][k] = transposed(halves_rest(y[0], y[1], h));
+                    if constexpr (PARTS == 2) p[1][i][nt][k] = transposed(halves_rest(y[0], y[1], h, REST));
                 }
         // ---- sums over the keys, transposed: rows are entries of a head
 #pragma unroll

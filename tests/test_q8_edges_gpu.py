@@ -68,3 +68,34 @@ def test_portions_beside_a_row_with_no_numbers(window, planes, monkeypatch):
             assert torch.equal(mine.isnan(), want.isnan()) and want.isnan().any() and not want.isnan().all()
             tol = tolerance(torch.bfloat16, hd, want, spread, reach, True)
             assert ((mine - want).abs() <= tol)[~want.isnan()].all()
+
+
+@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("hd", [64, 128, 48])
+def test_small_probabilities_beside_a_key_of_zeros_in_32_bits(new, hd):
+    """One key with nearly all of the probability and values of zero, as an attention sink has: the output comes from keys
+    with probabilities of 2^-17 to 2^-20 of it.  In units of sum_j p_j |v_j|: a probability as two halves, the second scaled
+    by 2^11, is off by at most 2^-36 against 2^5 * 2^-20 or more, 2^-21; scores are products of one entry, exact but
+    for three roundings (scale, its unit, their product) of at most 10 (base 2), for the key and for the sink 2 * 30 * 2^-24,
+    2^-18; the exponentials 2^-22 each; sums over 64 to 68 keys at most 2^-18 (16 keys an instruction, cut off at
+    2^-23 of the sum's largest part, and five additions, for each of a warp's tiles), the meeting of four warps, the
+    denominator, the division and the result 2^-20: less than 2^-16.5 together."""
+    H, G, page, n = 4, 2, 16, 63
+    gen = torch.Generator().manual_seed(hd)
+    c = Cache(G, hd, page, 16, [n + new], gen).fill([(n + new, 0)], gen, 0.0)
+    e4m3 = lambda x: plain.round_e4m3(torch.tensor(x).double()).view(torch.uint8)  # noqa: E731
+    for pos in range(n + new):
+        at, cell = int(c.table[0, pos // page]), pos % page
+        c.scales[at, 0] = 127
+        c.pages[at, 0, :, cell] = 0
+        c.pages[at, 0, :, cell, 0] = e4m3(10.0 if pos == 0 else -8.0 - pos % 3)
+        if pos == 0:
+            c.pages[at, 1, :, cell] = 0
+    q = torch.zeros(new, H, hd)
+    q[:, :, 0] = 8.0
+    scale = 0.97 * math.log(2.0) / 8.0
+    rows = [(n, new)]
+    got = attend_on_device(c, q.view(new, -1).to(DEV), rows, c.device(), H, scale).double().cpu()
+    want, spread, _ = plain.attend(q.view(new, -1), c.pages, c.scales, c.table, rows, page, H, G, hd, scale)
+    far = ((got - want).abs() / spread).max()
+    assert far <= 2.0 ** -16.5, f"{float(far):.3g} of sum p |v|"
