@@ -56,7 +56,9 @@ struct Q8Args {
     int64_t q_stride, out_stride;
     const uint8_t* pages; const uint8_t* scales; const int* table;
     const int* row_start; const int* row_pos0; const int* row_list;
-    float* part; int64_t part_tokens;                    // [tokens, H, n_splits, HD + 2]: sums, maximum, denominator
+    // [part_tokens, H, n_splits, HD + 2]: sums, maximum, denominator; listed row i's tokens from i * part_new on, or, where that
+    // is 0, every token of the step at its own place
+    float* part; int64_t part_tokens; int part_new;
     int table_stride, table_width, page_size, block, H, G, window, n_splits, per_split, one_length, q_vec, run, tiled, cluster;
     float scale_log2;
     Divisor page_div, block_div;
@@ -205,6 +207,12 @@ __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args
     }
 }
 
+// Token tok of the i-th listed row, whose first one is token t0: its place in a.part; -1: none.
+__device__ __forceinline__ int64_t part_place(const Q8Args& a, int i, int t0, int tok) {
+    const int64_t at = (a.part_new ? (int64_t)i * a.part_new : t0) + tok;
+    return (a.part_new == 0 || tok < a.part_new) && at < a.part_tokens ? at : -1;
+}
+
 // The queries of a row and kv head are packed: p = token * GS + j is the row's token `token` and query head g GS + j.  A
 // CTA takes 8 NT packed queries over a share of the keys; its warps take turns at the tiles.  (Warps that share the
 // queries between them, up to four times as many a CTA, fetch and turn every key as often, and were slower nearly
@@ -252,8 +260,8 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     if (tile_begin >= tile_end && a.n_splits > 1 && !a.cluster) {      // no share: nothing is read or merged
         for (int i = tid; i < nq; i += THREADS) {
             const int p = q0 + i, tok = p / GS, h = g * GS + p - tok * GS;
-            if (t0 + tok < a.part_tokens)
-                a.part[(((int64_t)(t0 + tok) * a.H + h) * a.n_splits + split) * (HD + 2) + HD + 1] = 0.f;
+            const int64_t place = part_place(a, blockIdx.z, t0, tok);
+            if (place >= 0) a.part[((place * a.H + h) * a.n_splits + split) * (HD + 2) + HD + 1] = 0.f;
         }
         return;
     }
@@ -624,8 +632,8 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         } else if (a.cluster) {
             sums[i * LD + d] = sum;                      // (query i's place of the first warp)
             if (d == 0) { all_top[i] = top; all_total[i] = total; }
-        } else if (t0 + tok < a.part_tokens) {
-            float* part = a.part + (((int64_t)(t0 + tok) * a.H + h) * a.n_splits + split) * (HD + 2);
+        } else if (const int64_t place = part_place(a, blockIdx.z, t0, tok); place >= 0) {
+            float* part = a.part + ((place * a.H + h) * a.n_splits + split) * (HD + 2);
             part[d] = sum;
             if (d == 0) { part[HD] = top; part[HD + 1] = total; }
         }
@@ -696,9 +704,9 @@ __global__ void __launch_bounds__(THREADS) attn_q8_merge_kernel(T* __restrict__ 
     pdl_trigger();
     const int r = a.row_list ? a.row_list[blockIdx.y] : blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tok = blockIdx.x / a.H, h = blockIdx.x - tok * a.H, t0 = a.row_start[r];
-    if (tok >= a.row_start[r + 1] - t0 || t0 + tok >= a.part_tokens) return;
-    const int64_t ld = HD + 2;
-    const float* part = a.part + ((int64_t)(t0 + tok) * a.H + h) * a.n_splits * ld;
+    const int64_t ld = HD + 2, place = part_place(a, blockIdx.y, t0, tok);
+    if (tok >= a.row_start[r + 1] - t0 || place < 0) return;
+    const float* part = a.part + (place * a.H + h) * a.n_splits * ld;
     float top = LOWEST, total = 0.f, sum[DPL];
     // (a total of zero: a share without a key)
     for (int k = lane; k < a.n_splits; k += 32)
@@ -893,7 +901,8 @@ SLLM_EXPORT int sllm_attn_q8_error() {
 }
 
 // nt: queries of a CTA / 8, 1 or 2.  merge 1: up to 8 splits are a cluster; else part, float [part_tokens, H,
-// n_splits, HD + 2], takes the splits' sums, of shares of one length (0) or of rows cut evenly (2).
+// n_splits, HD + 2], takes the splits' sums, of shares of one length (0) or of rows cut evenly (2): part_tokens is n_list *
+// max_new, or the tokens of the step where these are fewer.
 SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages, int64_t n_pages, const void* scales,
                              const int* table, int table_stride, int table_width, int page_size, int block,
                              const int* row_start, const int* row_pos0, const int* row_list, int n_list, int max_new,
@@ -912,7 +921,8 @@ SLLM_EXPORT int sllm_attn_q8(const void* q, int64_t q_stride, const void* pages,
     const int64_t share = ((keys + KT - 1) / KT + n_splits - 1) / n_splits;          // a row's at most
     const int q_vec = (uintptr_t)q % (4 * es) == 0 && q_stride % 4 == 0;
     const Q8Args a = {q_stride, out_stride, (const uint8_t*)pages, (const uint8_t*)scales, table, row_start, row_pos0, row_list,
-                      part, part_tokens, table_stride, table_width, page_size, block, H, G, window, n_splits,
+                      part, part_tokens, part_tokens == (int64_t)n_list * max_new ? max_new : 0, table_stride, table_width, page_size,
+                      block, H, G, window, n_splits,
                       (int)(share < 1 ? 1 : share), merge == 0, q_vec, 0, 0, merge == 1 && n_splits > 1, scale * LOG2E,
                       divisor(page_size), divisor(block)};
     typedef __nv_bfloat16 bf16;

@@ -1222,14 +1222,15 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
         return out
     nt, n_splits, merge = _attention_q8_plan(device, head_dim, code, n_list, max_new, max_context, n_heads, n_kv_heads,
                                              window)
-    part = None
+    part, part_tokens = None, min(n, n_list * max_new)
     if n_splits > 1 and merge != 1:
-        part = torch.empty(n * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
+        part = torch.empty(part_tokens * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
     _check(_q8_function("sllm_attn_q8", head_dim, "plplppiiiipppiiipliifiiiiplip")(
         q_at, q_stride, pages.data_ptr(), pages.shape[0], scales.data_ptr(), block_table.data_ptr(),
         block_table.stride()[0], block_table.shape[1], page_size, block, row_start.data_ptr(), row_pos0.data_ptr(),
         0 if row_list is None else row_list.data_ptr(), n_list, max_new, max_context, out_at, out_stride, n_heads,
-        n_kv_heads, scale, window, code, nt, n_splits, 0 if part is None else part.data_ptr(), n, int(merge), stream),
+        n_kv_heads, scale, window, code, nt, n_splits, 0 if part is None else part.data_ptr(), part_tokens, int(merge),
+        stream),
         "attention_q8")
     return out
 

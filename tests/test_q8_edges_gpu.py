@@ -99,3 +99,33 @@ def test_small_probabilities_beside_a_key_of_zeros_in_32_bits(new, hd):
     want, spread, _ = plain.attend(q.view(new, -1), c.pages, c.scales, c.table, rows, page, H, G, hd, scale)
     far = ((got - want).abs() / spread).max()
     assert far <= 2.0 ** -16.5, f"{float(far):.3g} of sum p |v|"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("listed", [[1], [2, 1], [3]])
+def test_workspace_of_the_listed_rows(listed, dtype):
+    """What a launch sets aside for the parts of its sums goes by the rows that it is asked for, not by the step's tokens."""
+    H, G, hd, page = 16, 4, 128, 64
+    rows = [(0, 3000), (8191, 1), (5000, 1), (6000, 3)]
+    gen = torch.Generator().manual_seed(3)
+    c = Cache(G, hd, page, 64, [b + m for b, m in rows], gen).fill([(b + m, 0) if r else (0, 0) for r, (b, m) in enumerate(rows)], gen, 0.5)
+    n, s = sum(m for _, m in rows), starts(rows)
+    q = torch.randn(n, H * hd, generator=gen).to(dtype)
+    dev, out, on = c.device(), torch.full((n, H * hd), 7.0, dtype=dtype, device=DEV), q.to(DEV)
+    attend_on_device(c, on, rows, dev, H, hd ** -0.5, row_list=listed, out=out)      # (what is loaded once)
+    out.fill_(7.0)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    attend_on_device(c, on, rows, dev, H, hd ** -0.5, row_list=listed, out=out)
+    took = torch.cuda.max_memory_allocated() - before
+    # 64 shares at most, each with a head's sums, maximum and denominator for every token that a listed row may bring
+    assert took <= 4 * 64 * len(listed) * 3 * H * (hd + 2) + (1 << 16), took
+    for r in range(len(rows)):
+        part = out[s[r]:s[r + 1]]
+        if r not in listed:
+            assert (part == 7).all()
+            continue
+        only = [row if i == r else (0, 0) for i, row in enumerate(rows)]
+        want, spread, reach = plain.attend(q[s[r]:s[r + 1]], c.pages, c.scales, c.table, only, page, H, G, hd, hd ** -0.5)
+        assert ((part.double().cpu() - want).abs() <= tolerance(dtype, hd, want, spread, reach)).all()
