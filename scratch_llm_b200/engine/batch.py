@@ -121,6 +121,9 @@ class StepBatch:
     #: the most tokens a row brings, or an upper bound that a padded step's sizes allow (above 1 only
     #: where rows of several tokens may be there)
     max_row: int = 0
+    #: the most tokens a row of several brings; in a padded step the next power of two, so that launches planned by it are
+    #: at most twice too large (a captured step is then one for such a bound: ModelRunner.step)
+    max_row_multi: int = 0
     min_new: int = 1          # the fewest tokens a row brings (a lower bound)
     min_new_multi: int = 2    # the fewest a row of several brings (a lower bound)
     max_context_single: int = 0
@@ -139,6 +142,7 @@ class StepBatch:
 
     def __post_init__(self) -> None:
         self.max_row = self.max_row or self.max_new
+        self.max_row_multi = self.max_row_multi or self.max_new_multi
 
 
 class BatchStager:
@@ -352,6 +356,7 @@ def _padded_batch(stager: BatchStager, plan: PadPlan, token_ids, positions, toke
         row_pos0=dev[4], row_slot=dev[5], logit_index=dev[6], single_rows=dev[7],
         multi_rows=dev[8], block_tables=dev[9:], n_single=plan.n_single, n_multi=plan.n_multi,
         max_new_multi=plan.n_tokens if plan.n_multi else 0, max_row=plan.max_row,
+        max_row_multi=min(plan.max_row, _next_power_of_two(max(lens))) if plan.n_multi else 0,
         min_new=1 if plan.n_single else 2,
         max_context_single=ctx_single, context_bucket=context_bucket(ctx_single),
         host_row_new=list(lens) + [0] * (rows_padded - n_rows),

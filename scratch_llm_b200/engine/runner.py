@@ -195,9 +195,11 @@ class ModelRunner:
                 width *= 2
             width = min(width, self._table_width)
             batch = self.build_batch(rows, table_width=width, pad=True)
+            # (over pages in 8 bits launches are planned by the longest row's bound as well)
+            longest = batch.max_row_multi if self.cache.scale_block is not None else 0
             logits = self._graph_step(batch, ("padded", batch.n_tokens, batch.n_single,
                                               batch.n_multi, batch.n_out, batch.context_bucket,
-                                              width), self.capture_padded_after)
+                                              width, longest), self.capture_padded_after)
             if logits is not None and batch.n_real_out != batch.n_out:
                 logits = logits[:batch.n_real_out]
         else:

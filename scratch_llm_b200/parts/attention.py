@@ -207,7 +207,7 @@ class GQAttention(Mixer):
         """Over pages held in 8 bits: the rotated queries go to a buffer of their own, keys and values are
         quantised as they are stored, and rows with one new token and rows with several are attended to in a
         launch each.  What a captured step plans with has to hold for every step that replays it: the
-        single rows' context bucket, and for the others what their block tables can name."""
+        single rows' context bucket, and for the others the longest row's bound and what their block tables can name."""
         H, G, hd = self.n_heads, self.n_kv_heads, self.head_dim
         cos, sin, interleaved, write = rope
         q = (torch.zeros if batch.padded else torch.empty)(
@@ -220,7 +220,7 @@ class GQAttention(Mixer):
         if batch.n_multi:
             context = cache.block_table.shape[1] * cache.page_size if batch.padded else batch.max_context
             rows = None if batch.n_multi == batch.n_rows else batch.multi_rows
-            ops.attention_q8(*common, rows, batch.n_multi, batch.max_new_multi, context, H, G, hd, self.scale,
+            ops.attention_q8(*common, rows, batch.n_multi, batch.max_row_multi, context, H, G, hd, self.scale,
                              self.window)
         if batch.n_single:
             rows = None if batch.n_single == batch.n_rows else batch.single_rows

@@ -1,0 +1,45 @@
+"""Edges of the cache held in 8 bits and of drafted tokens that need no GPU: what launches are planned with, and what is refused."""
+
+import ctypes
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from scratch_llm_b200.cache import CacheManager
+from scratch_llm_b200.engine.batch import RowInput, build_batch
+from scratch_llm_b200.kernels import ops
+from scratch_llm_b200.parts import KVSpec
+
+
+class Stager:
+    def upload(self, arrays):
+        return [torch.from_numpy(np.asarray(a, dtype=np.int32)) for a in arrays]
+
+
+@pytest.mark.parametrize("n_rows,new,before", [(8, 6, 2111), (16, 6, 2111), (32, 6, 2111), (8, 16, 4096), (16, 16, 4096), (32, 16, 4096),
+                                               (1, 300, 3000), (3, 5, 100), (2, 200, 1000), (1, 500, 20)])
+@pytest.mark.parametrize("decoded", [0, 20])
+def test_a_padded_step_is_planned_by_its_longest_row(n_rows, new, before, decoded, monkeypatch):
+    """Whatever a step is padded to, its portions go the way that the same step goes without padding."""
+    H, G, hd, page = 32, 8, 128, 64
+    monkeypatch.setattr(ops, "_sm_count", lambda device: 148)
+    cache = CacheManager([KVSpec(G, hd, None)], [None], page, 4000, 64)
+    rows = []
+    for i in range(n_rows + decoded):
+        cache.admit(i)
+        assert cache.reserve(i, before)
+        cache.commit(i, before)
+        rows.append(RowInput(i, [1] * (new if i < n_rows else 1)))
+        assert cache.reserve(i, len(rows[-1].tokens))
+    width = 8
+    while width * page < before + new:
+        width *= 2
+    exact = build_batch(cache, Stager(), rows, 10, 1 << 20)
+    padded = build_batch(cache, Stager(), rows, 10, 1 << 20, table_width=width, pad=True)
+    assert exact.max_row_multi == new <= padded.max_row_multi < 2 * new
+    ways = [ops._attention_q8_in_16_bits.__wrapped__(0, b.n_multi, b.max_row_multi, context, H, G, hd, page, 0)
+            for b, context in ((exact, exact.max_context), (padded, width * page))]
+    assert ways[0] == ways[1]

@@ -129,3 +129,38 @@ def test_workspace_of_the_listed_rows(listed, dtype):
         only = [row if i == r else (0, 0) for i, row in enumerate(rows)]
         want, spread, reach = plain.attend(q[s[r]:s[r + 1]], c.pages, c.scales, c.table, only, page, H, G, hd, hd ** -0.5)
         assert ((part.double().cpu() - want).abs() <= tolerance(dtype, hd, want, spread, reach)).all()
+
+
+def test_captured_steps_whose_longest_rows_differ(model_dirs, monkeypatch):
+    """Steps of the same padded sizes whose longest rows differ share no captured graph that would be too small for one of them,
+    and launches are asked for no more than twice the longest row."""
+    from configs import PAGE_SIZE
+    from plain import llama_plain as P
+    from scratch_llm_b200.engine import ModelRunner, RowInput
+    from scratch_llm_b200.engine.runner import load_model
+    from scratch_llm_b200.kernels import ops
+    from test_q8_engine_gpu import PlainModel
+    cfg, w = P.read_model_dir(model_dirs["B"])
+    runner = ModelRunner(load_model(model_dirs["B"], "float32", verbose=False), PAGE_SIZE["B"], 60, 4, poison_free_pages=True,
+                         cache_dtype="float8_e4m3fn")
+    runner.capture_padded_after = 2
+    asked, call = [], ops.attention_q8
+
+    def attention(*a, **k):
+        asked.append(a[10])
+        return call(*a, **k)
+
+    monkeypatch.setattr(ops, "attention_q8", attention)
+    gen = torch.Generator().manual_seed(4)
+    models = {n: PlainModel(cfg, w, PAGE_SIZE["B"], runner.cache.scale_block) for n in "abc"}
+    for n in models:
+        assert runner.admit(n)
+    for step in [dict(a=8, b=8), dict(a=7, b=6), dict(a=5, b=8), dict(a=2, b=14), dict(a=14, b=2), dict(a=3, b=13), dict(a=8, b=8),
+                 dict(a=4, b=3, c=3), dict(a=4, b=3, c=3), dict(a=2, b=9, c=2)]:
+        ids = {n: torch.randint(0, cfg["vocab_size"], (k,), generator=gen).tolist() for n, k in step.items()}
+        asked.clear()
+        got = runner.step([RowInput(n, t, [len(t) - 1]) for n, t in ids.items()]).cpu()
+        want = torch.cat([models[n].step(t)[-1:] for n, t in ids.items()])
+        assert (got - want).norm() / want.norm() < 4e-3
+        assert all(max(step.values()) <= m < 2 * max(step.values()) for m in asked)
+    assert runner.replayed_steps >= 4
