@@ -426,7 +426,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
 
     for (; tile < tile_end; tile += WARPS) {
         const int kt = k_lo + tile * KT;
-        ok = mbar_wait(&full[warp], parity, 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[warp], parity, 1));      // (a warp goes on or gives up as a whole)
         if (!ok) {                        // (given up on: once more as long for the copies under way)
             mbar_wait(&full[warp], parity, 1);
             break;
