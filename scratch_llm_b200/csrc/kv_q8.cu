@@ -458,7 +458,7 @@ SLLM_EXPORT int sllm_rope_kv_write_q8(const void* qkv, void* q_out, const int* r
                                       int table_stride, int page_size, int block, int H, int G, int hd, int write, int dtype,
                                       cudaStream_t stream) {
     if (n_rows <= 0 || n_tokens <= 0 || max_new <= 0) return 0;
-    if (H <= 0 || G <= 0 || hd <= 0 || hd % 16 || rot < 0 || rot > hd || rot % 2 || page_size <= 0 || block <= 0 ||
+    if (H <= 0 || G <= 0 || hd <= 0 || hd > 256 || hd % 16 || rot < 0 || rot > hd || rot % 2 || page_size <= 0 || block <= 0 ||
         page_size % block || (dtype != 0 && dtype != 1))
         return (int)cudaErrorInvalidValue;
     if (((uintptr_t)pages | (uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)bias | (uintptr_t)cos_t | (uintptr_t)sin_t) & 15)

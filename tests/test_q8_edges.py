@@ -1,6 +1,5 @@
 """Edges of the cache held in 8 bits and of drafted tokens that need no GPU: what launches are planned with, and what is refused."""
 
-import ctypes
 import subprocess
 import sys
 
@@ -43,3 +42,25 @@ def test_a_padded_step_is_planned_by_its_longest_row(n_rows, new, before, decode
     ways = [ops._attention_q8_in_16_bits.__wrapped__(0, b.n_multi, b.max_row_multi, context, H, G, hd, page, 0)
             for b, context in ((exact, exact.max_context), (padded, width * page))]
     assert ways[0] == ways[1]
+
+
+def entry_statuses(library: str, calls: list[str]) -> list[int]:
+    """What an entry of a built library returns for each call, in a process of its own (refusals come before any GPU is
+    touched)."""
+    done = subprocess.run([sys.executable, "-c", f"""
+from ctypes import c_float, c_int, c_int64, c_void_p
+from scratch_llm_b200.kernels import ops
+lib = {library}
+P, I, L, F = c_void_p, c_int, c_int64, c_float
+print(*[int(x) for x in [{", ".join("lib." + c for c in calls)}]])
+"""], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, f"the process ended with {done.returncode}: {done.stderr[-500:]}"
+    return [int(x) for x in done.stdout.splitlines()[-1].split()]
+
+
+def test_write_entry_refuses_large_heads():
+    """A head for which a CTA has too few threads is an error code, whoever calls."""
+    at = ", ".join(["P(0)"] * 4)
+    calls = [f"sllm_rope_kv_write_q8({at}, I(1), I(1), I(1), P(0), P(0), I({rot}), I(1), P(0), P(0), P(0), P(0), I(1), I(16), "
+             f"I(16), I(1), I(1), I({hd}), I(1), I(1), P(0))" for hd, rot in [(272, 0), (528, 2), (2064, 0), (4096, 8), (1 << 30, 0)]]
+    assert entry_statuses("ops._core('sllm_kv_q8')", calls) == [1] * 5            # cudaErrorInvalidValue
