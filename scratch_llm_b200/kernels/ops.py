@@ -951,6 +951,16 @@ def _is_matrix(t: torch.Tensor, dtype: torch.dtype, device: int, rows: int, colu
         and (columns <= 1 or t.stride()[1] == 1)
 
 
+def _apart(a: int, a_stride: int, b: int, b_stride: int, rows: int, columns: int, size: int) -> bool:
+    """Whether two matrices [rows, columns] of entries of ``size`` bytes, at ``a`` and ``b``, share no memory: they lie one behind
+    the other, or side by side in rows of one length."""
+    width = columns * size
+    if a + (rows - 1) * a_stride * size + width <= b or b + (rows - 1) * b_stride * size + width <= a:
+        return True
+    step = a_stride * size
+    return a_stride == b_stride and step > 0 and width <= (b - a) % step <= step - width
+
+
 def _refuse(t: torch.Tensor, name: str, dtype: torch.dtype | None, device: int, wanted: str) -> None:
     _need(t, dtype, name, contiguous=False)
     if t.get_device() != device:
@@ -1211,7 +1221,7 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     if n_list <= 0 or max_new <= 0:
         return out
     q_at, out_at, q_stride, out_stride = q.data_ptr(), out.data_ptr(), q.stride()[0], out.stride()[0]
-    if q_at == out_at:
+    if n and not _apart(q_at, q_stride, out_at, out_stride, n, width, q.element_size()):
         raise KernelError("out must be memory of its own: queries are read while outputs are written")
     stream = _stream_of(device)
     if code == 1 and max_new > 1 and _attention_q8_in_16_bits(device, n_list, max_new, max_context, n_heads, n_kv_heads,

@@ -6,10 +6,12 @@ import sys
 import numpy as np
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from scratch_llm_b200.cache import CacheManager
 from scratch_llm_b200.engine.batch import RowInput, build_batch
 from scratch_llm_b200.kernels import ops
+from scratch_llm_b200.kernels.ops import KernelError
 from scratch_llm_b200.parts import KVSpec
 
 
@@ -64,3 +66,51 @@ def test_write_entry_refuses_large_heads():
     calls = [f"sllm_rope_kv_write_q8({at}, I(1), I(1), I(1), P(0), P(0), I({rot}), I(1), P(0), P(0), P(0), P(0), I(1), I(16), "
              f"I(16), I(1), I(1), I({hd}), I(1), I(1), P(0))" for hd, rot in [(272, 0), (528, 2), (2064, 0), (4096, 8), (1 << 30, 0)]]
     assert entry_statuses("ops._core('sllm_kv_q8')", calls) == [1] * 5            # cudaErrorInvalidValue
+
+
+F32, I32, BF16 = torch.float32, torch.int32, torch.bfloat16
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    """Tensors on a pretended cuda:0 (test_q8_refusals.py); ``at`` places them, and a call that passes every check raises Reached."""
+    monkeypatch.setattr(ops, "_device", lambda: 0)
+    monkeypatch.setattr(ops, "_stream_of", lambda device: 0)
+    monkeypatch.setattr(ops, "_attention_q8_plan", lambda *a: (1, 1, 0))
+    monkeypatch.setattr(ops, "_attention_q8_in_16_bits", lambda *a: False)
+
+    def reach(*a):
+        raise Reached
+
+    monkeypatch.setattr(ops, "_q8_function", lambda *a: reach)
+    placed = []
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda self: next((at for t, at in placed if t is self), 1 << 40))
+
+    def make(*shape, dtype=F32, at=None, stride=None):
+        t = torch.empty(shape if stride is None else (shape[0], stride), dtype=dtype, device="cuda")
+        t = t if stride is None else t[:, :shape[1]]
+        placed.append((t, at if at is not None else (len(placed) + 1) << 24))
+        return t
+
+    with FakeTensorMode():
+        yield make
+
+
+class Reached(Exception):
+    pass
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("q_stride,out_stride,off,apart", [
+    (64, 64, 0, False), (64, 64, 8, False), (64, 64, 5 * 64, True), (64, 64, -5 * 64, True), (64, 64, 4 * 64, False), (64, 64, -64, False),
+    (160, 160, 64, True), (160, 160, 96, True), (160, 160, 104, False), (160, 160, 56, False), (160, 160, -64, True), (160, 160, -56, False),
+    (160, 160, 160 + 64, True), (160, 96, 64, False), (96, 160, 4 * 96 + 64, True), (160, 96, 4 * 160 + 56, False)])
+def test_attention_refuses_outputs_in_its_queries(fake, dtype, q_stride, out_stride, off, apart):
+    """Outputs that share memory with queries, wholly or in part; columns side by side are taken."""
+    size = 4 if dtype == F32 else 2
+    pages, scales = fake(8, 2, 2, 16, 16, dtype=torch.float8_e4m3fn), fake(8, 2, 2, 1, dtype=torch.float8_e8m0fnu)
+    q = fake(5, 64, dtype=dtype, stride=q_stride, at=1 << 32)
+    out = fake(5, 64, dtype=dtype, stride=out_stride, at=(1 << 32) + off * size)
+    with pytest.raises(Reached) if apart else pytest.raises(KernelError, match="memory of its own"):
+        ops.attention_q8(q, pages, scales, fake(2, 4, dtype=I32), 16, fake(3, dtype=I32), fake(2, dtype=I32), out, None, 2, 1, 40, 4, 2,
+                         16, 0.1)
