@@ -1282,10 +1282,13 @@ def verify_drafts(probs: torch.Tensor, drafts: torch.Tensor, draft_start: torch.
         raise KernelError(f"max_drafts must not be negative, got {max_drafts}")
     if n == 0:
         return
+    drafts_at, tokens_at = drafts.data_ptr(), tokens.data_ptr()
+    if k and drafts_at < tokens_at + 4 * (k + n) and tokens_at < drafts_at + 4 * k:
+        raise KernelError("tokens must be memory of its own: drafts are read while tokens are written")
     _check(_q8_function("sllm_verify_drafts", 0, "plplpppiippp")(
         probs.data_ptr(), probs.stride()[0], 0 if draft_probs is None else draft_probs.data_ptr(),
-        0 if draft_probs is None else draft_probs.stride()[0], drafts.data_ptr(), draft_start.data_ptr(), uniforms.data_ptr(), n,
-        v, tokens.data_ptr(), accepted.data_ptr(), _stream_of(device)), "verify_drafts")
+        0 if draft_probs is None else draft_probs.stride()[0], drafts_at, draft_start.data_ptr(), uniforms.data_ptr(), n,
+        v, tokens_at, accepted.data_ptr(), _stream_of(device)), "verify_drafts")
 
 
 def argmax_scratch_bytes(n_rows: int) -> int:

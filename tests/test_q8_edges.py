@@ -114,3 +114,10 @@ def test_attention_refuses_outputs_in_its_queries(fake, dtype, q_stride, out_str
     with pytest.raises(Reached) if apart else pytest.raises(KernelError, match="memory of its own"):
         ops.attention_q8(q, pages, scales, fake(2, 4, dtype=I32), 16, fake(3, dtype=I32), fake(2, dtype=I32), out, None, 2, 1, 40, 4, 2,
                          16, 0.1)
+
+
+@pytest.mark.parametrize("off,apart", [(0, False), (4, False), (-4, False), (12, True), (-20, True), (-16, False), (8, False)])
+def test_verify_refuses_tokens_in_its_drafts(fake, off, apart):
+    with pytest.raises(Reached) if apart else pytest.raises(KernelError, match="memory of its own"):
+        ops.verify_drafts(fake(5, 99), fake(3, dtype=I32, at=1 << 32), fake(3, dtype=I32), fake(5),
+                          fake(5, dtype=I32, at=(1 << 32) + off), fake(2, dtype=I32), 3)
