@@ -1280,6 +1280,8 @@ def verify_drafts(probs: torch.Tensor, drafts: torch.Tensor, draft_start: torch.
         _refuse(draft_probs, "draft_probs", torch.float32, device, f"[{k}, {v}] with contiguous rows")
     if max_drafts < 0:
         raise KernelError(f"max_drafts must not be negative, got {max_drafts}")
+    if k > n * max_drafts:
+        raise KernelError(f"{k} drafts in {n} rows: more than max_drafts {max_drafts} a row")
     if n == 0:
         return
     drafts_at, tokens_at = drafts.data_ptr(), tokens.data_ptr()

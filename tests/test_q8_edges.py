@@ -121,3 +121,14 @@ def test_verify_refuses_tokens_in_its_drafts(fake, off, apart):
     with pytest.raises(Reached) if apart else pytest.raises(KernelError, match="memory of its own"):
         ops.verify_drafts(fake(5, 99), fake(3, dtype=I32, at=1 << 32), fake(3, dtype=I32), fake(5),
                           fake(5, dtype=I32, at=(1 << 32) + off), fake(2, dtype=I32), 3)
+
+
+def test_verify_refuses_more_drafts_than_it_is_told(fake):
+    args = lambda k, n: (fake(k + n, 99), fake(k, dtype=I32), fake(n + 1, dtype=I32), fake(k + n), fake(k + n, dtype=I32),  # noqa: E731
+                         fake(n, dtype=I32))
+    for k, n, most in ((3, 2, 1), (1, 1, 0), (9, 2, 4), (1, 0, 5)):
+        with pytest.raises(KernelError, match="more than max_drafts"):
+            ops.verify_drafts(*args(k, n), most)
+    for k, n, most in ((3, 2, 2), (0, 1, 0), (8, 2, 4)):
+        with pytest.raises(Reached):
+            ops.verify_drafts(*args(k, n), most)
