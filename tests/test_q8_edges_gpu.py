@@ -164,3 +164,30 @@ def test_captured_steps_whose_longest_rows_differ(model_dirs, monkeypatch):
         assert (got - want).norm() / want.norm() < 4e-3
         assert all(max(step.values()) <= m < 2 * max(step.values()) for m in asked)
     assert runner.replayed_steps >= 4
+
+
+def test_requests_that_are_set_back_read_what_they_wrote(model_dirs):
+    """A pool so small that requests are set back and their pages used again (free ones hold NaN): every token's
+    log-probability is what the model, with room for all, says of the same tokens.  A request that comes in again stores its
+    tokens in other portions; that moves a value only where a block's scale grew in between and the value is a subnormal of it,
+    or where a 32-bit rounding lies at the border between two e4m3 numbers (one of a row's thousands, by 2^-3 of itself): some
+    thousandths of a nat for this model, where a stale scale or a wrong page moves it by units."""
+    from scratch_llm_b200 import LLM, Request, SamplingParams
+    from scratch_llm_b200.engine import ModelRunner
+    gen = torch.Generator().manual_seed(6)
+    prompts = [torch.randint(0, 256, (n,), generator=gen).tolist() for n in (30, 25, 28, 9, 33, 20)]
+    params = SamplingParams(temperature=0.0, max_tokens=40)
+    make = lambda n, **k: LLM(model_dirs["A"], dtype="float32", max_tokens=n, page_size=16, max_requests=4,  # noqa: E731
+                              cache_dtype="float8_e4m3fn", **k)
+    small, big = make(160), make(2048)
+    small.runner = ModelRunner(small.model, 16, 10, 4, poison_free_pages=True, cache_dtype="float8_e4m3fn")
+    got = small.serve([Request(i, p, params) for i, p in enumerate(prompts)], want_logprobs=True)
+    assert got.stats.preemptions > 0
+    worst = 0.0
+    for c, prompt in zip(got.completed, prompts):
+        tokens = list(c.token_ids)
+        assert len(tokens) == 40 and len(c.logprobs) == 40
+        worst = max(worst, *(abs(a - b) for a, b in zip(c.logprobs, big.score(prompt, tokens))))
+    assert worst < 0.05, worst
+    small.runner.cache.check()
+    assert not small.runner.cache.requests
