@@ -132,3 +132,12 @@ def test_verify_refuses_more_drafts_than_it_is_told(fake):
     for k, n, most in ((3, 2, 2), (0, 1, 0), (8, 2, 4)):
         with pytest.raises(Reached):
             ops.verify_drafts(*args(k, n), most)
+
+
+@pytest.mark.parametrize("new", [1, 6])
+def test_attention_of_no_tokens(fake, new):
+    """A step in which every row is empty asks for nothing (and for no workspace, which would have no address)."""
+    pages, scales = fake(8, 2, 2, 16, 16, dtype=torch.float8_e4m3fn), fake(8, 2, 2, 1, dtype=torch.float8_e8m0fnu)
+    out = fake(0, 64)
+    assert ops.attention_q8(fake(0, 64), pages, scales, fake(2, 4, dtype=I32), 16, fake(3, dtype=I32), fake(2, dtype=I32), out, None, 2,
+                            new, 40, 4, 2, 16, 0.1) is out
