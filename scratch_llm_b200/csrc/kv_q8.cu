@@ -344,6 +344,7 @@ __device__ __forceinline__ void store_32_bytes(__nv_bfloat16* to, const float* v
 // heads of 64 to 32 bits 8.2.  Two stores of 16 bytes, so that a warp's store fills halves of sectors, took 148 and 13.6,
 // pieces that become 16 bytes 143 and 10.3.  grid (pieces of a page, pages of a row, rows).
 constexpr int READ_THREADS = 256, READ_PIECES = 4;
+constexpr float BF16_MAX = 3.38953139e38f;
 template <typename T> constexpr int READ_BYTES = 32 / (int)sizeof(T);
 
 struct ReadArgs {
@@ -351,8 +352,8 @@ struct ReadArgs {
     int page_size, block, G, hd, first_row;
     // positions [row_from[r], row_to[r]) of row r through out_table, or, where row_start is given: everything that the
     // queries of the listed rows see, page p of the i-th of them to page i * listed_pages + p, which the kernel writes
-    // into out_table[r] itself (-1 where a page is not needed); a NaN becomes zero there, and odd[i * listed_pages + p,
-    // blockIdx.x] is set to whether the CTA met one
+    // into out_table[r] itself (-1 where a page is not needed); a NaN becomes zero there, what would be infinite the largest
+    // finite number, and odd[i * listed_pages + p, blockIdx.x] is set to whether the CTA met a NaN
     const int* row_from; const int* row_to;
     const int* row_start; const int* row_pos0; const int* row_list; int window, listed_pages;
     int* out_table; int out_stride; uint8_t* odd;
@@ -432,6 +433,10 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(T* __restrict_
                 v[4 * j + 2] = hi.x * power;
                 v[4 * j + 3] = hi.y * power;
             }
+            // (numbers from 2^128 on, which an infinity would stand for, would reach what does not see them as a NaN does)
+            if (listed && b[k] >= 247 && b[k] < 255)
+#pragma unroll
+                for (int j = 0; j < BYTES; ++j) v[j] = fminf(fmaxf(v[j], -BF16_MAX), BF16_MAX);
             store_32_bytes(dst + (int64_t)(c0 + k * READ_THREADS) * BYTES, v);
         }
         if (listed) {

@@ -191,3 +191,23 @@ def test_requests_that_are_set_back_read_what_they_wrote(model_dirs):
     assert worst < 0.05, worst
     small.runner.cache.check()
     assert not small.runner.cache.requests
+
+
+@pytest.mark.parametrize("portions", [False, True])
+def test_largest_values_reach_only_what_sees_them(portions, monkeypatch):
+    """The largest bfloat16 numbers are stored as 2^128, for which bfloat16 has an infinity: queries that do not see them get
+    what they get without them."""
+    from scratch_llm_b200.kernels import ops
+    monkeypatch.setattr(ops, "_attention_q8_in_16_bits", lambda *a: portions)
+    H, G, hd, page = 8, 2, 64, 16
+    rows = [(100, 60)]
+    gen = torch.Generator().manual_seed(12)
+    c = Cache(G, hd, page, 1, [160], gen).fill([(160, 0)], gen, 0.5)
+    q = torch.randn(60, H * hd, generator=gen).bfloat16()
+    clean = attend_on_device(c, q.to(DEV), rows, c.device(), H, hd ** -0.5)
+    at = int(c.table[0, 130 // page]), 130 % page
+    for plane, byte in ((0, 0x78), (1, 0xF8)):                    # 256, -256
+        c.pages[at[0], plane, 1, at[1], 7], c.scales[at[0], plane, 1, at[1]] = byte, 247
+    got = attend_on_device(c, q.to(DEV), rows, c.device(), H, hd ** -0.5)
+    assert torch.equal(got[:30], clean[:30])
+    assert torch.equal(got.view(60, H, hd)[:, :4], clean.view(60, H, hd)[:, :4])
