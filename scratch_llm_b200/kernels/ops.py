@@ -1221,7 +1221,9 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     if n_list <= 0 or max_new <= 0 or n == 0:
         return out
     q_at, out_at, q_stride, out_stride = q.data_ptr(), out.data_ptr(), q.stride()[0], out.stride()[0]
-    if not _apart(q_at, q_stride, out_at, out_stride, n, width, q.element_size()):
+    size = 2 if code else 4
+    if -n * out_stride * size < out_at - q_at < n * q_stride * size and \
+            not _apart(q_at, q_stride, out_at, out_stride, n, width, size):
         raise KernelError("out must be memory of its own: queries are read while outputs are written")
     stream = _stream_of(device)
     if code == 1 and max_new > 1 and _attention_q8_in_16_bits(device, n_list, max_new, max_context, n_heads, n_kv_heads,
