@@ -100,24 +100,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// d += a * (the sum of b's parts), for sums over all keys.  The instruction cuts its sums off towards zero, which adds up over
-// a row's keys: in the 32-bit form each product starts from nothing and is added with a rounding.  300 tokens after
-// 3,000, heads of 64: 0.7e-6 off the exact result instead of 2.1e-6 (32-bit arithmetic as written: 1.3e-6), 129 us instead
-// of 123; 24 tokens over 4,096 keys 0.7e-6 instead of 1.2e-6, 37 us either way.  (The scores' short sums likewise: 0.4e-6 in
-// both, 134 and 39 us.)
-template <int PARTS, typename B> __device__ __forceinline__ void mma_parts(float (&d)[4], const uint32_t (&a)[4], B b) {
-    if constexpr (PARTS == 1) {
-        mma_f16(d, a, b(0, 0), b(0, 1));
-    } else {
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_f16(x, a, b(1, 0), b(1, 1));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= 1.f / REST;
-        mma_f16(x, a, b(0, 0), b(0, 1));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] += x[i];
-    }
-}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {       // an 8 x 8 tile of halves
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
@@ -207,11 +189,14 @@ __device__ __noinline__ void attend_scalar(const T* __restrict__ q, const Q8Args
     }
 }
 
-// Token tok of the i-th listed row, whose first one is token t0: its place in a.part; -1: none.
-__device__ __forceinline__ int64_t part_place(const Q8Args& a, int i, int t0, int tok) {
-    const int64_t at = (a.part_new ? (int64_t)i * a.part_new : t0) + tok;
-    return (a.part_new == 0 || tok < a.part_new) && at < a.part_tokens ? at : -1;
-}
+// The place in a.part of the first token of the i-th listed row, token t0 of the step, and how many of the row's have one.
+struct PartPlace {
+    int64_t first; int tokens;
+    __device__ __forceinline__ PartPlace(const Q8Args& a, int i, int t0) {
+        first = a.part_new ? (int64_t)i * a.part_new : t0;
+        tokens = a.part_new ? a.part_new : (int)(a.part_tokens - t0);
+    }
+};
 
 // The queries of a row and kv head are packed: p = token * GS + j is the row's token `token` and query head g GS + j.  A
 // CTA takes 8 NT packed queries over a share of the keys; its warps take turns at the tiles.  (Warps that share the
@@ -258,10 +243,10 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
     const int tile_begin = min(n_tiles, split * per_split), tile_end = min(n_tiles, tile_begin + per_split);
 
     if (tile_begin >= tile_end && a.n_splits > 1 && !a.cluster) {      // no share: nothing is read or merged
+        const PartPlace place(a, blockIdx.z, t0);
         for (int i = tid; i < nq; i += THREADS) {
             const int p = q0 + i, tok = p / GS, h = g * GS + p - tok * GS;
-            const int64_t place = part_place(a, blockIdx.z, t0, tok);
-            if (place >= 0) a.part[((place * a.H + h) * a.n_splits + split) * (HD + 2) + HD + 1] = 0.f;
+            if (tok < place.tokens) a.part[(((place.first + tok) * a.H + h) * a.n_splits + split) * (HD + 2) + HD + 1] = 0.f;
         }
         return;
     }
@@ -561,10 +546,11 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
                     p[0][i][nt][k] = transposed(h);
                     if constexpr (PARTS == 2) p[1][i][nt][k] = transposed(halves_rest(y[0], y[1], h, REST));
                 }
-        // ---- sums over the keys, transposed: rows are entries of a head
-#pragma unroll
-        for (int i = 0; i < KG; ++i) {
-            uint32_t vr[4][VREGS];
+        // ---- sums over the keys, transposed: rows are entries of a head.  The instruction cuts its sums off towards zero, which adds
+        // up over a row's keys: in the 32-bit form a tile's products start from nothing, both parts by themselves, and are added
+        // with a rounding.  300 tokens after 3,000, heads of 64: 0.7e-6 off the exact result instead of 2.1e-6 (32-bit arithmetic as
+        // written: 1.3e-6).  (Product after product, each with its second part brought back, took 174 us for heads of 128; this 169.)
+        auto take_values = [&](int i, uint32_t (&vr)[4][VREGS]) {             // of keys 16 i .. 16 i + 15
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 take<HD / 8>(v_at[k & 1], (2 * i + (k >> 1)) * EIGHT, vr[k]);
@@ -572,19 +558,47 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
 #pragma unroll
                     for (int w = 0; w < VREGS; ++w) vr[k][w] = 0u;         // (a place without a key that is seen may hold a NaN)
             }
+        };
+        auto entries = [&](int j, const uint32_t (&vr)[4][VREGS], uint32_t (&f)[4]) {
+            // (bytes 0 and 1: entry 2 j of two keys, bytes 2 and 3: entry 2 j + 1)
+            constexpr uint32_t LOW = 0x5140, HIGH = 0x7362;
+            const int w = V_WORDS ? j / 2 : j;
+            const uint32_t pick = V_WORDS && (j & 1) ? HIGH : LOW;
+            const uint32_t x = __byte_perm(vr[0][w], vr[1][w], pick);
+            const uint32_t y = __byte_perm(vr[2][w], vr[3][w], pick);
+            halves_of(x, f[0], f[1]);
+            halves_of(y, f[2], f[3]);
+        };
+        if constexpr (PARTS == 1) {
+#pragma unroll
+            for (int i = 0; i < KG; ++i) {
+                uint32_t vr[4][VREGS], f[4];
+                take_values(i, vr);
+#pragma unroll
+                for (int j = 0; j < KSTEPS; ++j) {
+                    entries(j, vr, f);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_f16(o[j][nt], f, p[0][i][nt][0], p[0][i][nt][1]);
+                }
+            }
+        } else {
+            uint32_t vr[KG][4][VREGS], f[KG][4];
+#pragma unroll
+            for (int i = 0; i < KG; ++i) take_values(i, vr[i]);
 #pragma unroll
             for (int j = 0; j < KSTEPS; ++j) {
-                // (bytes 0 and 1: entry 2 j of two keys, bytes 2 and 3: entry 2 j + 1)
-                constexpr uint32_t LOW = 0x5140, HIGH = 0x7362;
-                const int w = V_WORDS ? j / 2 : j;
-                const uint32_t pick = V_WORDS && (j & 1) ? HIGH : LOW;
-                const uint32_t x = __byte_perm(vr[0][w], vr[1][w], pick);
-                const uint32_t y = __byte_perm(vr[2][w], vr[3][w], pick);
-                uint32_t f[4];
-                halves_of(x, f[0], f[1]);
-                halves_of(y, f[2], f[3]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_parts<PARTS>(o[j][nt], f, [&](int part, int k) { return p[part][i][nt][k]; });
+                for (int i = 0; i < KG; ++i) entries(j, vr[i], f[i]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float x[PARTS][4] = {};
+#pragma unroll
+                    for (int i = 0; i < KG; ++i)
+#pragma unroll
+                        for (int part = 0; part < PARTS; ++part) mma_f16(x[part], f[i], p[part][i][nt][0], p[part][i][nt][1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][nt][e] += fmaf(x[PARTS - 1][e], 1.f / REST, x[0][e]);
+                }
             }
         }
         __syncwarp();                     // (the tile is read)
@@ -625,6 +639,7 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         const int p = q0 + i, tok = p / GS, h = g * GS + p - tok * GS;
         out[(int64_t)(t0 + tok) * a.out_stride + (int64_t)h * HD + d] = from_float<T>(total == 0.f ? 0.f : sum / total);
     };
+    const PartPlace place(a, blockIdx.z, t0);
     auto leave = [&](int i, int d, float sum, float top, float total) {
         const int p = q0 + i, tok = p / GS, h = g * GS + p - tok * GS;
         if (a.n_splits == 1) {
@@ -632,8 +647,8 @@ attn_q8_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_consta
         } else if (a.cluster) {
             sums[i * LD + d] = sum;                      // (query i's place of the first warp)
             if (d == 0) { all_top[i] = top; all_total[i] = total; }
-        } else if (const int64_t place = part_place(a, blockIdx.z, t0, tok); place >= 0) {
-            float* part = a.part + ((place * a.H + h) * a.n_splits + split) * (HD + 2);
+        } else if (tok < place.tokens) {
+            float* part = a.part + (((place.first + tok) * a.H + h) * a.n_splits + split) * (HD + 2);
             part[d] = sum;
             if (d == 0) { part[HD] = top; part[HD + 1] = total; }
         }
@@ -704,9 +719,10 @@ __global__ void __launch_bounds__(THREADS) attn_q8_merge_kernel(T* __restrict__ 
     pdl_trigger();
     const int r = a.row_list ? a.row_list[blockIdx.y] : blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tok = blockIdx.x / a.H, h = blockIdx.x - tok * a.H, t0 = a.row_start[r];
-    const int64_t ld = HD + 2, place = part_place(a, blockIdx.y, t0, tok);
-    if (tok >= a.row_start[r + 1] - t0 || place < 0) return;
-    const float* part = a.part + (place * a.H + h) * a.n_splits * ld;
+    const PartPlace place(a, blockIdx.y, t0);
+    if (tok >= a.row_start[r + 1] - t0 || tok >= place.tokens) return;
+    const int64_t ld = HD + 2;
+    const float* part = a.part + ((place.first + tok) * a.H + h) * a.n_splits * ld;
     float top = LOWEST, total = 0.f, sum[DPL];
     // (a total of zero: a share without a key)
     for (int k = lane; k < a.n_splits; k += 32)
