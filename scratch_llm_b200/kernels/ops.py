@@ -1222,7 +1222,7 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
         return out
     q_at, out_at, q_stride, out_stride = q.data_ptr(), out.data_ptr(), q.stride()[0], out.stride()[0]
     size = 2 if code else 4
-    if -n * out_stride * size < out_at - q_at < n * q_stride * size and \
+    if -((n - 1) * out_stride + width) * size < out_at - q_at < ((n - 1) * q_stride + width) * size and \
             not _apart(q_at, q_stride, out_at, out_stride, n, width, size):
         raise KernelError("out must be memory of its own: queries are read while outputs are written")
     stream = _stream_of(device)

@@ -92,6 +92,7 @@ def fake(monkeypatch):
         placed.append((t, at if at is not None else (len(placed) + 1) << 24))
         return t
 
+    make.placed = placed
     with FakeTensorMode():
         yield make
 
@@ -114,6 +115,20 @@ def test_attention_refuses_outputs_in_its_queries(fake, dtype, q_stride, out_str
     with pytest.raises(Reached) if apart else pytest.raises(KernelError, match="memory of its own"):
         ops.attention_q8(q, pages, scales, fake(2, 4, dtype=I32), 16, fake(3, dtype=I32), fake(2, dtype=I32), out, None, 2, 1, 40, 4, 2,
                          16, 0.1)
+
+
+@pytest.mark.parametrize("rows,q_row,out_row,off,apart", [(1, 0, 0, 0, False), (1, 0, 64, 32, False), (1, 0, 0, 64, True), (5, 0, 64, 0, False),
+                                                          (5, 0, 64, 64, True), (1, 1, 1, -63, False), (1, 1, 1, -64, True)])
+def test_attention_refuses_outputs_in_queries_that_all_rows_share(fake, rows, q_row, out_row, off, apart):
+    """Rows that are one (a stride of 0), and a single row, whose stride says nothing."""
+    pages, scales = fake(8, 2, 2, 16, 16, dtype=torch.float8_e4m3fn), fake(8, 2, 2, 1, dtype=torch.float8_e8m0fnu)
+    views = []
+    for row, at in ((q_row, 1 << 32), (out_row, (1 << 32) + 4 * off)):
+        views.append(torch.empty(64 * rows, dtype=F32, device="cuda").as_strided((rows, 64), (row, 1)))
+        fake.placed.append((views[-1], at))
+    with pytest.raises(Reached) if apart else pytest.raises(KernelError, match="memory of its own"):
+        ops.attention_q8(views[0], pages, scales, fake(2, 4, dtype=I32), 16, fake(3, dtype=I32), fake(2, dtype=I32), views[1], None, 2, 1,
+                         40, 4, 2, 16, 0.1)
 
 
 @pytest.mark.parametrize("off,apart", [(0, False), (4, False), (-4, False), (12, True), (-20, True), (-16, False), (8, False)])
