@@ -152,7 +152,7 @@ __device__ __forceinline__ int row_of(const WriteArgs& a, int n) { return last_r
 // queries: 42 us (29 at the copy rate; 46 where every unit asks for a bias); 1,581 tokens of 3 x 40 heads, blocks of 64,
 // in 32 bits with biases: 38 (22); eight rows of one token 2.5.  With the block in registers 49, 60 and 3.0; with a CTA a
 // block and a thread's unit in several heads 45, 36 and 2.9, but up to 60 % more where rows fill parts of blocks.  The
-// queries stream (26 us alone); the blocks' CTAs are bound by instruction issue, so that the two parts' times add up in
+// queries stream (24.5 us alone); the blocks' CTAs are bound by instruction issue, so that the two parts' times add up in
 // whichever order their CTAs start.
 // Row r has the slots from row_start[r] / block + 2 r on, at least as many as it touches blocks: n new tokens touch at
 // most n / block + 2.  The other CTAs turn the queries.

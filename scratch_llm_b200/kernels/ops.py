@@ -1018,7 +1018,9 @@ def rope_kv_write_q8(qkv: torch.Tensor, row_start: torch.Tensor, row_pos0: torch
     ``scales`` float8_e8m0fnu [n_pages, 2, G, page_size / block]: one power of two per block of tokens, the smallest
     with which the block's largest finite value is at most 448.  Row r brings the tokens ``row_start[r]`` to
     ``row_start[r + 1] - 1`` (at most ``max_new``), at the positions from ``row_pos0[r]`` on; a block in which the row has
-    earlier tokens keeps its scale or takes a larger one, at which the earlier tokens' numbers are rounded again.
+    earlier tokens keeps its scale or takes a larger one, at which the earlier tokens' numbers are rounded again.  It never takes a
+    smaller one: a drafted token that is refused and written over leaves its block's scale, and that second rounding, behind,
+    which only blocks of one token rule out.
     Infinities and NaN are stored as NaN.  Two rows of a step share no block.  Tables of fewer than ``head_dim / 2``
     columns rotate only the first ``2 * columns`` entries of a head; ``cos`` None rotates nothing."""
     device, dtype = _device(), qkv.dtype
@@ -1109,7 +1111,7 @@ def _attention_q8_plan(device: int, head_dim: int, code: int, n_list: int, max_n
     """How a launch is shared out: (queries of a CTA / 8, CTAs along the keys, 1 where these are a cluster that merges by
     itself, else 2 where all CTAs fit and 0 where they do not).  Sixteen queries a CTA where that leaves few places empty and
     there is work to fill the device: 16 ragged rows of 32 packed queries after up to 4,000 tokens 65 us against 74, 300
-    tokens of 32 bits after 3,000 168 against 189; 4 rows of 32 after 300 14.8 against 10.4.  The number of CTAs along the keys is the one with the least cost in turns of a warp (a
+    tokens of 32 bits after 3,000 169 against 191; 4 rows of 32 after 300 14.8 against 10.4.  The number of CTAs along the keys is the one with the least cost in turns of a warp (a
     tile): a CTA costs 1.5 turns beside its own, launches of more CTAs than fit take between the whole and the
     fractional number of rounds, a cluster merges in 1.8 turns and more where the device is nearly full of clusters, a
     kernel of its own in 4.9.  The numbers are those with which 215 launches (1 to 64 rows of 300 to 16,000 keys, even and
@@ -1195,8 +1197,10 @@ def attention_q8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, blo
     """Causal attention of the listed rows (all ``n_list`` of them in order for ``row_list`` None) over a cache held in 8
     bits (:func:`rope_kv_write_q8`), for single tokens, drafted tokens and portions of prompts alike.  ``q`` [N, H * hd] may be
     a column slice; bfloat16 or float32, and ``out`` likewise.  No row brings more than ``max_new`` tokens, and no query
-    stands at a position of ``max_context`` or more.  A listed row may be empty or listed twice, but ``row_start``,
-    ``row_pos0`` and ``block_table`` have to hold it."""
+    stands at a position of ``max_context`` or more: launches are planned by both bounds, so they should be close.  A listed row
+    may be empty or listed twice, but ``row_start``, ``row_pos0`` and ``block_table`` have to hold it.  A NaN in the cache reaches
+    the queries that see it and no other.  ``out`` shares no memory with ``q`` (columns side by side may).  In float32
+    queries and probabilities are multiplied as numbers of 22 bits."""
     device, dtype, shape, width = _device(), q.dtype, q.shape, n_heads * head_dim
     code, n = _code(dtype), shape[0] if shape else 0
     block = _q8_cache(pages, scales, n_kv_heads, page_size, head_dim, device)

@@ -211,3 +211,31 @@ def test_largest_values_reach_only_what_sees_them(portions, monkeypatch):
     got = attend_on_device(c, q.to(DEV), rows, c.device(), H, hd ** -0.5)
     assert torch.equal(got[:30], clean[:30])
     assert torch.equal(got.view(60, H, hd)[:, :4], clean.view(60, H, hd)[:, :4])
+
+
+@pytest.mark.parametrize("block", [1, 16])
+def test_refused_drafts_leave_no_trace_in_blocks_of_one_token(block):
+    """Loud drafts are stored, refused and written over: in blocks of one token the cache then holds what it holds without them; in
+    larger ones a block keeps its scale, and no value of its earlier tokens moves by more than half a step of it."""
+    from test_q8_cache_gpu import write_on_device
+    H, G, hd, page = 2, 1, 64, 16
+    gen = torch.Generator().manual_seed(2)
+    c = Cache(G, hd, page, block, [40], gen)
+    tokens = torch.randn(26, (H + 2 * G) * hd, generator=gen).bfloat16()
+    loud = 3000.0 * torch.randn(4, (H + 2 * G) * hd, generator=gen).bfloat16()
+    plainly, drafted = c.device(), c.device()
+    write_on_device(c, tokens[:21], [(0, 21)], None, None, H, True, plainly)
+    write_on_device(c, tokens[:21], [(0, 21)], None, None, H, True, drafted)
+    write_on_device(c, loud, [(21, 4)], None, None, H, True, drafted)
+    for dev in (plainly, drafted):
+        write_on_device(c, tokens[21:], [(21, 5)], None, None, H, True, dev)
+    held = [(dev[0].view(torch.uint8).cpu(), dev[1].view(torch.uint8).cpu()) for dev in (plainly, drafted)]
+    a, b = (plain.values(*x, c.table[0], 26, page) for x in held)
+    if block == 1:
+        assert torch.equal(a, b)
+    else:
+        assert torch.equal(a[:, :16], b[:, :16])
+        unit = plain.power(held[1][1][c.table[0].long()]).permute(1, 0, 3, 2).reshape(2, -1, G).repeat_interleave(block, 1)[:, :26]
+        # (a first rounding to 2^-4 of the value at most on either side, or half a step of subnormals)
+        assert ((a - b).abs() <= 2.0 ** -10 * unit[..., None] + 2.0 ** -3 * a.abs()).all()
+        assert not torch.equal(held[0][1], held[1][1])
